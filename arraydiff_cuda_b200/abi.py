@@ -70,6 +70,27 @@ class FilterItem(C.Structure):
                 ("K", u32), ("C", u32), ("kh", u32), ("kw", u32), ("crsk_k", u32), ("reserved", u32)]
 
 
+class LogprobArgs(C.Structure):
+    _fields_ = [
+        ("dtype", i32), ("layout", i32), ("N", u32), ("C", u32), ("HW", u32), ("scale", f32),
+        ("logits", vp), ("pitch", i64), ("label", vp),
+        ("lse", vp), ("entropy", vp), ("logp", vp), ("rank", vp),
+        ("top", u32), ("reserved", u32), ("top_class", vp), ("top_logp", vp),
+        ("dlse", vp), ("dentropy", vp), ("dlogp", vp),
+        ("dlogits", vp), ("dlogits_pitch", i64), ("accumulate", i32), ("reserved_tail", i32),
+    ]
+
+
+class DistillArgs(C.Structure):
+    _fields_ = [
+        ("dtype", i32), ("layout", i32), ("N", u32), ("C", u32), ("HW", u32), ("scale", f32),
+        ("logits", vp), ("pitch", i64), ("top", u32), ("rest", i32),
+        ("top_class", vp), ("top_logit", vp), ("top_lse", vp), ("top_scale", f32), ("reserved", u32),
+        ("loss", vp), ("dloss", vp),
+        ("dlogits", vp), ("dlogits_pitch", i64), ("accumulate", i32), ("reserved_tail", i32),
+    ]
+
+
 class ConvProfileEntry(C.Structure):
     _fields_ = [("pass_", i32), ("kernel", i32), ("status", i32),
                 ("N", u32), ("C", u32), ("H", u32), ("W", u32), ("K", u32), ("kh", u32), ("kw", u32),
@@ -111,6 +132,10 @@ SIGNATURES = {
     "ad_softmax_nll_loss_bwd": (C.c_int, [u32, u32, vp, vp, vp, vp, vp]),
     "ad_softmax_ce_pixel_fwd": (C.c_int, [i32, i32, u32, u32, u32, vp, vp, vp, vp, vp]),
     "ad_softmax_ce_pixel_bwd": (C.c_int, [i32, i32, u32, u32, u32, vp, vp, vp, vp, i32, vp]),
+    "ad_logprob_fwd": (C.c_int, [C.POINTER(LogprobArgs), vp]),
+    "ad_logprob_bwd": (C.c_int, [C.POINTER(LogprobArgs), vp]),
+    "ad_distill_fwd": (C.c_int, [C.POINTER(DistillArgs), vp]),
+    "ad_distill_bwd": (C.c_int, [C.POINTER(DistillArgs), vp]),
     "ad_bn_scratch_bytes": (sz, [u32]),
     "ad_bn_fwd_train": (C.c_int, [C.POINTER(Tensor4), C.POINTER(Tensor4), vp, vp, vp, vp, vp, f32, i32, vp, sz, vp]),
     "ad_bn_fwd_train_noalloc": (C.c_int, [C.POINTER(Tensor4), C.POINTER(Tensor4), vp, vp, vp, vp, vp, f32, i32, vp]),

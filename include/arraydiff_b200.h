@@ -246,6 +246,88 @@ int ad_softmax_ce_pixel_bwd(int32_t dtype, int32_t layout, uint32_t N, uint32_t 
                             const void* logits, const uint32_t* label, const float* dloss, void* dlogits,
                             int32_t accumulate, void* stream);
 
+/*
+ * Log probabilities over any number of classes: of a given class, with the entropy, the class's rank and the top
+ * alternatives of every row.  No counterpart in the reference.  A row is one position: logits [N][HW][C] (AD_NHWC; HW = 1
+ * for a [rows][classes] matrix) or [N][C][HW] (AD_NCHW), rows numbered n * HW + t, and everything else lies by rows.
+ * `pitch` (elements; 0 = packed) is the distance between positions (NHWC, >= C) or between class planes (NCHW, >= HW).
+ *   z = scale * logits (1 / temperature, in [1e-30, 1e30]), lse = logsumexp_c z, p = exp(z - lse)
+ *   fwd (each result is written where its pointer is not NULL):
+ *     lse, entropy = -sum p log p, logp = z[label] - lse,
+ *     rank = number of classes in front of the label by (logit descending, class ascending): top-k accuracy is rank < k,
+ *     top_class / top_logp [rows][top]: the first `top` <= 128 classes in that order and their log probabilities.
+ *   bwd: dlogits (+)= the gradient of  sum_rows dlse * lse + dentropy * entropy + dlogp * logp  (a NULL factor is zero, one
+ *     at least is given); accumulate != 0 adds.  The statistics are worked out anew, nothing is kept from fwd; lse, entropy
+ *     and logp are written here too where their pointers are not NULL (a training step whose factors are known beforehand is
+ *     this call alone); rank and top are fwd's.
+ * A label >= C is no class: its logp is 0, its rank 0xffffffff, and no gradient comes from its dlogp.  Places of a list
+ * behind the last class (top > C) hold class 0xffffffff and -inf.  A row whose logits are all -inf has lse = -inf,
+ * entropy 0, log probabilities of -inf and a gradient of zero.  A row that holds NaN or +inf has NaN for all computed
+ * numbers; a NaN is no candidate for a list and counts in no rank.  Equal logits (-0 and 0 too) rank by class.
+ * dlogits may be logits itself (same pitch, accumulate 0); any other meeting of their extents is AD_ERR_BAD_ARG.
+ * Sums run in a fixed order: the same call gives the same bits.  C <= 2^30.
+ */
+typedef struct {
+  int32_t dtype, layout;
+  uint32_t N, C, HW;
+  float scale;
+  const void* logits;
+  int64_t pitch;
+  const uint32_t* label;    /* [N*HW], or NULL where neither logp, rank nor dlogp is asked for */
+  float *lse, *entropy, *logp;
+  uint32_t* rank;           /* fwd */
+  uint32_t top, reserved;   /* fwd */
+  uint32_t* top_class;      /* fwd; [N*HW][top] */
+  float* top_logp;          /* fwd; [N*HW][top] */
+  const float *dlse, *dentropy, *dlogp; /* bwd */
+  void* dlogits;            /* bwd; dtype and layout of logits */
+  int64_t dlogits_pitch;    /* bwd; 0 = packed */
+  int32_t accumulate;       /* bwd */
+  int32_t reserved_tail;
+} ad_logprob_args;
+int ad_logprob_fwd(const ad_logprob_args* args, void* stream);
+int ad_logprob_bwd(const ad_logprob_args* args, void* stream);
+
+/*
+ * Distillation from a teacher's top classes.  No counterpart in the reference.  Rows, layouts, pitch and scale as above;
+ * p = softmax(scale * logits) is the student.  The teacher's list of a row is `top` <= 128 classes and numbers t:
+ *   rest == 0: q = softmax over the list of top_scale * t;
+ *   rest != 0: q_j = exp(top_scale * t_j - top_lse[row]) (top_lse NULL: 0), and q_r = max(0, 1 - sum q) for all classes
+ *     outside of the list together, whose probability is p_r.  Lists of ad_logprob_fwd: top_scale = 1, top_lse = NULL with
+ *     top_logp; top_scale = 1 / temperature and its logsumexp with logits.
+ *   loss[row] = sum_j q_j (log q_j - log p[class_j]) + q_r (log q_r - log p_r)
+ *   dlogits (+)= dloss[row] * d loss / d logits = dloss * scale * (p_c (sum q + q_r) - sum_{class_j = c} q_j, and
+ *     - q_r p_c / p_r where c is outside of the list)
+ * fwd writes loss; bwd writes dlogits, and loss too where its pointer is not NULL (a training step is this call alone).
+ * An entry whose class is >= C is no entry; a class that stands twice counts twice.  The classes outside of the list are left
+ * out (q_r = 0) where they have no probability at all: a list of all classes, or all others masked by -inf.  A class with
+ * q = 0 adds nothing, whatever the student; one that the student masks and the teacher does not gives a loss of +inf and
+ * the gradient above.  A row of the student that is all -inf has loss 0 and gradient 0.  NaN or +inf among the student's
+ * logits gives NaN.  dlogits as for ad_logprob_bwd.  Fixed orders of sums; C <= 2^30.
+ */
+typedef struct {
+  int32_t dtype, layout;
+  uint32_t N, C, HW;
+  float scale;
+  const void* logits;
+  int64_t pitch;
+  uint32_t top;
+  int32_t rest;
+  const uint32_t* top_class; /* [N*HW][top] */
+  const float* top_logit;    /* [N*HW][top] */
+  const float* top_lse;      /* [N*HW] or NULL; rest != 0 */
+  float top_scale;           /* in [1e-30, 1e30] */
+  uint32_t reserved;
+  float* loss;               /* [N*HW]; bwd: may be NULL */
+  const float* dloss;        /* bwd; [N*HW] */
+  void* dlogits;             /* bwd; dtype and layout of logits */
+  int64_t dlogits_pitch;     /* bwd; 0 = packed */
+  int32_t accumulate;        /* bwd */
+  int32_t reserved_tail;
+} ad_distill_args;
+int ad_distill_fwd(const ad_distill_args* args, void* stream);
+int ad_distill_bwd(const ad_distill_args* args, void* stream);
+
 /* ------------------------------------------------------------------------------------------
  * Strided 4-D tensor view used by the normalisation / pooling / conversion kernels.
  * Element (n, c, y, x) lives at base + n*sn + c*sc + y*sy + x*sx (strides in ELEMENTS), so one
