@@ -1,9 +1,13 @@
 // Rows of logits: what the log-probability and the distillation kernels share.
 //
-// A row's numbers are worked out in units of log 2: with m the row's maximum, cs = scale * log2(e) and u_c = (x_c - m) * cs,
-//   S = sum 2^u_c,   log2 p_c = u_c - log2 S,   lse = scale * m + ln2 * log2 S,
-//   entropy = ln2 * (log2 S - sum 2^u_c u_c / S).
-// A row of -inf takes m = 0: every term is 0 and so is S, which is how it is recognised afterwards.
+// A row's numbers are worked out in units of log 2: with m the row's maximum, cs = scale * log2(e), mc = m * cs as rounded,
+//   u_c = x_c * cs - mc (one FMA),   S = sum 2^u_c,   E = sum 2^u_c u_c,   p_c = 2^u_c / S,
+//   entropy = ln2 (log2 S - E / S),   log p_c = scale (x_c - m) - ln2 (log2 S + (mc - m * cs)),
+// where mc - m * cs, the rounding of mc, is what an FMA gives.  One pass over the row: a thread keeps its own maximum,
+// and S and E against it, and rescales them when the maximum of a batch of loads is larger.
+// A reference is at least kFloor, so that a share of -inf or of the type's lowest value adds 2^-inf = 0 and no inf - inf.
+// Rows that this does not serve (a maximum beyond +-1e36 in units of log 2, +inf, NaN) are done again by plain loops
+// over x_c - m.  A row of -inf has S = 0, which is how it is recognised.
 #pragma once
 
 #include "common.cuh"
@@ -14,6 +18,7 @@ constexpr float kLn2 = 0.693147180559945309f;
 constexpr double kLog2e = 1.442695040888963407;
 constexpr uint32_t kMostTop = 128;                 // entries of a row's list
 constexpr uint32_t kNoClass = 0xffffffffu;
+constexpr float kFloor = -1e37f, kFar = 1e36f;
 
 // Where the rows lie: row r's class c is at offset(r) + c * step (elements)
 struct Rows {
@@ -68,8 +73,235 @@ __device__ __forceinline__ float exp2_fast(float v) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));   // 2 ulp; -inf gives 0
   return r;
 }
+// v, not below -200 (2^-200 is 0 here), and NaN where v is: what may be multiplied by its exponential
+__device__ __forceinline__ float above_nothing(float v) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(v), "f"(-200.f));
+  return r;
+}
 
 // In front of: the larger value, then the lower class
 __device__ __forceinline__ bool in_front(float v, uint32_t c, float w, uint32_t d) { return v > w || (v == w && c < d); }
+// The same order as whole numbers.  -0 and 0 are one value.
+__device__ __forceinline__ uint32_t value_key(float v) {
+  const uint32_t b = __float_as_uint(v + 0.f);
+  return b ^ (b >> 31 ? 0xffffffffu : 0x80000000u);
+}
+__device__ __forceinline__ float key_value(uint32_t k) { return __uint_as_float(k ^ (k >> 31 ? 0x80000000u : 0xffffffffu)); }
+typedef unsigned long long Key;   // value, then the complement of the class; 0: none
+__device__ __forceinline__ Key key_of(float v, uint32_t c) { return (Key)value_key(v) << 32 | (uint32_t)~c; }
+__device__ __forceinline__ uint32_t key_class(Key k) { return ~(uint32_t)k; }
+
+// ---- threads that work on one row: a warp, or a block of 256 with `red` (10 words of shared memory)
+template <int NT> struct Group;
+template <> struct Group<32> {
+  uint32_t tid = threadIdx.x & 31;
+  __device__ explicit Group(void*) {}
+  __device__ void sync() { __syncwarp(); }
+  __device__ float max(float v) { return warp_max(v); }
+  __device__ float sum(float v) { return warp_sum(v); }
+  __device__ uint32_t sum(uint32_t v) { return __reduce_add_sync(0xffffffffu, v); }
+  __device__ Key max(Key v) {
+    const uint32_t h = __reduce_max_sync(0xffffffffu, (uint32_t)(v >> 32));
+    const uint32_t l = __reduce_max_sync(0xffffffffu, (uint32_t)(v >> 32) == h ? (uint32_t)v : 0u);
+    return (Key)h << 32 | l;
+  }
+};
+constexpr int kRowThreads = 256, kRowWarps = kRowThreads / 32;
+template <> struct Group<kRowThreads> {
+  uint32_t tid = threadIdx.x;
+  Key* red;   // one per warp
+  __device__ explicit Group(void* r) : red((Key*)r) {}
+  __device__ void sync() { __syncthreads(); }
+  template <typename V, typename F>
+  __device__ V all(V w, F f) {   // of the warps' values, in order
+    __syncthreads();
+    if ((tid & 31) == 0) *(V*)&red[tid >> 5] = w;
+    __syncthreads();
+    V v = *(V*)&red[0];
+#pragma unroll
+    for (int i = 1; i < kRowWarps; ++i) v = f(v, *(V*)&red[i]);
+    return v;
+  }
+  __device__ float max(float v) { return all(warp_max(v), [](float a, float b) { return fmaxf(a, b); }); }
+  __device__ float sum(float v) { return all(warp_sum(v), [](float a, float b) { return a + b; }); }
+  __device__ uint32_t sum(uint32_t v) { return all(__reduce_add_sync(0xffffffffu, v), [](uint32_t a, uint32_t b) { return a + b; }); }
+  __device__ Key max(Key v) { return all(Group<32>(nullptr).max(v), [](Key a, Key b) { return a > b ? a : b; }); }
+};
+
+// ---- 16 bytes of a row
+template <typename T> struct Vec;
+template <> struct Vec<float> {
+  static constexpr int V = 4;
+  typedef float Max;
+  __device__ static uint4 none() { return make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u); }
+  __device__ static void unpack(uint4 w, float* f) {
+    f[0] = __uint_as_float(w.x); f[1] = __uint_as_float(w.y); f[2] = __uint_as_float(w.z); f[3] = __uint_as_float(w.w);
+  }
+  __device__ static uint4 pack(const float* f) {
+    return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+  }
+  __device__ static Max max(uint4 w) {
+    float f[4];
+    unpack(w, f);
+    return fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3]));
+  }
+  __device__ static Max max(Max a, Max b) { return fmaxf(a, b); }
+  __device__ static float value(Max a) { return a; }
+  __device__ static uint32_t above(uint4 w, float t) {
+    return (__uint_as_float(w.x) > t) + (__uint_as_float(w.y) > t) + (__uint_as_float(w.z) > t) + (__uint_as_float(w.w) > t);
+  }
+  __device__ static float below(float v) {   // the next lower number
+    const uint32_t b = __float_as_uint(v);
+    return __uint_as_float((b << 1) == 0 ? 0x80000001u : b >> 31 ? b + 1 : b - 1);
+  }
+  static constexpr int kKeyShift = 0;   // low bits of a value's key that say nothing
+};
+template <> struct Vec<__nv_bfloat16> {
+  static constexpr int V = 8;
+  typedef __nv_bfloat162 Max;
+  __device__ static __nv_bfloat162 two(uint32_t w) { return *reinterpret_cast<const __nv_bfloat162*>(&w); }
+  __device__ static uint4 none() { return make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u); }
+  __device__ static void unpack(uint4 w, float* f) {
+    const uint32_t* p = &w.x;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { f[2 * i] = __uint_as_float(p[i] << 16); f[2 * i + 1] = __uint_as_float(p[i] & 0xffff0000u); }
+  }
+  __device__ static uint4 pack(const float* f) {
+    uint4 w;
+    uint32_t* p = &w.x;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+      p[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    return w;
+  }
+  __device__ static Max max(uint4 w) { return __hmax2(__hmax2(two(w.x), two(w.y)), __hmax2(two(w.z), two(w.w))); }
+  __device__ static Max max(Max a, Max b) { return __hmax2(a, b); }
+  __device__ static float value(Max a) { return fmaxf(__low2float(a), __high2float(a)); }
+  __device__ static uint32_t above(uint4 w, float t) {
+    const __nv_bfloat162 tt = __float2bfloat162_rn(t);
+    // masks of 0xffff: with a set in the low halves and b in the high ones the sum is -a + ((a - b) << 16)
+    const uint32_t s = __hgt2_mask(two(w.x), tt) + __hgt2_mask(two(w.y), tt) + __hgt2_mask(two(w.z), tt) + __hgt2_mask(two(w.w), tt);
+    const uint32_t a = (0u - s) & 0xffffu;
+    return a + ((a - ((s + a) >> 16)) & 0xffffu);
+  }
+  __device__ static float below(float v) {
+    const uint32_t b = __float_as_uint(v);
+    return __uint_as_float((b << 1) == 0 ? 0x80010000u : b >> 31 ? b + 0x10000u : b - 0x10000u);
+  }
+  static constexpr int kKeyShift = 16;
+};
+
+// A row as single elements up to a 16-byte boundary, vectors, and single elements behind them; of a row that the blocks of a
+// cluster share, the vectors [vb, ve), the elements in front with the first block, those behind with the last.
+template <typename T>
+struct Strip {
+  static constexpr uint32_t V = Vec<T>::V;
+  uint32_t head, nv, tail, vb, ve;
+  bool first, last;
+  __device__ Strip(const T* x, uint32_t C, uint32_t part = 0, uint32_t parts = 1) {
+    head = (uint32_t)((0u - (uint32_t)(uintptr_t)x) & 15u) / (uint32_t)sizeof(T);
+    if (head > C) head = C;
+    nv = (C - head) / V;
+    tail = C - head - nv * V;
+    vb = (uint32_t)((uint64_t)nv * part / parts);
+    ve = (uint32_t)((uint64_t)nv * (part + 1) / parts);
+    first = part == 0;
+    last = part + 1 == parts;
+  }
+  __device__ uint32_t class_of(uint32_t v) const { return head + v * V; }
+  // the single elements, at most 2 V - 2 of them: thread i has its i-th, or none
+  __device__ uint32_t single(uint32_t i) const {
+    if (i < V) return first && i < head ? i : kNoClass;
+    return last && i - V < tail ? head + nv * V + (i - V) : kNoClass;
+  }
+  __device__ uint32_t begin() const { return first ? 0u : class_of(vb); }
+  __device__ uint32_t end() const { return last ? head + nv * V + tail : class_of(ve); }
+};
+
+// What a thread, a group or a block of a cluster knows about its share of a row
+struct Part {
+  float m, mc, S, E;
+  uint32_t cnt;
+  __device__ void clear() { m = -INFINITY; mc = kFloor; S = E = 0.f; cnt = 0; }
+  __device__ static float reference(float m, float cs) { return fmaxf(m * cs, kFloor); }
+  template <bool ENT> __device__ void refer(float mcn) {   // S and E against a larger reference
+    const float d = mc - mcn, f = exp2_fast(d);
+    if (ENT) E = (E + d * S) * f;
+    S *= f;
+    mc = mcn;
+  }
+  template <bool ENT> __device__ void add(float x, float cs) {
+    if (x > m) {
+      m = x;
+      refer<ENT>(reference(m, cs));
+    }
+    const float u = ENT ? above_nothing(fmaf(x, cs, -mc)) : fmaf(x, cs, -mc), e = exp2_fast(u);
+    S += e;
+    if (ENT) E = fmaf(e, u, E);
+  }
+  template <bool ENT> __device__ void join(const Part& o) {   // the same bits whichever of the two is asked
+    m = fmaxf(m, o.m);
+    cnt += o.cnt;
+    const float mcn = fmaxf(mc, o.mc);
+    Part q = o;
+    refer<ENT>(mcn);
+    q.refer<ENT>(mcn);
+    S += q.S;
+    if (ENT) E += q.E;
+  }
+  template <bool ENT> __device__ void join_lanes() {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      Part q;
+      q.m = __shfl_xor_sync(0xffffffffu, m, o);
+      q.mc = __shfl_xor_sync(0xffffffffu, mc, o);
+      q.S = __shfl_xor_sync(0xffffffffu, S, o);
+      q.E = ENT ? __shfl_xor_sync(0xffffffffu, E, o) : 0.f;
+      q.cnt = 0;
+      join<ENT>(q);
+    }
+    cnt = __reduce_add_sync(0xffffffffu, cnt);
+  }
+  // not for the fast pass: beyond the range of its products, or not a number
+  __device__ bool strange(float cs) const { return S != S || fabsf(m * cs) > kFar && m != -INFINITY; }
+};
+
+// What the row's results are made of
+struct RowSums {
+  float m, mc, S, L, low;   // L = log2 S; low = L + (mc - m * cs)
+  bool some;
+  __device__ void set(float m_, float mc_, float S_, float cs) {
+    m = m_; mc = mc_; S = S_;
+    some = S != 0.f;
+    L = some ? log2f(S) : 0.f;
+    low = some ? L + fmaf(-m, cs, mc) : 0.f;
+  }
+  __device__ float log_p(float x, float scale) const { return some ? (x - m) * scale - kLn2 * low : -INFINITY; }
+  __device__ float lse(float scale) const { return some ? m * scale + kLn2 * low : -INFINITY; }
+};
+
+// Plain loops over a row in any layout: what the fast pass does not serve
+template <typename G, typename T, bool ENT>
+__device__ void plain_sums(G& g, const T* x, int64_t st, uint32_t C, float cs, RowSums& s, float& E) {
+  const uint32_t NT = sizeof(G) == sizeof(Group<32>) ? 32 : kRowThreads;
+  float m = -INFINITY, S = 0.f;
+  for (uint32_t c = g.tid; c < C; c += NT) m = fmaxf(m, ld_f(x + c * st));
+  m = g.max(m);
+  if (m == -INFINITY) m = 0.f;
+  E = 0.f;
+  for (uint32_t c = g.tid; c < C; c += NT) {
+    const float u = (ld_f(x + c * st) - m) * cs, e = exp2_fast(u);
+    S += e;
+    if (ENT && e > 0.f) E += e * u;
+  }
+  S = g.sum(S);
+  if (ENT) E = g.sum(E);
+  s.m = m; s.mc = 0.f; s.S = S;
+  s.some = S != 0.f;
+  s.low = s.L = s.some ? log2f(S) : 0.f;
+}
 
 }  // namespace adk
