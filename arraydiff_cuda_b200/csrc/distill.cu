@@ -1,5 +1,15 @@
 // Distillation from a teacher's top classes: the loss and its gradient.
+//
+// Bytes of the logits, read once (backward: once more out of the L2 or L1, and the gradient written).  The gradient of a
+// class outside of the list is dloss * scale * p_c * (Q - q_r / p_r), which the group writes everywhere; the list's logits
+// are read before, and their gradients written over that.  With rest the pass over the row leaves the list's classes out
+// (a byte of mask per vector in shared memory) and sums the others alone, against their own maximum: p_r is then exact
+// however little of the row it is, and the row's sum is theirs and that of the list, each class of it once.
+#include <cooperative_groups.h>
+
 #include "rows.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace adk {
 
@@ -18,133 +28,380 @@ struct DistillP {
   int accumulate;
 };
 
-// Any layout: a warp per row, an element per lane and step.  The gradient of a class outside of the list is
-// dloss * scale * p_c * (Q - q_r / p_r), which the warp writes everywhere; the list's classes are read beforehand and written over it.
+constexpr size_t kMostMask = 160 * 1024;   // bytes of mask in shared memory
+
+// A row's list in shared memory
+struct List {
+  uint32_t cls[kMostTop];
+  float a[kMostTop], x[kMostTop];   // log2 q and the student's logit
+};
+
+// What a group knows of a row when its loss is known
+struct Distilled {
+  float S, mt, Q, qr, loss;   // the row's sum against mt (a maximum); sum q + q_r
+  float out, rS;              // gradient outside of the list: dloss * scale * out * 2^((x - m) cs), with m and its rounding as the pass had them
+  bool some;
+};
+
+// One warp: the teacher's weights, the list's share of the row and the loss.  o: the sums of the pass over the row, of all
+// classes or (rest) of those outside of the list; `off` = mc - m * cs, the rounding of its reference.
+__device__ __forceinline__ Distilled distill_row(const DistillP& p, size_t r, List& list, float m, float off, float R) {
+  const uint32_t lane = threadIdx.x & 31, k = p.top, C = p.x.C;
+  Distilled d;
+  float a[4], x[4], am = -INFINITY;
+  bool in[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t j = lane + 32 * i;
+    in[i] = j < k && list.cls[j] < C;
+    a[i] = in[i] ? list.a[j] : -INFINITY;
+    x[i] = in[i] ? list.x[j] : 0.f;
+    am = fmaxf(am, a[i]);
+  }
+  float shift;
+  if (p.rest) {
+    shift = p.top_lse ? (float)(p.top_lse[r] * kLog2e) : 0.f;
+  } else {
+    am = warp_max(am);
+    if (am == -INFINITY) am = 0.f;
+    float z = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) z += exp2f(a[i] - am);
+    z = warp_sum(z);
+    shift = z != 0.f ? am + log2f(z) : 0.f;
+  }
+  float q[4], Q = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    a[i] -= shift;
+    q[i] = exp2f(a[i]);
+    Q += q[i];
+  }
+  Q = warp_sum(Q);
+  float mk = -INFINITY, K = 0.f;
+  if (p.rest) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (in[i]) mk = fmaxf(mk, x[i]);
+    mk = warp_max(mk);
+    if (mk == -INFINITY) mk = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (in[i]) {   // a class that stands twice has its weight once
+        const uint32_t c = list.cls[lane + 32 * i];
+        bool first = true;
+        for (uint32_t j = 0; j < lane + 32 * i; ++j) first &= list.cls[j] != c;
+        if (first) K += exp2_fast((x[i] - mk) * p.cs);
+      }
+    K = warp_sum(K);
+  }
+  if (m == -INFINITY) m = 0.f;
+  // R is off by 2^-off against m: `off` stays in the logarithms and in `out`
+  float to = 0.f, L = 0.f;
+  d.S = R;
+  d.mt = m;
+  bool by_list = false;
+  if (K != 0.f) {
+    if (R == 0.f) {
+      d.S = K;
+      by_list = true;
+    } else if (m >= mk) {
+      d.S = R + K * exp2_fast((mk - m) * p.cs - off);
+    } else {
+      to = (mk - m) * p.cs - off;
+      d.S = K + R * exp2_fast(-to);
+      by_list = true;
+    }
+    if (by_list) d.mt = mk;
+  }
+  const float offt = by_list ? 0.f : off;   // the rounding of the reference of S
+  d.some = d.S != 0.f;
+  if (d.some) L = log2f(d.S);
+  d.qr = p.rest && R != 0.f ? fmaxf(1.f - Q, 0.f) : 0.f;
+  float loss = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (q[i] != 0.f) loss += q[i] * (kLn2 * (a[i] + L + offt) - (x[i] - d.mt) * p.scale);
+  loss = warp_sum(loss);
+  if (d.qr > 0.f) loss += d.qr * (kLn2 * (log2f(d.qr) - log2f(R) + L + (offt - off)) + (d.mt - m) * p.scale);
+  d.loss = d.some ? loss + 0.f * L : 0.f;   // NaN without any entry, too
+  d.Q = Q + d.qr;
+  d.rS = d.some ? 1.f / d.S : 0.f;
+  d.out = d.some ? d.Q * d.rS * exp2_fast(-to) - (d.qr > 0.f ? d.qr / R : 0.f) : 0.f;
+  // each entry's q, for the gradient: of the entries of a class, the first one has the sum
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (lane + 32 * i < k) list.a[lane + 32 * i] = q[i];
+  // p of a listed class is 2^((x - mt) cs - offt) / S
+  d.rS *= exp2_fast(-offt);
+  return d;
+}
+// The gradient of entry j's class
+__device__ __forceinline__ float listed_grad(const DistillP& p, const Distilled& d, const List& list, uint32_t j, float f) {
+  const uint32_t c = list.cls[j];
+  float sum = 0.f;
+  for (uint32_t i = 0; i < p.top; ++i) sum += list.cls[i] == c ? list.a[i] : 0.f;
+  return d.some ? f * (exp2_fast((list.x[j] - d.mt) * p.cs) * d.rS * d.Q - sum) : 0.f;
+}
+
+// Any layout, any numbers: plain loops of a group over one row, whose list is in place
+template <int NT, typename T, bool BWD>
+__device__ void plain_row(Group<NT>& g, const DistillP& p, size_t r, List& list, Distilled* shared) {
+  const T* x = (const T*)p.logits + p.x.offset(r);
+  const int64_t st = p.x.step;
+  const uint32_t C = p.x.C, k = p.top;
+  auto outside = [&](uint32_t c) {
+    bool in = false;
+    if (p.rest)
+      for (uint32_t j = 0; j < k; ++j) in |= list.cls[j] == c;
+    return !in;
+  };
+  float m = -INFINITY, R = 0.f;
+  for (uint32_t c = g.tid; c < C; c += NT)
+    if (outside(c)) m = fmaxf(m, ld_f(x + c * st));
+  m = g.max(m);
+  if (m == -INFINITY) m = 0.f;
+  for (uint32_t c = g.tid; c < C; c += NT)
+    if (outside(c)) R += exp2_fast((ld_f(x + c * st) - m) * p.cs);
+  R = g.sum(R);
+  if (threadIdx.x % NT < 32) {
+    const Distilled d = distill_row(p, r, list, m, 0.f, R);
+    if (g.tid == 0) {
+      *shared = d;
+      if (p.loss) p.loss[r] = d.loss;
+    }
+  }
+  g.sync();
+  if constexpr (BWD) {
+    const Distilled d = *shared;
+    T* o = (T*)p.dlogits + p.g.offset(r);
+    const float f = p.dloss[r] * p.scale;
+    float old[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t j = g.tid + i * NT;
+      old[i] = p.accumulate && j < k && list.cls[j] < C ? ld_f(o + list.cls[j] * p.g.step) : 0.f;
+    }
+    g.sync();
+    for (uint32_t c = g.tid; c < C; c += NT) {
+      float v = f * (exp2_fast((ld_f(x + c * st) - m) * p.cs) * d.out);
+      if (p.accumulate) v += ld_f(o + c * p.g.step);
+      st_f(o + c * p.g.step, v);
+    }
+    g.sync();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t j = g.tid + i * NT;
+      if (j < k && list.cls[j] < C) {
+        const float v = listed_grad(p, d, list, j, f);
+        st_f(o + list.cls[j] * p.g.step, p.accumulate ? old[i] + v : v);
+      }
+    }
+  }
+  g.sync();
+}
+
+// A row's list into shared memory: entry j by the group's thread j
+template <int NT, typename T>
+__device__ __forceinline__ void fetch_list(Group<NT>& g, const DistillP& p, size_t r, const T* x, int64_t st, List& list) {
+  for (uint32_t j = g.tid; j < p.top; j += NT) {
+    const uint32_t c = p.top_class[r * p.top + j];
+    list.cls[j] = c;
+    list.a[j] = p.top_logit[r * p.top + j] * p.ts;
+    list.x[j] = c < p.x.C ? ld_f(x + c * st) : 0.f;
+  }
+}
+
 template <typename T, bool BWD>
 __global__ void __launch_bounds__(256) distill_any(DistillP p) {
   grid_dependency();
-  __shared__ uint32_t s_cls[8][kMostTop];
-  __shared__ float s_q[8][kMostTop];
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  __shared__ List lists[8];
+  __shared__ Distilled shared[8];
+  Group<32> g(nullptr);
+  const uint32_t w = threadIdx.x >> 5;
   const size_t warp = ((size_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5, nw = ((size_t)gridDim.x * blockDim.x) >> 5;
-  const uint32_t C = p.x.C, k = p.top;
-  uint32_t* cls = s_cls[w];
-  float* qs = s_q[w];
   for (size_t r = warp; r < p.x.rows; r += nw) {
+    fetch_list<32, T>(g, p, r, (const T*)p.logits + p.x.offset(r), p.x.step, lists[w]);
+    g.sync();
+    plain_row<32, T, BWD>(g, p, r, lists[w], &shared[w]);
+  }
+}
+
+// ---------------------------------------------------------------- rows of many neighbouring classes
+// NT 32: a warp per row, eight vectors per lane and batch.  NT 256: a block per row, or a cluster of blocks, four vectors.
+// REST: the classes of the list are left out of the pass.
+template <int NT, typename T, bool REST, bool BWD>
+__global__ void __launch_bounds__(256) distill_rows(DistillP p) {
+  constexpr int U = NT == 32 ? 8 : 4, V = Vec<T>::V;
+  typedef Vec<T> X;
+  extern __shared__ __align__(16) uint8_t masks[];   // a byte per vector of the row's share (NT 32: of each warp's row)
+  __shared__ Key red[kRowWarps];
+  __shared__ Part parts[kRowWarps], whole;
+  __shared__ List lists[NT == 32 ? kRowWarps : 1];
+  __shared__ Distilled shared[NT == 32 ? kRowWarps : 1];
+  grid_dependency();
+  cg::cluster_group cluster = cg::this_cluster();
+  const uint32_t parts_n = NT == 32 ? 1 : cluster.num_blocks(), part = NT == 32 ? 0 : cluster.block_rank();
+  Group<NT> g(red);
+  const uint32_t C = p.x.C, warp = threadIdx.x >> 5, k = p.top;
+  List& list = lists[NT == 32 ? warp : 0];
+  uint8_t* mask = masks + (NT == 32 ? (size_t)warp * ((C / V + 15) / 16 * 16) : 0);
+  const size_t row0 = NT == 32 ? (size_t)blockIdx.x * kRowWarps + warp : blockIdx.x / parts_n;
+  const size_t rows_n = NT == 32 ? (size_t)gridDim.x * kRowWarps : gridDim.x / parts_n;
+  for (size_t r = row0; r < p.x.rows; r += rows_n) {
     const T* x = (const T*)p.logits + p.x.offset(r);
-    const int64_t st = p.x.step;
-    // the list: a_j = log2 q_j
-    float a[4], xj[4], am = -INFINITY;
-    uint32_t cj[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t j = lane + 32 * i;
-      cj[i] = j < k ? p.top_class[r * k + j] : kNoClass;
-      a[i] = cj[i] < C ? p.top_logit[r * k + j] * p.ts : -INFINITY;
-      xj[i] = cj[i] < C ? ld_f(x + cj[i] * st) : 0.f;
-      am = fmaxf(am, a[i]);
-    }
-    float shift;
-    if (p.rest) {
-      shift = p.top_lse ? (float)(p.top_lse[r] * kLog2e) : 0.f;
-    } else {
-      am = warp_max(am);
-      if (am == -INFINITY) am = 0.f;
-      float z = 0.f;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) z += exp2f(a[i] - am);
-      z = warp_sum(z);
-      shift = z != 0.f ? am + log2f(z) : 0.f;
-    }
-    float q[4], Q = 0.f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      a[i] -= shift;
-      q[i] = exp2f(a[i]);
-      Q += q[i];
-      const uint32_t j = lane + 32 * i;
-      if (j < k) { cls[j] = cj[i]; qs[j] = q[i]; }
-    }
-    Q = warp_sum(Q);
-    __syncwarp();
-    // every class, or with rest the classes outside of the list: reference m, sum R; the list's own beside them
-    auto listed = [&](uint32_t c) {
-      bool in = false;
-      if (p.rest)
-        for (uint32_t j = 0; j < k; ++j) in |= cls[j] == c;
-      return in;
-    };
-    float m = -INFINITY, R = 0.f, mk = -INFINITY, K = 0.f;
-    for (uint32_t c = lane; c < C; c += 32)
-      if (!listed(c)) m = fmaxf(m, ld_f(x + c * st));
-    m = warp_max(m);
-    if (m == -INFINITY) m = 0.f;
-    for (uint32_t c = lane; c < C; c += 32)
-      if (!listed(c)) R += exp2_fast((ld_f(x + c * st) - m) * p.cs);
-    R = warp_sum(R);
-    if (p.rest) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (cj[i] < C) mk = fmaxf(mk, xj[i]);
-      mk = warp_max(mk);
-      if (mk == -INFINITY) mk = 0.f;
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (cj[i] < C) {   // a class that stands twice has its weight once
-          bool first = true;
-          for (uint32_t j = 0; j < (uint32_t)(lane + 32 * i); ++j) first &= cls[j] != cj[i];
-          if (first) K += exp2_fast((xj[i] - mk) * p.cs);
+    const Strip<T> b(x, C, part, parts_n);
+    const uint4* xv = (const uint4*)(x + b.head);
+    if (REST)
+      for (uint32_t i = g.tid; i < (b.ve - b.vb + 15) / 16; i += NT) ((uint4*)mask)[i] = make_uint4(0, 0, 0, 0);
+    fetch_list<NT, T>(g, p, r, x, 1, list);
+    g.sync();
+    bool apart = true;   // this thread's single element is outside of the list
+    const uint32_t sc = g.tid < 2 * V ? b.single(g.tid) : kNoClass;
+    if (REST) {
+      for (uint32_t j = g.tid; j < k; j += NT) {
+        const uint32_t c = list.cls[j], v = (c - b.head) / V;
+        if (c < C && c >= b.head && v >= b.vb && v < b.ve) {
+          const uint32_t at = v - b.vb;
+          atomicOr((uint32_t*)mask + at / 4, 1u << (at % 4 * 8 + (c - b.head) % V));
         }
-      K = warp_sum(K);
+      }
+      if (sc != kNoClass)
+        for (uint32_t j = 0; j < k; ++j) apart &= list.cls[j] != sc;
+      g.sync();
     }
-    float S = R, mt = m, to = 0.f, L = 0.f;   // S against its own reference mt = m + to / cs
-    if (K != 0.f) {
-      if (R == 0.f) {
-        S = K;
-        mt = mk;
-      } else if (m >= mk) {
-        S = R + K * exp2_fast((mk - m) * p.cs);
-      } else {
-        to = (mk - m) * p.cs;
-        S = K + R * exp2_fast(-to);
-        mt = mk;
+    Part a;
+    a.clear();
+    if (sc != kNoClass && apart) a.add<false>(ld_f(x + sc), p.cs);
+    for (uint32_t v0 = b.vb; v0 < b.ve; v0 += U * NT) {
+      uint4 w[U];
+      typename X::Max most;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const uint32_t v = v0 + u * NT + g.tid;
+        w[u] = v < b.ve ? xv[v] : X::none();
+      }
+      if (REST) {
+        uint32_t out[U], any = 0;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const uint32_t v = v0 + u * NT + g.tid;
+          out[u] = v < b.ve ? mask[v - b.vb] : 0;
+          any |= out[u];
+        }
+        if (any) {
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            uint32_t* q = &w[u].x;
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+              if (out[u] >> i & 1) {
+                if (V == 4) q[i] = 0xff800000u;
+                else q[i / 2] = i & 1 ? (q[i / 2] & 0xffffu) | 0xff800000u : (q[i / 2] & 0xffff0000u) | 0xff80u;
+              }
+          }
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) most = u ? X::max(most, X::max(w[u])) : X::max(w[u]);
+      const float bm = X::value(most);
+      if (bm > a.m) {
+        a.m = bm;
+        a.refer<false>(fmaxf(a.mc, Part::reference(bm, p.cs)));
+      }
+      float S[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (v0 + u * NT >= b.ve) break;
+        float f[V];
+        X::unpack(w[u], f);
+#pragma unroll
+        for (int i = 0; i < V; ++i) S[i & 3] += exp2_fast(fmaf(f[i], p.cs, -a.mc));
+      }
+      a.S += (S[0] + S[1]) + (S[2] + S[3]);
+    }
+    a.join_lanes<false>();
+    if (NT != 32) {
+      if ((g.tid & 31) == 0) parts[warp] = a;
+      __syncthreads();
+      a = parts[0];
+#pragma unroll
+      for (int i = 1; i < kRowWarps; ++i) a.join<false>(parts[i]);
+      if (parts_n > 1) {
+        if (g.tid == 0) whole = a;
+        cluster.sync();
+        a = *cluster.map_shared_rank(&whole, 0);
+        for (uint32_t q = 1; q < parts_n; ++q) a.join<false>(*cluster.map_shared_rank(&whole, q));
       }
     }
-    const bool some = S != 0.f;
-    if (some) L = log2f(S);
-    const float qr = p.rest && R != 0.f ? fmaxf(1.f - Q, 0.f) : 0.f;
-    float loss = 0.f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (q[i] != 0.f) loss += q[i] * (kLn2 * (a[i] + L) - (xj[i] - mt) * p.scale);
-    loss = warp_sum(loss);
-    if (qr > 0.f) loss += qr * (kLn2 * (log2f(qr) - log2f(R) + L) + (mt - m) * p.scale);
-    if (lane == 0 && p.loss) p.loss[r] = some ? loss + 0.f * L : 0.f;   // NaN without any entry, too
+    if (a.strange(p.cs)) {
+      if (part == 0) plain_row<NT, T, BWD>(g, p, r, list, shared + (NT == 32 ? warp : 0));
+      if (parts_n > 1) cluster.sync();
+      else g.sync();
+      continue;
+    }
+    const float off = a.m == -INFINITY ? 0.f : fmaf(-a.m, p.cs, a.mc);
+    Distilled d;
+    if (NT == 32 || warp == 0) {
+      d = distill_row(p, r, list, a.m, off, a.S);
+      if (g.tid == 0 && part == 0 && p.loss) p.loss[r] = d.loss;
+      if (NT != 32 && BWD && g.tid == 0) shared[0] = d;
+    }
+    g.sync();
     if constexpr (BWD) {
-      T* g = (T*)p.dlogits + p.g.offset(r);
-      const float d = p.dloss[r] * p.scale;
-      float old[4];
+      if (NT != 32) d = shared[0];
+      T* o = (T*)p.dlogits + p.g.offset(r);
+      const bool even = (((uintptr_t)o ^ (uintptr_t)x) & 15u) == 0;   // both have their vectors at the same classes
+      const float f = p.dloss[r] * p.scale, coef = f * d.out, mc = a.mc;
+      auto grad = [&](float v) { return coef * exp2_fast(fmaf(v, p.cs, -mc)); };
+      float gl[NT == 32 ? 4 : 1];   // the list's gradients, written last
 #pragma unroll
-      for (int i = 0; i < 4; ++i) old[i] = p.accumulate && cj[i] < C ? ld_f(g + cj[i] * p.g.step) : 0.f;
-      __syncwarp();
-      Q += qr;
-      const float rS = some ? 1.f / S : 0.f, out = some ? Q * rS * exp2_fast(-to) - (qr > 0.f ? qr / R : 0.f) : 0.f;
-      for (uint32_t c = lane; c < C; c += 32) {
-        float v = d * (exp2_fast((ld_f(x + c * st) - m) * p.cs) * out);
-        if (p.accumulate) v += ld_f(g + c * p.g.step);
-        st_f(g + c * p.g.step, v);
+      for (int i = 0; i < (NT == 32 ? 4 : 1); ++i) {
+        const uint32_t j = g.tid + i * NT;
+        if (j < k && list.cls[j] >= b.begin() && list.cls[j] < b.end()) gl[i] = listed_grad(p, d, list, j, f) + (p.accumulate ? ld_f(o + list.cls[j]) : 0.f);
       }
-      __syncwarp();
+      if (p.accumulate) g.sync();
+      if (sc != kNoClass) st_f(o + sc, grad(ld_f(x + sc)) + (p.accumulate ? ld_f(o + sc) : 0.f));
+      uint4* ov = (uint4*)(o + b.head);
+      for (uint32_t v0 = b.vb; v0 < b.ve; v0 += U * NT) {
+        uint4 w[U];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (cj[i] < C) {
-          float sum = 0.f;
-          for (uint32_t j = 0; j < k; ++j) sum += cls[j] == cj[i] ? qs[j] : 0.f;
-          const float v = some ? d * (exp2_fast((xj[i] - mt) * p.cs) * rS * Q - sum) : 0.f;
-          st_f(g + cj[i] * p.g.step, p.accumulate ? old[i] + v : v);
+        for (int u = 0; u < U; ++u) {
+          const uint32_t v = v0 + u * NT + g.tid;
+          if (v < b.ve) w[u] = xv[v];
         }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const uint32_t v = v0 + u * NT + g.tid;
+          if (v >= b.ve) break;
+          float h[V];
+          X::unpack(w[u], h);
+#pragma unroll
+          for (int i = 0; i < V; ++i) h[i] = grad(h[i]);
+          if (even) {
+            if (p.accumulate) {
+              float q[V];
+              X::unpack(ov[v], q);
+#pragma unroll
+              for (int i = 0; i < V; ++i) h[i] += q[i];
+            }
+            ov[v] = X::pack(h);
+          } else {
+            T* os = o + b.class_of(v);
+#pragma unroll
+            for (int i = 0; i < V; ++i) st_f(os + i, p.accumulate ? h[i] + ld_f(os + i) : h[i]);
+          }
+        }
+      }
+      g.sync();
+#pragma unroll
+      for (int i = 0; i < (NT == 32 ? 4 : 1); ++i) {
+        const uint32_t j = g.tid + i * NT;
+        if (j < k && list.cls[j] >= b.begin() && list.cls[j] < b.end()) st_f(o + list.cls[j], gl[i]);
+      }
     }
-    __syncwarp();
+    if (parts_n > 1) cluster.sync();   // what the others read of this block's
+    else g.sync();
   }
 }
 
@@ -183,9 +440,34 @@ static int distill_args(const ad_distill_args* a, bool bwd, DistillP& p) {
   return AD_OK;
 }
 
+
+template <int NT, typename T, bool REST, bool BWD>
+static int launch_rows(const DistillP& p, uint32_t n, size_t smem, cudaStream_t s) {
+  auto kernel = distill_rows<NT, T, REST, BWD>;
+  // the limit belongs to the function: the most that it takes
+  if (smem > 32 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMostMask) != cudaSuccess) {
+    cudaGetLastError();
+    return AD_ERR_CUDA;
+  }
+  launch_row_kernel(kernel, p, NT == 32 ? (p.x.rows + kRowWarps - 1) / kRowWarps : p.x.rows, n, smem, s);
+  return AD_OK;
+}
+
 template <typename T, bool BWD>
 static int launch_distill(const DistillP& p, cudaStream_t s) {
-  launch(distill_any<T, BWD>, grid_for(p.x.rows, 8), 256, 0, s, p);
+  int rc = AD_OK;
+  const size_t vectors = p.x.C / Vec<T>::V;
+  const uint32_t n = row_parts(p.x.rows, (size_t)p.x.C * sizeof(T));
+  const size_t mask = p.rest ? (vectors / n + 17) / 16 * 16 : 0;
+  if (p.x.step != 1 || (BWD && p.g.step != 1) || p.x.C <= 64 || mask > kMostMask) {
+    launch(distill_any<T, BWD>, grid_for(p.x.rows, 8), 256, 0, s, p);
+  } else if (p.x.C * sizeof(T) <= 8192) {
+    const size_t all = p.rest ? kRowWarps * ((vectors + 15) / 16 * 16) : 0;
+    rc = p.rest ? launch_rows<32, T, true, BWD>(p, 1, all, s) : launch_rows<32, T, false, BWD>(p, 1, all, s);
+  } else {
+    rc = p.rest ? launch_rows<256, T, true, BWD>(p, n, mask, s) : launch_rows<256, T, false, BWD>(p, n, mask, s);
+  }
+  if (rc != AD_OK) return rc;
   count_launch();
   return launch_status();
 }

@@ -507,13 +507,6 @@ static int launch_any(const LogprobP& p, cudaStream_t s) {
   return AD_OK;
 }
 
-// Blocks of a row: few rows share the machine, a part at least 8 KB
-static uint32_t row_parts(size_t rows, size_t row_bytes) {
-  uint32_t n = 1;
-  while (n < 8 && rows * n * 2 <= 4 * kNumSMs && row_bytes / (n * 2) >= 8192) n *= 2;
-  return n;
-}
-
 template <int NT, typename T, bool ENT, bool RANK, bool TOP, bool BWD>
 static int launch_rows(const LogprobP& p, cudaStream_t s) {
   auto kernel = logprob_rows<NT, T, ENT, RANK, TOP, BWD>;
@@ -525,21 +518,7 @@ static int launch_rows(const LogprobP& p, cudaStream_t s) {
     cudaGetLastError();
     return AD_ERR_CUDA;
   }
-  cudaLaunchConfig_t cfg{};
-  cudaLaunchAttribute at[2];
-  const size_t blocks = NT == 32 ? (p.x.rows + kRowWarps - 1) / kRowWarps : p.x.rows;
-  cfg.gridDim = (unsigned)((blocks < (1u << 20) ? blocks : (1u << 20)) * n);
-  cfg.blockDim = 256;
-  cfg.dynamicSmemBytes = keys * sizeof(Key);
-  cfg.stream = s;
-  if (n > 1) {
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = n;
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-    cfg.numAttrs = 1;
-  }
-  launch_attr(cfg, at);
-  cudaLaunchKernelEx(&cfg, kernel, p);
+  launch_row_kernel(kernel, p, NT == 32 ? (p.x.rows + kRowWarps - 1) / kRowWarps : p.x.rows, n, keys * sizeof(Key), s);
   return AD_OK;
 }
 
@@ -562,7 +541,7 @@ template <typename T, bool BWD>
 static int launch_logprob(const LogprobP& p, cudaStream_t s) {
   int rc;
   if (p.x.step != 1 || (BWD && p.g.step != 1) || p.x.C <= 64) rc = launch_any<T, BWD>(p, s);
-  else if (p.x.C * sizeof(T) <= 8192 || p.x.rows > (1u << 30)) rc = BWD ? launch_bwd<32, T>(p, s) : launch_fwd<32, T>(p, s);
+  else if (p.x.C * sizeof(T) <= 8192) rc = BWD ? launch_bwd<32, T>(p, s) : launch_fwd<32, T>(p, s);
   else rc = BWD ? launch_bwd<256, T>(p, s) : launch_fwd<256, T>(p, s);
   if (rc != AD_OK) return rc;
   count_launch();

@@ -304,4 +304,29 @@ __device__ void plain_sums(G& g, const T* x, int64_t st, uint32_t C, float cs, R
   s.low = s.L = s.some ? log2f(S) : 0.f;
 }
 
+// Blocks of a row: few rows share the machine, a part at least 8 KB
+inline uint32_t row_parts(size_t rows, size_t row_bytes) {
+  uint32_t n = 1;
+  while (n < 8 && rows * n * 2 <= 4 * kNumSMs && row_bytes / (n * 2) >= 8192) n *= 2;
+  return n;
+}
+// `units` blocks, or clusters of n blocks; a kernel's blocks go on to further rows where there are more
+template <typename P>
+void launch_row_kernel(void (*kernel)(P), const P& p, size_t units, uint32_t n, size_t smem, cudaStream_t s) {
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute at[2];
+  cfg.gridDim = (unsigned)((units < (1u << 20) ? units : (1u << 20)) * n);
+  cfg.blockDim = kRowThreads;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  if (n > 1) {
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = n;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.numAttrs = 1;
+  }
+  launch_attr(cfg, at);
+  cudaLaunchKernelEx(&cfg, kernel, p);   // an error is what launch_status() returns
+}
+
 }  // namespace adk
