@@ -5,9 +5,10 @@
 //   entropy = ln2 (log2 S - E / S),   log p_c = scale (x_c - m) - ln2 (log2 S + (mc - m * cs)),
 // where mc - m * cs, the rounding of mc, is what an FMA gives.  One pass over the row: a thread keeps its own maximum,
 // and S and E against it, and rescales them when the maximum of a batch of loads is larger.
-// A reference is at least kFloor, so that a share of -inf or of the type's lowest value adds 2^-inf = 0 and no inf - inf.
-// Rows that this does not serve (a maximum beyond +-1e36 in units of log 2, +inf, NaN) are done again by plain loops
-// over x_c - m.  A row of -inf has S = 0, which is how it is recognised.
+// mc is off by up to 2^-24 of itself, and the terms by 2 to that: a row whose maximum is beyond +-kFar in units of log 2, or
+// that holds +inf or NaN, is done again by plain loops over x_c - m.  A share's reference is at least kFloor, so that
+// what is masked (-inf, the type's lowest value, -1e9) adds 2^-4e6 = 0 to the row and never inf or inf - inf.
+// A row of -inf has S = 0, which is how it is recognised.
 #pragma once
 
 #include "common.cuh"
@@ -18,7 +19,7 @@ constexpr float kLn2 = 0.693147180559945309f;
 constexpr double kLog2e = 1.442695040888963407;
 constexpr uint32_t kMostTop = 128;                 // entries of a row's list
 constexpr uint32_t kNoClass = 0xffffffffu;
-constexpr float kFloor = -1e37f, kFar = 1e36f;
+constexpr float kFloor = -4e6f, kFar = 1e6f;
 
 // Where the rows lie: row r's class c is at offset(r) + c * step (elements)
 struct Rows {
@@ -299,6 +300,109 @@ __device__ void plain_sums(G& g, const T* x, int64_t st, uint32_t C, float cs, R
   }
   S = g.sum(S);
   if (ENT) E = g.sum(E);
+  s.m = m; s.mc = 0.f; s.S = S;
+  s.some = S != 0.f;
+  s.low = s.L = s.some ? log2f(S) : 0.f;
+}
+
+// ---- a thread per position: few classes, or classes in planes
+// MODE 0: from global memory, neighbouring threads on neighbouring positions of a plane.  1, 2: rows that a block has copied
+// to shared memory, read by single elements (1: rows of any length, one behind the other) or by vectors (2: rows of whole
+// vectors, an odd number of them apart, so that eight lanes' loads fall into different banks).
+template <typename T, int MODE>
+struct Position {
+  const T* x;
+  int64_t step;   // MODE 0
+  uint32_t C;
+  __device__ float get(uint32_t c) const { return ld_f(MODE == 0 ? x + c * step : x + c); }
+  // classes [c, c + 8), -inf behind the last one
+  __device__ void batch(uint32_t c, float (&f)[8]) const {
+    constexpr uint32_t V = Vec<T>::V;
+    if (MODE == 2) {
+      Vec<T>::unpack(*(const uint4*)(x + c), f);
+      if (V == 4) Vec<T>::unpack(c + 4 < C ? *(const uint4*)(x + c + 4) : Vec<T>::none(), f + 8 - V);
+    } else if (c + 8 <= C) {
+#pragma unroll
+      for (uint32_t i = 0; i < 8; ++i) f[i] = get(c + i);
+    } else {
+#pragma unroll
+      for (uint32_t i = 0; i < 8; ++i) f[i] = c + i < C ? get(c + i) : -INFINITY;
+    }
+  }
+  __device__ void set(uint32_t c, float v) const { st_f(const_cast<T*>(MODE == 0 ? x + c * step : x + c), v); }
+};
+constexpr uint32_t kPositions = 128;         // of a block
+constexpr uint32_t kFewClasses = 64;         // of rows in shared memory
+// MODE 1, 2: elements from one row to the next in shared memory
+template <typename T, int MODE> __host__ __device__ inline uint32_t tile_pitch(uint32_t C) { return MODE == 2 ? (C / Vec<T>::V | 1u) * Vec<T>::V : C; }
+template <typename T, int MODE>
+__device__ __forceinline__ void copy_tile(const T* from, const Rows& g, size_t r0, uint32_t n, T* tile) {
+  constexpr uint32_t V = Vec<T>::V;
+  const T* src = from + r0 * (size_t)g.pitch;
+  auto async = [](void* d, const void* s) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(d)), "l"(s) : "memory");
+  };
+  if (MODE == 2) {
+    const uint32_t q = g.C / V, to = tile_pitch<T, 2>(g.C);
+    for (uint32_t i = threadIdx.x; i < n * q; i += kPositions) {
+      const uint32_t row = i / q, col = i - row * q;
+      async(tile + row * to + col * V, src + row * (size_t)g.pitch + col * V);
+    }
+  } else if (g.pitch == (int64_t)g.C) {
+    const uint32_t e = n * g.C, v = ((uintptr_t)src & 15u) == 0 ? e / V : 0;
+    for (uint32_t i = threadIdx.x; i < v; i += kPositions) async(tile + i * V, src + i * V);
+    for (uint32_t i = v * V + threadIdx.x; i < e; i += kPositions) tile[i] = src[i];
+  } else {
+    for (uint32_t i = threadIdx.x; i < n * g.C; i += kPositions) tile[i] = src[i / g.C * (size_t)g.pitch + i % g.C];
+  }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+}
+template <typename T, int MODE>
+__device__ __forceinline__ void write_tile(T* to, const Rows& g, size_t r0, uint32_t n, const T* tile) {
+  constexpr uint32_t V = Vec<T>::V;
+  T* dst = to + r0 * (size_t)g.pitch;
+  const uint32_t tp = tile_pitch<T, MODE>(g.C);
+  if (MODE == 2 && ((uintptr_t)dst & 15u) == 0 && g.pitch % V == 0) {
+    const uint32_t q = g.C / V;
+    for (uint32_t i = threadIdx.x; i < n * q; i += kPositions) {
+      const uint32_t row = i / q, col = i - row * q;
+      *(uint4*)(dst + row * (size_t)g.pitch + col * V) = *(const uint4*)(tile + row * tp + col * V);
+    }
+  } else if (MODE == 1 && g.pitch == (int64_t)g.C) {
+    const uint32_t e = n * g.C, v = ((uintptr_t)dst & 15u) == 0 ? e / V : 0;
+    for (uint32_t i = threadIdx.x; i < v; i += kPositions) ((uint4*)dst)[i] = ((const uint4*)tile)[i];
+    for (uint32_t i = v * V + threadIdx.x; i < e; i += kPositions) dst[i] = tile[i];
+  } else {
+    for (uint32_t i = threadIdx.x; i < n * g.C; i += kPositions) dst[i / g.C * (size_t)g.pitch + i % g.C] = tile[i / g.C * tp + i % g.C];
+  }
+}
+// Bytes of such a tile, a multiple of 16
+template <typename T, int MODE> inline size_t tile_bytes(uint32_t C) {
+  return MODE == 0 ? 0 : (kPositions * (size_t)tile_pitch<T, MODE>(C) * sizeof(T) + 15) / 16 * 16;
+}
+// The mode that a call's rows are for; -1: none of them
+template <typename T>
+inline int position_mode(const Rows& g, const void* x) {
+  if (g.HW) return g.C <= 0xffffu ? 0 : -1;
+  if (g.step != 1 || g.C > kFewClasses) return -1;
+  return g.C % Vec<T>::V == 0 && g.pitch % Vec<T>::V == 0 && aligned_to(x, 16) ? 2 : 1;
+}
+inline unsigned position_blocks(size_t rows) {
+  const size_t n = (rows + kPositions - 1) / kPositions;
+  return (unsigned)(n < (1u << 20) ? n : (1u << 20));
+}
+// One position by plain loops over x_c - m
+template <bool ENT, typename P>
+__device__ void plain_position(const P& x, float cs, RowSums& s, float& E) {
+  float m = -INFINITY, S = 0.f;
+  for (uint32_t c = 0; c < x.C; ++c) m = fmaxf(m, x.get(c));
+  if (m == -INFINITY) m = 0.f;
+  E = 0.f;
+  for (uint32_t c = 0; c < x.C; ++c) {
+    const float u = (x.get(c) - m) * cs, e = exp2_fast(u);
+    S += e;
+    if (ENT && e > 0.f) E += e * u;
+  }
   s.m = m; s.mc = 0.f; s.S = S;
   s.some = S != 0.f;
   s.low = s.L = s.some ? log2f(S) : 0.f;

@@ -70,7 +70,9 @@ def logprob_grad(x, scale, label, dlse, dent, dlogp):
     dl = np.where(known, dlogp, 0.0)[:, None]
     dz, de = dlse[:, None], dent[:, None]
     d = scale * (p * (dz - dl) - de * (plog + p * H_) + dl * hot)
-    mag = scale * (p * (abs(dz) + abs(dl)) + abs(de) * (abs(plog) + p * H_) + abs(dl) * hot)
+    # by tol, a row's error of log p: p is off by tol of itself, log p by tol, H by tol (2 + H) (its check): the entropy's term
+    # p (log p + H) by tol (|p log p| + p H) + p (tol + tol (2 + H)), which is not 0 where log p + H is
+    mag = scale * (p * (abs(dz) + abs(dl)) + abs(de) * (abs(plog) + p * (3 + 2 * H_)) + abs(dl) * hot)
     return d, mag
 
 
