@@ -28,12 +28,14 @@ struct DistillP {
   int accumulate;
 };
 
-constexpr size_t kMostMask = 160 * 1024;   // bytes of mask in shared memory
+constexpr size_t kMostMask = 120 * 1024;   // bytes of mask in shared memory
 
 // A row's list in shared memory
-struct List {
+struct __align__(16) List {
   uint32_t cls[kMostTop];
-  float a[kMostTop], x[kMostTop];   // log2 q and the student's logit
+  float a[kMostTop], x[kMostTop];   // log2 q, later q, and the student's logit
+  uint8_t first[kMostTop];          // no earlier entry has the class
+  bool twice;                       // some class stands twice
 };
 
 // What is known of a row when its list and its classes have been summed
@@ -122,12 +124,7 @@ __device__ __forceinline__ Distilled distill_row(const DistillP& p, size_t r, Li
     if (mk == -INFINITY) mk = 0.f;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      if (in[i]) {   // a class that stands twice has its weight once
-        const uint32_t c = list.cls[lane + 32 * i];
-        bool first = true;
-        for (uint32_t j = 0; j < lane + 32 * i; ++j) first &= list.cls[j] != c;
-        if (first) K += exp2_fast((x[i] - mk) * p.cs);
-      }
+      if (in[i] && list.first[lane + 32 * i]) K += exp2_fast((x[i] - mk) * p.cs);   // a class that stands twice has its weight once
     K = warp_sum(K);
   }
   float rest_loss;
@@ -145,8 +142,11 @@ __device__ __forceinline__ Distilled distill_row(const DistillP& p, size_t r, Li
 // The gradient of entry j's class
 __device__ __forceinline__ float listed_grad(const DistillP& p, const Distilled& d, const List& list, uint32_t j, float f) {
   const uint32_t c = list.cls[j];
-  float sum = 0.f;
-  for (uint32_t i = 0; i < p.top; ++i) sum += list.cls[i] == c ? list.a[i] : 0.f;
+  float sum = list.a[j];
+  if (list.twice) {
+    sum = 0.f;
+    for (uint32_t i = 0; i < p.top; ++i) sum += list.cls[i] == c ? list.a[i] : 0.f;
+  }
   return d.some ? f * (exp2_fast((list.x[j] - d.mt) * p.cs) * d.rS * d.Q - sum) : 0.f;
 }
 
@@ -208,15 +208,35 @@ __device__ void plain_row(Group<NT>& g, const DistillP& p, size_t r, List& list,
   g.sync();
 }
 
-// A row's list into shared memory: entry j by the group's thread j
+// A row's list into shared memory, entry j by the group's thread j.  Synchronises the group.
 template <int NT, typename T>
 __device__ __forceinline__ void fetch_list(Group<NT>& g, const DistillP& p, size_t r, const T* x, int64_t st, List& list) {
-  for (uint32_t j = g.tid; j < p.top; j += NT) {
-    const uint32_t c = p.top_class[r * p.top + j];
+  if (g.tid == 0) list.twice = false;
+  for (uint32_t j = g.tid; j < kMostTop; j += NT) {
+    const uint32_t c = j < p.top ? p.top_class[r * p.top + j] : kNoClass;
     list.cls[j] = c;
-    list.a[j] = p.top_logit[r * p.top + j] * p.ts;
-    list.x[j] = c < p.x.C ? ld_f(x + c * st) : 0.f;
+    if (j < p.top) {
+      list.a[j] = p.top_logit[r * p.top + j] * p.ts;
+      list.x[j] = c < p.x.C ? ld_f(x + c * st) : 0.f;
+    }
   }
+  g.sync();
+  for (uint32_t j = g.tid; j < p.top; j += NT) {
+    const uint32_t c = list.cls[j];
+    uint32_t before = 0, all = 0;
+    for (uint32_t i = 0; i < p.top; i += 8) {
+      const uint4 lo = *(const uint4*)&list.cls[i], hi = *(const uint4*)&list.cls[i + 4];
+      const uint32_t v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+      for (uint32_t q = 0; q < 8; ++q) {
+        all += v[q] == c;
+        before += v[q] == c && i + q < j;
+      }
+    }
+    list.first[j] = before == 0;
+    if (all > 1 && c < p.x.C) list.twice = true;
+  }
+  g.sync();
 }
 
 template <typename T, bool BWD>
@@ -229,7 +249,6 @@ __global__ void __launch_bounds__(256) distill_any(DistillP p) {
   const size_t warp = ((size_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5, nw = ((size_t)gridDim.x * blockDim.x) >> 5;
   for (size_t r = warp; r < p.x.rows; r += nw) {
     fetch_list<32, T>(g, p, r, (const T*)p.logits + p.x.offset(r), p.x.step, lists[w]);
-    g.sync();
     plain_row<32, T, BWD>(g, p, r, lists[w], &shared[w]);
   }
 }
@@ -238,10 +257,10 @@ __global__ void __launch_bounds__(256) distill_any(DistillP p) {
 // NT 32: a warp per row, eight vectors per lane and batch.  NT 256: a block per row, or a cluster of blocks, four vectors.
 // REST: the classes of the list are left out of the pass.
 template <int NT, typename T, bool REST, bool BWD>
-__global__ void __launch_bounds__(256) distill_rows(DistillP p) {
-  constexpr int U = NT == 32 ? 8 : 4, V = Vec<T>::V;
+__global__ void __launch_bounds__(256) distill_rows(DistillP p, uint32_t slots) {
+  constexpr int U = Feed<NT>::U, V = Vec<T>::V;
   typedef Vec<T> X;
-  extern __shared__ __align__(16) uint8_t masks[];   // a byte per vector of the row's share (NT 32: of each warp's row)
+  extern __shared__ __align__(16) uint8_t dyn[];   // batches of vectors, then a byte per vector of the row's share (NT 32: of each warp's row)
   __shared__ Key red[kRowWarps];
   __shared__ Part parts[kRowWarps], whole;
   __shared__ List lists[NT == 32 ? kRowWarps : 1];
@@ -252,7 +271,7 @@ __global__ void __launch_bounds__(256) distill_rows(DistillP p) {
   Group<NT> g(red);
   const uint32_t C = p.x.C, warp = threadIdx.x >> 5, k = p.top;
   List& list = lists[NT == 32 ? warp : 0];
-  uint8_t* mask = masks + (NT == 32 ? (size_t)warp * ((C / V + 15) / 16 * 16) : 0);
+  uint8_t* mask = dyn + (size_t)slots * Feed<NT>::kBatch * 16 + (NT == 32 ? (size_t)warp * ((C / V + 15) / 16 * 16) : 0);
   const size_t row0 = NT == 32 ? (size_t)blockIdx.x * kRowWarps + warp : blockIdx.x / parts_n;
   const size_t rows_n = NT == 32 ? (size_t)gridDim.x * kRowWarps : gridDim.x / parts_n;
   for (size_t r = row0; r < p.x.rows; r += rows_n) {
@@ -262,7 +281,6 @@ __global__ void __launch_bounds__(256) distill_rows(DistillP p) {
     if (REST)
       for (uint32_t i = g.tid; i < (b.ve - b.vb + 15) / 16; i += NT) ((uint4*)mask)[i] = make_uint4(0, 0, 0, 0);
     fetch_list<NT, T>(g, p, r, x, 1, list);
-    g.sync();
     bool apart = true;   // this thread's single element is outside of the list
     const uint32_t sc = g.tid < 2 * V ? b.single(g.tid) : kNoClass;
     if (REST) {
@@ -280,14 +298,9 @@ __global__ void __launch_bounds__(256) distill_rows(DistillP p) {
     Part a;
     a.clear();
     if (sc != kNoClass && apart) a.add<false>(ld_f(x + sc), p.cs);
-    for (uint32_t v0 = b.vb; v0 < b.ve; v0 += U * NT) {
-      uint4 w[U];
+    Feed<NT> feed = {xv, b.vb, b.ve, g.tid, slots, (uint4*)dyn};
+    feed.template run<T, false>([&](uint32_t v0, uint4 (&w)[U]) {
       typename X::Max most;
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const uint32_t v = v0 + u * NT + g.tid;
-        w[u] = v < b.ve ? xv[v] : X::none();
-      }
       if (REST) {
         uint32_t out[U], any = 0;
 #pragma unroll
@@ -311,11 +324,7 @@ __global__ void __launch_bounds__(256) distill_rows(DistillP p) {
       }
 #pragma unroll
       for (int u = 0; u < U; ++u) most = u ? X::max(most, X::max(w[u])) : X::max(w[u]);
-      const float bm = X::value(most);
-      if (bm > a.m) {
-        a.m = bm;
-        a.refer<false>(fmaxf(a.mc, Part::reference(bm, p.cs)));
-      }
+      a.reach<false>(X::value(most), p.cs);
       float S[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int u = 0; u < U; ++u) {
@@ -326,19 +335,20 @@ __global__ void __launch_bounds__(256) distill_rows(DistillP p) {
         for (int i = 0; i < V; ++i) S[i & 3] += exp2_fast(fmaf(f[i], p.cs, -a.mc));
       }
       a.S += (S[0] + S[1]) + (S[2] + S[3]);
-    }
-    a.join_lanes<false>();
+    });
+    a.join<false, 32>(p.cs);
     if (NT != 32) {
       if ((g.tid & 31) == 0) parts[warp] = a;
       __syncthreads();
-      a = parts[0];
-#pragma unroll
-      for (int i = 1; i < kRowWarps; ++i) a.join<false>(parts[i]);
+      a = parts[g.tid % kRowWarps];
+      a.join<false, kRowWarps>(p.cs);
       if (parts_n > 1) {
         if (g.tid == 0) whole = a;
         cluster.sync();
-        a = *cluster.map_shared_rank(&whole, 0);
-        for (uint32_t q = 1; q < parts_n; ++q) a.join<false>(*cluster.map_shared_rank(&whole, q));
+        const uint32_t q = g.tid % 8;
+        if (q < parts_n) a = *cluster.map_shared_rank(&whole, q);
+        else a.clear();
+        a.join<false, 8>(p.cs);
       }
     }
     if (a.strange(p.cs)) {
@@ -371,13 +381,7 @@ __global__ void __launch_bounds__(256) distill_rows(DistillP p) {
       if (p.accumulate) g.sync();
       if (sc != kNoClass) st_f(o + sc, grad(ld_f(x + sc)) + (p.accumulate ? ld_f(o + sc) : 0.f));
       uint4* ov = (uint4*)(o + b.head);
-      for (uint32_t v0 = b.vb; v0 < b.ve; v0 += U * NT) {
-        uint4 w[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const uint32_t v = v0 + u * NT + g.tid;
-          if (v < b.ve) w[u] = xv[v];
-        }
+      feed.template run<T, true>([&](uint32_t v0, const uint4 (&w)[U]) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           const uint32_t v = v0 + u * NT + g.tid;
@@ -400,7 +404,7 @@ __global__ void __launch_bounds__(256) distill_rows(DistillP p) {
             for (int i = 0; i < V; ++i) st_f(os + i, p.accumulate ? h[i] + ld_f(os + i) : h[i]);
           }
         }
-      }
+      });
       g.sync();
 #pragma unroll
       for (int i = 0; i < (NT == 32 ? 4 : 1); ++i) {
@@ -474,16 +478,14 @@ __global__ void __launch_bounds__(kPositions) distill_positions(DistillP p) {
           for (int i = 0; i < 8; ++i) f[i] = w >> i & 1u ? -INFINITY : f[i];
         }
         bm = fmaxf(fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3])), fmaxf(fmaxf(f[4], f[5]), fmaxf(f[6], f[7])));
-        if (bm > a.m) {
-          a.m = bm;
-          a.refer<false>(fmaxf(a.mc, Part::reference(bm, p.cs)));
-        }
+        a.reach<false>(bm, p.cs);
         float S[2] = {0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < 8; ++i) S[i & 1] += exp2_fast(fmaf(f[i], p.cs, -a.mc));
         a.S += S[0] + S[1];
       }
       const bool strange = a.strange(p.cs);
+      a.refer<false>(Part::reference(a.m, p.cs));
       float off = a.m == -INFINITY ? 0.f : fmaf(-a.m, p.cs, a.mc);
       if (strange) {
         off = a.S = 0.f;
@@ -575,14 +577,16 @@ static int distill_args(const ad_distill_args* a, bool bwd, DistillP& p) {
 
 
 template <int NT, typename T, bool REST, bool BWD>
-static int launch_rows(const DistillP& p, uint32_t n, size_t smem, cudaStream_t s) {
+static int launch_rows(const DistillP& p, uint32_t n, size_t mask, cudaStream_t s) {
   auto kernel = distill_rows<NT, T, REST, BWD>;
+  const uint32_t slots = NT == 32 ? 0 : feed_slots((size_t)p.x.C * sizeof(T), n, BWD ? kMostFeed : 0);
+  const size_t smem = slots * Feed<NT>::kBatch * 16 + mask;
   // the limit belongs to the function: the most that it takes
-  if (smem > 32 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMostMask) != cudaSuccess) {
+  if (smem > 32 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kMostFeed + kMostMask)) != cudaSuccess) {
     cudaGetLastError();
     return AD_ERR_CUDA;
   }
-  launch_row_kernel(kernel, p, NT == 32 ? (p.x.rows + kRowWarps - 1) / kRowWarps : p.x.rows, n, smem, s);
+  launch_row_kernel(kernel, p, slots, NT == 32 ? (p.x.rows + kRowWarps - 1) / kRowWarps : p.x.rows, n, smem, s);
   return AD_OK;
 }
 

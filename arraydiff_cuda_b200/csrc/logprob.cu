@@ -33,15 +33,26 @@ struct TopMem {
   Key *list, *cand;   // the result, in order; what is at or in front of the bound
   uint32_t cap, *n;   // room in cand, and how many there are (more than cap: not all are there)
   __host__ __device__ static constexpr uint32_t room(uint32_t k) { return 64 + 9 * k; }   // k vectors of equal elements and the single ones fit
-  __device__ void push(float v, uint32_t c) {
+  __device__ void push(float v, uint32_t c) const {
     const uint32_t at = atomicAdd(n, 1u);
     if (at < cap) cand[at] = key_of(v, c);
   }
 };
 
-// Of 256 shares, eight per lane (value key, 0 for none, and class): the k-th by value, then class.  value 0: fewer than k.
+// One warp: of 256 shares' maxima, eight per lane (keys, 0 for none), the k-th, or less; 0: fewer than k
 template <int SHIFT>
-__device__ void kth_share(const uint32_t (&kv)[8], const uint32_t (&kc)[8], uint32_t k, uint32_t& value, uint32_t& cls) {
+__device__ uint32_t kth_share(const uint32_t (&kv)[8], uint32_t k, uint32_t* mem) {
+  if (k <= 16) {   // the k-th of the lanes' largest: little less
+    uint32_t best = kv[0], at = 0;
+#pragma unroll
+    for (int i = 1; i < 8; ++i) best = max(best, kv[i]);
+    mem[threadIdx.x & 31] = best;
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 32; ++i) at += mem[i] > best;
+    __syncwarp();
+    return __reduce_min_sync(0xffffffffu, at < k ? best : 0xffffffffu);
+  }
   uint32_t t = 0;
   for (uint32_t bit = 1u << (31 - SHIFT); bit; bit >>= 1) {
     uint32_t n = 0;
@@ -49,23 +60,7 @@ __device__ void kth_share(const uint32_t (&kv)[8], const uint32_t (&kc)[8], uint
     for (int i = 0; i < 8; ++i) n += (kv[i] >> SHIFT) >= (t | bit);
     if (__reduce_add_sync(0xffffffffu, n) >= k) t |= bit;
   }
-  uint32_t over = 0, same = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) { over += (kv[i] >> SHIFT) > t; same += (kv[i] >> SHIFT) == t; }
-  over = __reduce_add_sync(0xffffffffu, over);
-  same = __reduce_add_sync(0xffffffffu, same);
-  value = t == 0 ? 0u : SHIFT ? t << SHIFT | (t >> (31 - SHIFT) ? 0u : (1u << SHIFT) - 1) : t;   // the bits that a key's sign tells
-  cls = kNoClass;
-  if (t != 0 && over + same > k) {
-    uint32_t u = 0;
-    for (uint32_t bit = 1u << 30; bit; bit >>= 1) {
-      uint32_t n = 0;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) n += (kv[i] >> SHIFT) == t && kc[i] < (u | bit);
-      if (over + __reduce_add_sync(0xffffffffu, n) < k) u |= bit;
-    }
-    cls = u;
-  }
+  return t == 0 ? 0u : SHIFT ? t << SHIFT | (t >> (31 - SHIFT) ? 0u : (1u << SHIFT) - 1) : t;   // the bits that a key's sign tells
 }
 
 // The list out of the candidates: each one's place is the number of those in front of it
@@ -107,6 +102,134 @@ __device__ void rounds(Group<NT>& g, const TopMem& t, const T* x, int64_t st, ui
     if (g.tid == 0) t.list[i] = best;
   }
   g.sync();
+}
+
+// One warp: pushes the elements of a strip that equal v, in order of their classes, until there are r of them
+template <typename T>
+__device__ void push_equal(const TopMem& t, const Strip<T>& b, const T* x, float v, uint32_t r) {
+  constexpr uint32_t V = Vec<T>::V;
+  const uint32_t lane = threadIdx.x & 31;
+  uint32_t have = 0;
+  for (uint32_t c0 = b.begin(); c0 < b.end() && have < r; c0 += 32 * V) {
+    uint32_t n = 0, hits = 0;
+    for (uint32_t i = 0; i < V; ++i) {
+      const uint32_t c = c0 + lane * V + i;
+      if (c < b.end() && ld_f(x + c) == v) { hits |= 1u << i; ++n; }
+    }
+    uint32_t before = n;   // of the lanes up to this one
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t q = __shfl_up_sync(0xffffffffu, before, o);
+      if (lane >= (uint32_t)o) before += q;
+    }
+    uint32_t at = have + before - n;
+    for (uint32_t i = 0; i < V; ++i)
+      if (hits >> i & 1 && at++ < r) t.push(v, c0 + lane * V + i);
+    have += __shfl_sync(0xffffffffu, before, 31);
+  }
+  __syncwarp();
+}
+
+// The maxima of what a thread has taken at a time: batches of four vectors, `1 << shift` of them together, as the upper
+// half of the number.  [slot][thread]; none: a share's vectors are looked at one by one.
+struct Maxima {
+  const uint16_t* m;
+  uint32_t shift, slots;
+};
+constexpr uint32_t kMostSlots = 16;
+__device__ __forceinline__ uint32_t half_key(uint32_t h) { return h & 0x8000u ? 0xffffu ^ h : h | 0x8000u; }   // value_key >> 16
+
+// One warp: a strip's list out of its 256 shares, of which lane i has number 32 j + i in kv[j]: the key of its largest value, 0
+// for none.  Share s is the vectors vb + s + 256 n, xv[0] being vector vb.  `single`: a single element of the strip in this
+// lane (class `sc`).  work: 256 words of 16 bits, with maxima 2048.
+template <typename T>
+__device__ void select_top(const TopMem& t, uint32_t k, const uint32_t (&kv)[8], const Maxima& mx, const Strip<T>& b, const T* x, const uint4* xv, uint32_t sc,
+                           float single, uint16_t* work) {
+  typedef Vec<T> X;
+  constexpr int V = X::V;
+  constexpr uint32_t kWork = 2048;
+  Group<32> g(nullptr);
+  const uint32_t lane = g.tid, below = (1u << lane) - 1;
+  const uint32_t tv = kth_share<X::kKeyShift>(kv, k, (uint32_t*)t.cand);
+  const float bound = tv ? key_value(tv) : -INFINITY;
+  const uint32_t nv = b.ve - b.vb, per = mx.m ? mx.slots : (nv + 255) / 256;
+  // all elements of the shares that reach the bound; where that is too many, those above it, and of the equal ones the first
+  for (int strict = 0; strict < 2; ++strict) {
+    auto reaches = [&](float v) { return strict ? v > bound : v >= bound; };
+    if (lane == 0) *t.n = 0;
+    uint32_t ns = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const bool in = kv[i] && (strict ? kv[i] > tv : kv[i] >= tv);
+      const uint32_t who = __ballot_sync(0xffffffffu, in);
+      if (in) work[ns + __popc(who & below)] = (uint16_t)(i * 32 + lane);
+      ns += __popc(who);
+    }
+    __syncwarp();
+    uint32_t vectors = ns * per;   // of the shares, or (maxima) of their slots that reach it
+    uint16_t* list = work + 256;
+    if (mx.m) {
+      uint32_t n = 0;
+      for (uint32_t i0 = 0; i0 < ns * per; i0 += 32) {
+        const uint32_t i = i0 + lane, s = i / per, slot = i - s * per;
+        bool in = false;
+        uint16_t at = 0;
+        if (i < ns * per) {
+          at = (uint16_t)(slot * 256 + work[s]);
+          in = half_key(mx.m[at]) >= tv >> 16;
+        }
+        const uint32_t who = __ballot_sync(0xffffffffu, in);
+        if (in && n + __popc(who & below) < kWork - 256) list[n + __popc(who & below)] = at;
+        n += __popc(who);
+      }
+      if (n > kWork - 256 && !strict) continue;
+      if (n > kWork - 256) n = 0, *t.n = t.cap + 1;
+      vectors = n * (4u << mx.shift);
+      __syncwarp();
+    }
+    for (uint32_t i0 = 0; i0 < vectors; i0 += 128) {   // four loads at a time
+      uint4 w[4];
+      uint32_t at[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const uint32_t i = i0 + q * 32 + lane;
+        uint32_t v = nv;
+        if (i < vectors) {
+          if (mx.m) {
+            const uint32_t e = list[i >> (2 + mx.shift)], sub = i & ((4u << mx.shift) - 1);
+            v = (((e >> 8) << (2 + mx.shift)) + sub) * 256 + (e & 255);
+          } else {
+            const uint32_t s = i / per;
+            v = (i - s * per) * 256 + work[s];
+          }
+        }
+        at[q] = v;
+        w[q] = v < nv ? xv[v] : X::none();
+      }
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        if (at[q] < nv && reaches(X::value(X::max(w[q])))) {
+          float f[V];
+          X::unpack(w[q], f);
+#pragma unroll
+          for (int j = 0; j < V; ++j)
+            if (reaches(f[j])) t.push(f[j], b.class_of(b.vb + at[q]) + j);
+        }
+      if (__any_sync(0xffffffffu, *(volatile uint32_t*)t.n > t.cap)) break;
+    }
+    if (sc != kNoClass && reaches(single)) t.push(single, sc);
+    __syncwarp();
+    const uint32_t n = *t.n;
+    if (n <= t.cap && strict) {
+      if (n < k) push_equal<T>(t, b, x, bound, k - n);
+    }
+    if (n <= t.cap) {
+      sort_candidates<32>(g, t, *t.n, k);
+      return;
+    }
+    __syncwarp();
+  }
+  rounds<32, T>(g, t, x, 1, b.begin(), b.end(), k);
 }
 
 __device__ __forceinline__ void put_top(const LogprobP& p, const RowSums& s, size_t r, uint32_t at, Key key) {
@@ -171,24 +294,109 @@ __global__ void __launch_bounds__(256) logprob_any(LogprobP p) {
 }
 
 // ---------------------------------------------------------------- rows of many neighbouring classes
-// NT 32: a warp per row, eight vectors per lane and batch.  NT 256: a block per row, or a cluster of blocks, four vectors.
+// What a thread finds in its vectors: sums, classes in front of the label, its shares of the row
+template <int NT, typename T, bool ENT, bool RANK, bool TOP>
+struct Scan {
+  static constexpr int U = NT == 32 ? 8 : 4, SH = NT == 32 ? 8 : 1;
+  typedef Vec<T> X;
+  Part a;
+  uint32_t km[SH];   // maxima of the eight shares of a lane, as keys; a thread's own share has a.m
+  __device__ void clear() {
+    a.clear();
+#pragma unroll
+    for (int i = 0; i < SH; ++i) km[i] = 0;
+  }
+  // v0: the first vector of the batch, lv: the label's; before that one counts what is above thr0, else what is above xl.
+  // The batch's maximum.
+  __device__ __forceinline__ float batch(uint32_t v0, const uint4 (&w)[U], bool full, const Strip<T>& b, uint32_t tid, float cs, float nothing, uint32_t lv, float xl, float thr0) {
+    typename X::Max mx[U], most;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      mx[u] = X::max(w[u]);
+      most = u ? X::max(most, mx[u]) : mx[u];
+    }
+    const float bm = X::value(most);
+    if (TOP && SH > 1) {
+#pragma unroll
+      for (int u = 0; u < SH; ++u)
+        if (v0 + u * NT + tid < b.ve) km[u] = max(km[u], value_key(X::value(mx[u])));
+    }
+    add_vectors<ENT, U, T>(a, w, full ? U : (int)((b.ve - v0 + NT - 1) / NT), bm, cs, nothing);
+    if (RANK && bm >= xl) {   // few batches hold something above a likely label
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const uint32_t v = v0 + u * NT + tid;
+        if (full || v < b.ve) a.cnt += X::above(w[u], v < lv ? thr0 : xl);
+      }
+    }
+    return bm;
+  }
+};
+// A label and what the rank's counting needs of it
+template <typename T>
+struct Label {
+  uint32_t l, lv;
+  float xl, thr0;
+  bool low;   // its logit is -inf, nothing is below: all classes in front of it count, whatever they hold
+  __device__ void fetch(const LogprobP& p, size_t r, const T* x, const Strip<T>& b) {
+    l = p.label ? p.label[r] : kNoClass;
+    xl = l < p.x.C ? ld_f(x + l) : 0.f;
+    low = xl == -INFINITY;
+    lv = l < b.head ? 0 : (l - b.head) / Vec<T>::V;
+    thr0 = low ? INFINITY : Vec<T>::below(xl);
+  }
+  // what the counting by vectors leaves out: lane i looks at the i-th element of the label's own vector
+  __device__ uint32_t own_vector(const Strip<T>& b, const T* x, uint32_t C, uint32_t i) const {
+    if (l >= C || l < b.head || lv < b.vb || lv >= b.ve || b.class_of(lv) + i >= l || i >= Vec<T>::V) return 0;
+    const float v = ld_f(x + b.class_of(lv) + i);
+    return low ? 0u - (v > xl) : (uint32_t)(v == xl);
+  }
+  __device__ bool single_counts(float v, uint32_t c) const { return low ? c > l && v > xl : in_front(v, c, xl, l); }
+  __device__ uint32_t rank(uint32_t cnt, uint32_t C) const { return l < C ? cnt + (low ? l : 0u) : kNoClass; }
+};
+// The gradient's factors: e (c0 + c1 u) with e = 2^u is scale p (A - dentropy (log p + H)); dl: what the label's class has besides
+struct Factors {
+  float c0, c1, dl, dh, dz;
+  __device__ void fetch(const LogprobP& p, size_t r, uint32_t l) {
+    dl = p.dlogp && l < p.x.C ? p.dlogp[r] : 0.f;
+    dh = p.dentropy ? p.dentropy[r] : 0.f;
+    dz = p.dlse ? p.dlse[r] : 0.f;
+  }
+  template <bool ENT> __device__ void set(const LogprobP& p, const RowSums& s, float H) {
+    if (!s.some) dl = 0.f;
+    const float A = dz - dl, k = s.some ? p.scale / s.S : 0.f;
+    c1 = ENT ? -k * dh * kLn2 : 0.f;
+    c0 = ENT ? k * (A - dh * (H - kLn2 * s.L)) : k * A;
+    dl *= p.scale;
+  }
+  template <bool ENT> __device__ float grad(float x, float cs, float mc) const {
+    float u = fmaf(x, cs, -mc);
+    if (ENT) u = above_nothing(u);
+    return exp2_fast(u) * (ENT ? fmaf(c1, u, c0) : c0);
+  }
+};
+
+// NT 32: a warp per row, eight vectors per lane and batch.  NT 256: for few rows, a block or a cluster of blocks per row.
 // ENT: the entropy is asked for.  RANK: the label's rank.  TOP: top classes.  BWD: the gradient.
 template <int NT, typename T, bool ENT, bool RANK, bool TOP, bool BWD>
-__global__ void __launch_bounds__(256) logprob_rows(LogprobP p) {
-  constexpr int U = NT == 32 ? 8 : 4, SH = NT == 32 ? 8 : 1, V = Vec<T>::V;
+__global__ void __launch_bounds__(256) logprob_rows(LogprobP p, uint32_t slots) {
+  typedef Scan<NT, T, ENT, RANK, TOP> S;
+  constexpr int U = S::U, V = Vec<T>::V;
   typedef Vec<T> X;
-  extern __shared__ Key dyn[];
+  extern __shared__ __align__(16) Key dyn[];   // batches of vectors, then what the top classes need
   __shared__ Key red[kRowWarps];
   __shared__ Part parts[kRowWarps], whole;
-  __shared__ uint32_t sv[NT == 32 ? 1 : 256], sc[NT == 32 ? 1 : 256], bound[2], flagged[kMostTop], count[kRowWarps], nflag;
+  __shared__ uint32_t sv[NT == 32 ? 1 : 256], count[kRowWarps];
+  __shared__ uint16_t work[NT == 32 ? kRowWarps : 1][TOP ? 256 : 1];
   grid_dependency();
   cg::cluster_group cluster = cg::this_cluster();
   const uint32_t parts_n = NT == 32 ? 1 : cluster.num_blocks(), part = NT == 32 ? 0 : cluster.block_rank();
   Group<NT> g(red);
   const uint32_t C = p.x.C, warp = threadIdx.x >> 5;
+  const float nothing = as_nothing(p.cs);
   TopMem t = {nullptr, nullptr, TopMem::room(p.top), &count[NT == 32 ? warp : 0]};
   if (TOP) {
-    t.list = dyn + (NT == 32 ? (size_t)warp * (p.top + t.cap) : 0);
+    t.list = dyn + (size_t)slots * Feed<NT>::kBatch * 2 + (NT == 32 ? (size_t)warp * (p.top + t.cap) : 0);
     t.cand = t.list + p.top;
   }
   const size_t row0 = NT == 32 ? (size_t)blockIdx.x * kRowWarps + warp : blockIdx.x / parts_n;
@@ -197,104 +405,31 @@ __global__ void __launch_bounds__(256) logprob_rows(LogprobP p) {
     const T* x = (const T*)p.logits + p.x.offset(r);
     const Strip<T> b(x, C, part, parts_n);
     const uint4* xv = (const uint4*)(x + b.head);
-    const uint32_t l = p.label ? p.label[r] : kNoClass;
-    const float xl = l < C ? ld_f(x + l) : 0.f;
-    // vectors in front of the label's count what is at least its logit, the others what is above it
-    const bool low = xl == -INFINITY;   // there is nothing below: all classes in front of it count, whatever they hold
-    const uint32_t lv = l < b.head ? 0 : (l - b.head) / V;
-    const float thr0 = low ? INFINITY : X::below(xl);
-    Part a;
-    a.clear();
-    float km[SH];
-    uint32_t kc[SH];
-#pragma unroll
-    for (int i = 0; i < SH; ++i) { km[i] = -INFINITY; kc[i] = kNoClass; }
-    if (g.tid < 2 * V) {
-      const uint32_t c = b.single(g.tid);
-      if (c != kNoClass) {
-        const float v = ld_f(x + c);
-        a.add<ENT>(v, p.cs);
-        if (RANK) a.cnt += low ? c > l && v > xl : in_front(v, c, xl, l);
-      }
-    }
-    for (uint32_t v0 = b.vb; v0 < b.ve; v0 += U * NT) {
-      uint4 w[U];
-      typename X::Max mx[U], most;
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const uint32_t v = v0 + u * NT + g.tid;
-        w[u] = v < b.ve ? xv[v] : X::none();
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        mx[u] = X::max(w[u]);
-        most = u ? X::max(most, mx[u]) : mx[u];
-      }
-      const float bm = X::value(most);
-      if (TOP && SH > 1) {
-#pragma unroll
-        for (int u = 0; u < SH; ++u) {
-          const float m = X::value(mx[u]);
-          const uint32_t v = v0 + u * NT + g.tid;
-          if (v < b.ve && (m > km[u] || kc[u] == kNoClass)) { km[u] = m; kc[u] = b.class_of(v); }
-        }
-      }
-      if (TOP && SH == 1 && (bm > km[0] || kc[0] == kNoClass)) {
-        km[0] = bm;
-#pragma unroll
-        for (int u = U - 1; u >= 0; --u) {
-          const uint32_t v = v0 + u * NT + g.tid;
-          if (v < b.ve && X::value(mx[u]) == bm) kc[0] = b.class_of(v);
-        }
-      }
-      if (bm > a.m) {
-        a.m = bm;
-        a.refer<ENT>(fmaxf(a.mc, Part::reference(bm, p.cs)));
-      }
-      float S[4] = {0.f, 0.f, 0.f, 0.f}, E[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (v0 + u * NT >= b.ve) break;
-        float f[V];
-        X::unpack(w[u], f);
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          float z = fmaf(f[i], p.cs, -a.mc);
-          if (ENT) z = above_nothing(z);
-          const float e = exp2_fast(z);
-          S[i & 3] += e;
-          if (ENT) E[i & 3] = fmaf(e, z, E[i & 3]);
-        }
-        if (RANK) {
-          const uint32_t v = v0 + u * NT + g.tid;
-          if (v < b.ve) a.cnt += X::above(w[u], v < lv ? thr0 : xl);
-        }
-      }
-      a.S += (S[0] + S[1]) + (S[2] + S[3]);
-      if (ENT) a.E += (E[0] + E[1]) + (E[2] + E[3]);
-    }
-    if (RANK && l < C && l >= b.head && lv >= b.vb && lv < b.ve && g.tid == 0)   // the label's own vector: the elements in front of it
-      for (uint32_t c = b.class_of(lv); c < l; ++c) {
-        const float v = ld_f(x + c);
-        if (low) a.cnt -= v > xl;
-        else a.cnt += v == xl;
-      }
-    a.join_lanes<ENT>();
+    Feed<NT> feed = {xv, b.vb, b.ve, g.tid, slots, (uint4*)dyn};
+    S scan;
+    scan.clear();
+    Part& a = scan.a;
+    const uint32_t cls = g.tid < 2 * V ? b.single(g.tid) : kNoClass;
+    const float single = cls != kNoClass ? ld_f(x + cls) : 0.f;
+    Label<T> label;
+    label.fetch(p, r, x, b);
+    feed.template run<T, false>([&](uint32_t v0, const uint4 (&w)[U]) { scan.batch(v0, w, false, b, g.tid, p.cs, nothing, label.lv, label.xl, label.thr0); });
+    if (TOP && NT != 32) sv[g.tid] = b.vb + g.tid < b.ve ? value_key(a.m) : 0u;
+    if (cls != kNoClass) a.add<ENT>(single, p.cs);
+    if (RANK) a.cnt += label.own_vector(b, x, C, g.tid) + (cls != kNoClass && label.single_counts(single, cls));
+    a.join<ENT, 32>(p.cs);
     if (NT != 32) {
       if ((g.tid & 31) == 0) parts[warp] = a;
-      if (TOP) {
-        sv[g.tid] = kc[0] == kNoClass ? 0u : value_key(km[0]);
-        sc[g.tid] = kc[0];
-      }
       __syncthreads();
-      a = parts[0];
-#pragma unroll
-      for (int i = 1; i < kRowWarps; ++i) a.join<ENT>(parts[i]);
+      a = parts[g.tid % kRowWarps];
+      a.join<ENT, kRowWarps>(p.cs);
       if (parts_n > 1) {
         if (g.tid == 0) whole = a;
         cluster.sync();
-        a = *cluster.map_shared_rank(&whole, 0);
-        for (uint32_t q = 1; q < parts_n; ++q) a.join<ENT>(*cluster.map_shared_rank(&whole, q));
+        const uint32_t q = g.tid % 8;
+        if (q < parts_n) a = *cluster.map_shared_rank(&whole, q);
+        else a.clear();
+        a.join<ENT, 8>(p.cs);
       }
     }
     if (a.strange(p.cs)) {
@@ -307,75 +442,20 @@ __global__ void __launch_bounds__(256) logprob_rows(LogprobP p) {
     s.set(a.m, a.mc, a.S, p.cs);
     const float H = s.some ? kLn2 * (s.L - a.E / s.S) : 0.f;
     if (g.tid == 0 && part == 0) {
-      put_row(p, s, r, H, l, xl);
-      if (RANK) p.rank[r] = l < C ? a.cnt + (low ? l : 0u) : kNoClass;
+      put_row(p, s, r, H, label.l, label.xl);
+      if (RANK) p.rank[r] = label.rank(a.cnt, C);
     }
     if constexpr (TOP) {
       const uint32_t k = p.top;
-      uint32_t tv, tc;
-      if (NT == 32) {
+      if (NT == 32 || warp == 0) {
         uint32_t kv[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) kv[i] = kc[i % SH] == kNoClass ? 0u : value_key(km[i % SH]);
-        uint32_t cc[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) cc[i] = kc[i % SH];
-        kth_share<X::kKeyShift>(kv, cc, k, tv, tc);
-        if (g.tid == 0) *t.n = 0;
-        g.sync();
-        const float least = tv ? key_value(tv) : -INFINITY;
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (kv[i] > tv || (kv[i] == tv && cc[i] <= tc && kv[i])) {
-            for (uint32_t v = b.vb + i * 32 + g.tid; v < b.ve; v += 256) {
-              float f[V];
-              X::unpack(xv[v], f);
-              const uint32_t c0 = b.class_of(v);
-#pragma unroll
-              for (int j = 0; j < V; ++j)
-                if (f[j] > least || (f[j] == least && c0 <= tc)) t.push(f[j], c0 + j);
-            }
-          }
-      } else {
-        if (warp == 0) {
-          uint32_t kv[8], cc[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) { kv[i] = sv[i * 32 + g.tid]; cc[i] = sc[i * 32 + g.tid]; }
-          kth_share<X::kKeyShift>(kv, cc, k, tv, tc);
-          if (g.tid == 0) { bound[0] = tv; bound[1] = tc; *t.n = 0; nflag = 0; }
-        }
-        __syncthreads();
-        tv = bound[0];
-        tc = bound[1];
-        const uint32_t mine = sv[g.tid];
-        if (mine > tv || (mine == tv && sc[g.tid] <= tc && mine)) flagged[atomicAdd(&nflag, 1u)] = g.tid;
-        __syncthreads();
-        const float least = tv ? key_value(tv) : -INFINITY;
-        const uint32_t per = (b.ve - b.vb + NT - 1) / NT;
-        // the shares' vectors, over all threads
-        for (uint32_t i = g.tid; i < nflag * per; i += NT) {
-          const uint32_t v = b.vb + i % per * NT + flagged[i / per];
-          if (v >= b.ve) continue;
-          float f[V];
-          X::unpack(xv[v], f);
-          const uint32_t c0 = b.class_of(v);
-#pragma unroll
-          for (int j = 0; j < V; ++j)
-            if (f[j] > least || (f[j] == least && c0 <= tc)) t.push(f[j], c0 + j);
-        }
+        for (int i = 0; i < 8; ++i) kv[i] = NT == 32 ? scan.km[i % S::SH] : sv[i * 32 + g.tid];
+        const Maxima none = {nullptr, 0, 0};
+        select_top<T>(t, k, kv, none, b, x, xv + b.vb, cls, single, work[NT == 32 ? warp : 0]);
       }
-      if (g.tid < 2 * V) {
-        const uint32_t c = b.single(g.tid);
-        if (c != kNoClass) {
-          const float v = ld_f(x + c), least = tv ? key_value(tv) : -INFINITY;
-          if (v > least || (v == least && c <= tc)) t.push(v, c);
-        }
-      }
-      g.sync();
-      const uint32_t n = *t.n;
-      if (n <= t.cap) sort_candidates<NT>(g, t, n, k);
-      else rounds<NT, T>(g, t, x, 1, b.begin(), b.end(), k);
       if (parts_n == 1) {
+        g.sync();
         for (uint32_t i = g.tid; i < k; i += NT) put_top(p, s, r, i, t.list[i]);
       } else {
         // every block's list is in order: an entry's place in the row's is its own and those in front of it in the others
@@ -400,63 +480,215 @@ __global__ void __launch_bounds__(256) logprob_rows(LogprobP p) {
       }
     }
     if constexpr (BWD) {
-      const float dl = p.dlogp && l < C && s.some ? p.dlogp[r] : 0.f, dh = p.dentropy ? p.dentropy[r] : 0.f;
-      const float A = (p.dlse ? p.dlse[r] : 0.f) - dl, k = s.some ? p.scale / s.S : 0.f;
-      // e (c0 + c1 u) with e = 2^u: scale p (A - dentropy (log p + H))
-      const float c1 = ENT ? -k * dh * kLn2 : 0.f, c0 = ENT ? k * (A - dh * (H - kLn2 * s.L)) : k * A;
+      Factors f;
+      f.fetch(p, r, label.l);
+      f.set<ENT>(p, s, H);
       T* o = (T*)p.dlogits + p.g.offset(r);
       const bool even = (((uintptr_t)o ^ (uintptr_t)x) & 15u) == 0;   // both have their vectors at the same classes
-      auto grad = [&](float v) {
-        float u = fmaf(v, p.cs, -s.mc);
-        if (ENT) u = above_nothing(u);
-        return exp2_fast(u) * (ENT ? fmaf(c1, u, c0) : c0);
-      };
       // the label's class is written last, over what the loop wrote
-      const bool mine = l < C && l >= b.begin() && l < b.end() && g.tid == 0;
+      const bool mine = label.l < C && label.l >= b.begin() && label.l < b.end() && g.tid == 0;
       float gl = 0.f;
-      if (mine) gl = grad(xl) + p.scale * dl + (p.accumulate ? ld_f(o + l) : 0.f);
+      if (mine) gl = f.grad<ENT>(label.xl, p.cs, s.mc) + f.dl + (p.accumulate ? ld_f(o + label.l) : 0.f);
       if (parts_n == 1) g.sync();   // its logit has been read by all, and what it adds to (a cluster has met already)
       else __syncthreads();
-      if (g.tid < 2 * V) {
-        const uint32_t c = b.single(g.tid);
-        if (c != kNoClass) st_f(o + c, grad(ld_f(x + c)) + (p.accumulate ? ld_f(o + c) : 0.f));
-      }
-      uint4* ov = (uint4*)(o + b.head);
-      for (uint32_t v0 = b.vb; v0 < b.ve; v0 += U * NT) {
-        uint4 w[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const uint32_t v = v0 + u * NT + g.tid;
-          if (v < b.ve) w[u] = xv[v];
-        }
+      if (cls != kNoClass) st_f(o + cls, f.grad<ENT>(single, p.cs, s.mc) + (p.accumulate ? ld_f(o + cls) : 0.f));
+      feed.template run<T, true>([&](uint32_t v0, const uint4 (&w)[U]) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           const uint32_t v = v0 + u * NT + g.tid;
           if (v >= b.ve) break;
-          float f[V];
-          X::unpack(w[u], f);
-#pragma unroll
-          for (int i = 0; i < V; ++i) f[i] = grad(f[i]);
-          if (even) {
-            if (p.accumulate) {
-              float d[V];
-              X::unpack(ov[v], d);
-#pragma unroll
-              for (int i = 0; i < V; ++i) f[i] += d[i];
-            }
-            ov[v] = X::pack(f);
-          } else {
-            T* os = o + b.class_of(v);
-#pragma unroll
-            for (int i = 0; i < V; ++i) st_f(os + i, p.accumulate ? f[i] + ld_f(os + i) : f[i]);
-          }
+          float h[V];
+          grad_vector<ENT, T>(w[u], h, p.cs, s.mc, f.c0, f.c1, nothing);
+          put_vector<T>(o + b.class_of(v), even, p.accumulate, h);
         }
-      }
+      });
       g.sync();
-      if (mine) st_f(o + l, gl);
+      if (mine) st_f(o + label.l, gl);
     }
     if (parts_n > 1) cluster.sync();   // what the others read of this block's
     else g.sync();
+  }
+}
+
+// Batches whose maxima share a slot: at most kMostSlots of them for a row
+template <typename T>
+__host__ __device__ inline uint32_t slot_shift(uint32_t C) {
+  uint32_t s = 0;
+  while ((C / Vec<T>::V + (1024u << s) - 1) / (1024u << s) > kMostSlots) ++s;
+  return s;
+}
+// Many rows of many classes: see Stream.  Two rows are in hand, by parity.
+template <typename T>
+struct LogprobSlot {
+  Label<T> label;
+  Part parts[kRowWarps];
+  uint32_t sv[256];
+  Factors f;
+  float mc;
+  bool strange;
+};
+template <typename T, bool ENT, bool RANK, bool TOP, bool BWD>
+__global__ void __launch_bounds__(kStreamThreads, kStreamBlocks) logprob_stream(LogprobP p) {
+  typedef Scan<kRowThreads, T, ENT, RANK, TOP> S;
+  typedef Stream<T, BWD> Str;
+  constexpr int U = Str::U, V = Vec<T>::V;
+  extern __shared__ __align__(16) uint4 ring[];   // batches of vectors, then what the top classes need
+  __shared__ LogprobSlot<T> slot[2];
+  __shared__ Key red[kRowWarps];
+  __shared__ uint32_t count;
+  __shared__ uint16_t work[TOP ? 2048 : 1];
+  grid_dependency();
+  const uint32_t shift = slot_shift<T>(p.x.C), slots = (p.x.C / V + (Str::kBatch << shift) - 1) / (Str::kBatch << shift);
+  uint16_t* maxima = (uint16_t*)(ring + Str::kAhead * Str::kBatch);   // [2][slots][256]
+  const uint32_t C = p.x.C, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const float nothing = as_nothing(p.cs);
+  if (warp < kRowWarps) {
+    Str stream((const T*)p.logits, p.x, ring);
+    uint32_t i = 0;
+    for (size_t r = blockIdx.x; r < p.x.rows; r += gridDim.x, ++i) {
+      LogprobSlot<T>& q = slot[i & 1];
+      const T* x = (const T*)p.logits + p.x.offset(r);
+      const Strip<T> b(x, C);
+      bar_wait(kBarReady + (i & 1));
+      const uint32_t lv = q.label.lv;
+      const float xl = q.label.xl, thr0 = q.label.thr0;
+      S scan;
+      scan.clear();
+      uint16_t* mine = maxima + (i & 1) * slots * 256 + tid;
+      float most = -INFINITY;
+      stream.run(b.nv, [&](uint32_t v0, const uint4 (&w)[U], bool full) {
+        const float bm = scan.batch(v0, w, full, b, tid, p.cs, nothing, lv, xl, thr0);
+        if (TOP) {   // the slot's maximum so far
+          const uint32_t n = v0 / Str::kBatch;
+          most = (n & ((1u << shift) - 1)) ? fmaxf(most, bm) : bm;
+          mine[(n >> shift) * 256] = (uint16_t)(__float_as_uint(most + 0.f) >> 16);
+        }
+      });
+      if (TOP) q.sv[tid] = tid < b.nv ? value_key(scan.a.m) : 0u;
+      scan.a.template join<ENT, 32>(p.cs);
+      if (lane == 0) q.parts[warp] = scan.a;
+      bar_arrive(kBarSums + (i & 1));
+      if constexpr (BWD) {
+        bar_wait(kBarResult + (i & 1));
+        T* o = (T*)p.dlogits + p.g.offset(r);
+        const bool even = (((uintptr_t)o ^ (uintptr_t)x) & 15u) == 0, plain = q.strange;
+        const Factors f = q.f;
+        const float mc = q.mc;
+        // the thread that has the label's vector writes its class once more
+        const uint32_t l = q.label.l < C && q.label.l >= b.head && lv < b.nv && lv % kRowThreads == tid ? lv : kNoClass;
+        const float gl = f.grad<ENT>(xl, p.cs, mc) + f.dl, old = l != kNoClass && p.accumulate ? ld_f(o + q.label.l) : 0.f;
+        T* to = o + b.head + tid * V;   // this thread's vector of the batch
+        stream.run(b.nv, [&](uint32_t v0, const uint4 (&w)[U], bool full) {
+          if (!plain) {
+            if (full && even && !p.accumulate) {
+#pragma unroll
+              for (int u = 0; u < U; ++u) {
+                float h[V];
+                grad_vector<ENT, T>(w[u], h, p.cs, mc, f.c0, f.c1, nothing);
+                *(uint4*)(to + u * kRowThreads * V) = Vec<T>::pack(h);
+              }
+            } else {
+#pragma unroll
+              for (int u = 0; u < U; ++u) {
+                if (v0 + u * kRowThreads + tid >= b.nv) break;
+                float h[V];
+                grad_vector<ENT, T>(w[u], h, p.cs, mc, f.c0, f.c1, nothing);
+                put_vector<T>(to + u * kRowThreads * V, even, p.accumulate, h);
+              }
+            }
+            if (l - v0 < Str::kBatch) st_f(o + q.label.l, gl + old);
+          }
+          to += Str::kBatch * V;
+        });
+        if (plain) {
+          Group<kRowThreads> g(red);
+          const TopMem none = {};
+          plain_row<kRowThreads, T, true>(g, p, r, none);
+        }
+        if (r + 2 * (size_t)gridDim.x < p.x.rows) bar_arrive(kBarFree + (i & 1));   // there is a row to come in this slot
+      }
+    }
+  } else {
+    TopMem t = {nullptr, nullptr, TopMem::room(p.top), &count};
+    t.list = (Key*)(maxima + (TOP ? 2 * slots * 256 : 0));
+    t.cand = t.list + p.top;
+    struct Row {   // what this warp keeps of a row between its two turns
+      uint32_t cls, own;
+      float single, old;
+      Factors f;
+    };
+    auto prepare = [&](size_t r, uint32_t i) {
+      Row w = {kNoClass, 0, 0.f, 0.f, {}};
+      if (r >= p.x.rows) return w;
+      if (BWD && i >= 2) bar_wait(kBarFree + (i & 1));
+      LogprobSlot<T>& q = slot[i & 1];
+      const T* x = (const T*)p.logits + p.x.offset(r);
+      const Strip<T> b(x, C);
+      Label<T> label;
+      label.fetch(p, r, x, b);
+      w.cls = lane < 2 * V ? b.single(lane) : kNoClass;
+      if (w.cls != kNoClass) {
+        w.single = ld_f(x + w.cls);
+        if (BWD && p.accumulate) w.old = ld_f((const T*)p.dlogits + p.g.offset(r) + w.cls);
+      }
+      if (RANK) w.own = label.own_vector(b, x, C, lane);
+      if (BWD) w.f.fetch(p, r, label.l);
+      if (lane == 0) q.label = label;
+      __syncwarp();
+      bar_arrive(kBarReady + (i & 1));
+      return w;
+    };
+    uint32_t i = 0;
+    Row now = prepare(blockIdx.x, 0);
+    for (size_t r = blockIdx.x; r < p.x.rows; r += gridDim.x, ++i) {
+      const Row next = prepare(r + gridDim.x, i + 1);
+      LogprobSlot<T>& q = slot[i & 1];
+      const T* x = (const T*)p.logits + p.x.offset(r);
+      const Strip<T> b(x, C);
+      const Label<T> label = q.label;
+      bar_wait(kBarSums + (i & 1));
+      Part a;
+      a.clear();
+      if (lane < kRowWarps) a = q.parts[lane];
+      if (now.cls != kNoClass) a.add<ENT>(now.single, p.cs);
+      if (RANK) a.cnt += now.own + (now.cls != kNoClass && label.single_counts(now.single, now.cls));
+      a.join<ENT, 32>(p.cs);
+      const bool strange = a.strange(p.cs);
+      RowSums s;
+      s.set(a.m, a.mc, a.S, p.cs);
+      const float H = s.some ? kLn2 * (s.L - a.E / s.S) : 0.f;
+      if constexpr (BWD) {
+        Factors f = now.f;
+        f.set<ENT>(p, s, H);
+        if (lane == 0) {
+          q.f = f;
+          q.mc = s.mc;
+          q.strange = strange;
+        }
+        bar_arrive(kBarResult + (i & 1));
+        if (!strange && now.cls != kNoClass)
+          st_f((T*)p.dlogits + p.g.offset(r) + now.cls, f.grad<ENT>(now.single, p.cs, s.mc) + (now.cls == label.l ? f.dl : 0.f) + now.old);
+      }
+      if (strange) {
+        Group<32> g(nullptr);
+        if (!BWD) plain_row<32, T, false>(g, p, r, t);
+      } else {
+        if (lane == 0) {
+          put_row(p, s, r, H, label.l, label.xl);
+          if (RANK) p.rank[r] = label.rank(a.cnt, C);
+        }
+        if constexpr (TOP) {
+          uint32_t kv[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) kv[j] = q.sv[j * 32 + lane];
+          const Maxima mx = {maxima + (i & 1) * slots * 256, shift, slots};
+          select_top<T>(t, p.top, kv, mx, b, x, (const uint4*)(x + b.head), now.cls, now.single, work);
+          for (uint32_t j = lane; j < p.top; j += 32) put_top(p, s, r, j, t.list[j]);
+          __syncwarp();
+        }
+      }
+      now = next;
+    }
   }
 }
 
@@ -523,10 +755,7 @@ __global__ void __launch_bounds__(kPositions) logprob_positions(LogprobP p) {
         float f[8], bm;
         x.batch(c, f);
         bm = fmaxf(fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3])), fmaxf(fmaxf(f[4], f[5]), fmaxf(f[6], f[7])));
-        if (bm > a.m) {
-          a.m = bm;
-          a.refer<true>(fmaxf(a.mc, Part::reference(bm, p.cs)));
-        }
+        a.reach<true>(bm, p.cs);
         float S[2] = {0.f, 0.f}, E[2] = {0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -548,7 +777,10 @@ __global__ void __launch_bounds__(kPositions) logprob_positions(LogprobP p) {
       }
       RowSums s;
       if (a.strange(p.cs)) plain_position<true>(x, p.cs, s, a.E);
-      else s.set(a.m, a.mc, a.S, p.cs);
+      else {
+        a.refer<true>(Part::reference(a.m, p.cs));
+        s.set(a.m, a.mc, a.S, p.cs);
+      }
       put_row(p, s, r, s.some ? kLn2 * (s.L - a.E / s.S) : 0.f, l, xl);
       if (p.rank) p.rank[r] = l < C ? a.cnt : kNoClass;
       if (KT) {
@@ -602,10 +834,7 @@ __global__ void __launch_bounds__(kPositions) logprob_positions_bwd(LogprobP p) 
         float f[8], bm;
         x.batch(c, f);
         bm = fmaxf(fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3])), fmaxf(fmaxf(f[4], f[5]), fmaxf(f[6], f[7])));
-        if (bm > a.m) {
-          a.m = bm;
-          a.refer<ENT>(fmaxf(a.mc, Part::reference(bm, p.cs)));
-        }
+        a.reach<ENT>(bm, p.cs);
         float S[2] = {0.f, 0.f}, E[2] = {0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -621,7 +850,10 @@ __global__ void __launch_bounds__(kPositions) logprob_positions_bwd(LogprobP p) 
       RowSums s;
       const bool strange = a.strange(p.cs);
       if (strange) plain_position<ENT>(x, p.cs, s, a.E);
-      else s.set(a.m, a.mc, a.S, p.cs);
+      else {
+        a.refer<ENT>(Part::reference(a.m, p.cs));
+        s.set(a.m, a.mc, a.S, p.cs);
+      }
       const float H = s.some ? kLn2 * (s.L - a.E / s.S) : 0.f;
       put_row(p, s, r, H, l, xl);
       const float dl = p.dlogp && l < C && s.some ? p.dlogp[r] : 0.f, dh = p.dentropy ? p.dentropy[r] : 0.f;
@@ -698,16 +930,31 @@ static int launch_any(const LogprobP& p, cudaStream_t s) {
 
 template <int NT, typename T, bool ENT, bool RANK, bool TOP, bool BWD>
 static int launch_rows(const LogprobP& p, cudaStream_t s) {
+  const size_t bytes = (size_t)p.x.C * sizeof(T), list = p.top + TopMem::room(p.top);
+  // the limits belong to the functions: the most that they take
+  if (NT != 32 && stream_worth(p.x.rows)) {
+    auto kernel = logprob_stream<T, ENT, RANK, TOP, BWD>;
+    typedef Stream<T, BWD> Str;
+    constexpr size_t ring = Str::kAhead * Str::kBytes;
+    const uint32_t shift = slot_shift<T>(p.x.C), slots = (p.x.C / Vec<T>::V + (Str::kBatch << shift) - 1) / (Str::kBatch << shift);
+    const size_t smem = ring + (TOP ? list * sizeof(Key) + 2 * slots * 256 * 2 : 0);
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(ring + 2 * kMostSlots * 256 * 2 + sizeof(Key) * (kMostTop + TopMem::room(kMostTop)))) != cudaSuccess) {
+      cudaGetLastError();
+      return AD_ERR_CUDA;
+    }
+    launch(kernel, stream_grid(p.x.rows), kStreamThreads, smem, s, p);
+    return AD_OK;
+  }
   auto kernel = logprob_rows<NT, T, ENT, RANK, TOP, BWD>;
-  const uint32_t n = NT == 32 ? 1 : row_parts(p.x.rows, (size_t)p.x.C * sizeof(T));
-  const size_t keys = TOP ? (NT == 32 ? (size_t)kRowWarps * (p.top + TopMem::room(p.top)) : p.top + TopMem::room(p.top) + (n > 1 ? n * p.top : 0)) : 0;
-  constexpr int most = (int)(sizeof(Key) * kRowWarps * (kMostTop + TopMem::room(kMostTop)));   // a warp per row
-  // the limit belongs to the function: the most that it takes
-  if (keys * sizeof(Key) > 48 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most) != cudaSuccess) {
+  const uint32_t n = NT == 32 ? 1 : row_parts(p.x.rows, bytes), slots = NT == 32 ? 0 : feed_slots(bytes, n, BWD ? kMostFeed : 0);
+  const size_t keys = TOP ? (NT == 32 ? kRowWarps * list : list + (n > 1 ? n * p.top : 0)) : 0;
+  const size_t smem = slots * Feed<NT>::kBatch * 16 + keys * sizeof(Key);
+  constexpr int most = (int)(NT == 32 ? sizeof(Key) * kRowWarps * (kMostTop + TopMem::room(kMostTop)) : kMostFeed + sizeof(Key) * (9 * kMostTop + TopMem::room(kMostTop)));
+  if (smem > 40 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most) != cudaSuccess) {
     cudaGetLastError();
     return AD_ERR_CUDA;
   }
-  launch_row_kernel(kernel, p, NT == 32 ? (p.x.rows + kRowWarps - 1) / kRowWarps : p.x.rows, n, keys * sizeof(Key), s);
+  launch_row_kernel(kernel, p, slots, NT == 32 ? (p.x.rows + kRowWarps - 1) / kRowWarps : p.x.rows, n, smem, s);
   return AD_OK;
 }
 

@@ -74,6 +74,22 @@ __device__ __forceinline__ float exp2_fast(float v) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));   // 2 ulp; -inf gives 0
   return r;
 }
+__device__ __forceinline__ uint32_t shared_address(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ uint4 load_shared(uint32_t a) {
+  uint4 w;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(a) : "memory");
+  return w;
+}
+__device__ __forceinline__ void copy_async(uint32_t to, const void* from) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory"); }
+__device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void wait_copies() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+// two fp32 numbers at once
+typedef unsigned long long F2;
+__device__ __forceinline__ F2 pair(float a, float b) { F2 r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b)); return r; }
+__device__ __forceinline__ float2 halves(F2 v) { float2 r; asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v)); return r; }
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) { F2 r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
+__device__ __forceinline__ F2 add2(F2 a, F2 b) { F2 r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) { F2 r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
 // v, not below -200 (2^-200 is 0 here), and NaN where v is: what may be multiplied by its exponential
 __device__ __forceinline__ float above_nothing(float v) {
   float r;
@@ -113,12 +129,12 @@ template <> struct Group<kRowThreads> {
   uint32_t tid = threadIdx.x;
   Key* red;   // one per warp
   __device__ explicit Group(void* r) : red((Key*)r) {}
-  __device__ void sync() { __syncthreads(); }
+  __device__ void sync() { __syncwarp(); asm volatile("bar.sync 9, 256;" ::: "memory"); }   // these threads alone: a block may have more
   template <typename V, typename F>
   __device__ V all(V w, F f) {   // of the warps' values, in order
-    __syncthreads();
+    sync();
     if ((tid & 31) == 0) *(V*)&red[tid >> 5] = w;
-    __syncthreads();
+    sync();
     V v = *(V*)&red[0];
 #pragma unroll
     for (int i = 1; i < kRowWarps; ++i) v = f(v, *(V*)&red[i]);
@@ -149,6 +165,13 @@ template <> struct Vec<float> {
   }
   __device__ static Max max(Max a, Max b) { return fmaxf(a, b); }
   __device__ static float value(Max a) { return a; }
+  // not below v, NaN as it is
+  __device__ static uint4 above_or(uint4 w, float v) {
+    uint32_t* p = &w.x;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) asm("max.NaN.f32 %0, %0, %1;" : "+r"(p[i]) : "r"(__float_as_uint(v)));
+    return w;
+  }
   __device__ static uint32_t above(uint4 w, float t) {
     return (__uint_as_float(w.x) > t) + (__uint_as_float(w.y) > t) + (__uint_as_float(w.z) > t) + (__uint_as_float(w.w) > t);
   }
@@ -180,6 +203,16 @@ template <> struct Vec<__nv_bfloat16> {
   }
   __device__ static Max max(uint4 w) { return __hmax2(__hmax2(two(w.x), two(w.y)), __hmax2(two(w.z), two(w.w))); }
   __device__ static Max max(Max a, Max b) { return __hmax2(a, b); }
+  __device__ static uint4 above_or(uint4 w, float v) {
+    const __nv_bfloat162 t = __float2bfloat162_rn(v);
+    uint32_t* p = &w.x;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __nv_bfloat162 m = __hmax2_nan(two(p[i]), t);
+      p[i] = *reinterpret_cast<const uint32_t*>(&m);
+    }
+    return w;
+  }
   __device__ static float value(Max a) { return fmaxf(__low2float(a), __high2float(a)); }
   __device__ static uint32_t above(uint4 w, float t) {
     const __nv_bfloat162 tt = __float2bfloat162_rn(t);
@@ -222,53 +255,110 @@ struct Strip {
   __device__ uint32_t end() const { return last ? head + nv * V + tail : class_of(ve); }
 };
 
-// What a thread, a group or a block of a cluster knows about its share of a row
+// What a thread, a group or a block of a cluster knows about its share of a row.  S and E stand against mc, which follows the
+// maximum when that is kAhead beyond it (a term is then 2^kAhead at most), and is moved to the maximum when shares are joined.
+constexpr float kAhead = 16.f;
 struct Part {
   float m, mc, S, E;
   uint32_t cnt;
   __device__ void clear() { m = -INFINITY; mc = kFloor; S = E = 0.f; cnt = 0; }
   __device__ static float reference(float m, float cs) { return fmaxf(m * cs, kFloor); }
-  template <bool ENT> __device__ void refer(float mcn) {   // S and E against a larger reference
+  template <bool ENT> __device__ void refer(float mcn) {
     const float d = mc - mcn, f = exp2_fast(d);
     if (ENT) E = (E + d * S) * f;
     S *= f;
     mc = mcn;
   }
+  // before elements of which bm is the largest
+  template <bool ENT> __device__ void reach(float bm, float cs) {
+    m = fmaxf(m, bm);
+    if (bm * cs > mc + kAhead) refer<ENT>(bm * cs);
+  }
   template <bool ENT> __device__ void add(float x, float cs) {
-    if (x > m) {
-      m = x;
-      refer<ENT>(reference(m, cs));
-    }
+    reach<ENT>(x, cs);
     const float u = ENT ? above_nothing(fmaf(x, cs, -mc)) : fmaf(x, cs, -mc), e = exp2_fast(u);
     S += e;
     if (ENT) E = fmaf(e, u, E);
   }
-  template <bool ENT> __device__ void join(const Part& o) {   // the same bits whichever of the two is asked
-    m = fmaxf(m, o.m);
-    cnt += o.cnt;
-    const float mcn = fmaxf(mc, o.mc);
-    Part q = o;
-    refer<ENT>(mcn);
-    q.refer<ENT>(mcn);
-    S += q.S;
-    if (ENT) E += q.E;
-  }
-  template <bool ENT> __device__ void join_lanes() {
+  // the sum over lanes that differ in the bits below N, the same in all of them
+  template <bool ENT, int N> __device__ void join(float cs) {
+    float M = m;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      Part q;
-      q.m = __shfl_xor_sync(0xffffffffu, m, o);
-      q.mc = __shfl_xor_sync(0xffffffffu, mc, o);
-      q.S = __shfl_xor_sync(0xffffffffu, S, o);
-      q.E = ENT ? __shfl_xor_sync(0xffffffffu, E, o) : 0.f;
-      q.cnt = 0;
-      join<ENT>(q);
+    for (int o = N / 2; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    m = M;
+    refer<ENT>(reference(M, cs));
+#pragma unroll
+    for (int o = N / 2; o > 0; o >>= 1) {
+      S += __shfl_xor_sync(0xffffffffu, S, o);
+      if (ENT) E += __shfl_xor_sync(0xffffffffu, E, o);
+      cnt += __shfl_xor_sync(0xffffffffu, cnt, o);
     }
-    cnt = __reduce_add_sync(0xffffffffu, cnt);
   }
   // not for the fast pass: beyond the range of its products, or not a number
-  __device__ bool strange(float cs) const { return S != S || fabsf(m * cs) > kFar && m != -INFINITY; }
+  __device__ bool strange(float cs) const { return S != S || (fabsf(m * cs) > kFar && m != -INFINITY); }
 };
+
+// The vectors w[0..U) of a thread, of which bm is the largest element, into its share.  ENT: `nothing`, a number whose product
+// with cs is far below every reference and finite, stands for what is lower: 2^u u is then 0 and not 0 * inf.
+__device__ __forceinline__ float as_nothing(float cs) { return fmaxf(-1e30f / cs, -3e38f); }
+template <bool ENT, int U, typename T>
+__device__ __forceinline__ void add_vectors(Part& a, const uint4 (&w)[U], int n, float bm, float cs, float nothing) {
+  constexpr int V = Vec<T>::V;
+  a.reach<ENT>(bm, cs);
+  const F2 c = pair(cs, cs), m = pair(-a.mc, -a.mc);
+  F2 S[2] = {0, 0}, E[2] = {0, 0};
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    if (u >= n) break;
+    float f[V];
+    Vec<T>::unpack(ENT ? Vec<T>::above_or(w[u], nothing) : w[u], f);
+#pragma unroll
+    for (int i = 0; i < V; i += 2) {
+      const F2 z = fma2(pair(f[i], f[i + 1]), c, m);
+      const float2 q = halves(z);
+      const F2 e = pair(exp2_fast(q.x), exp2_fast(q.y));
+      S[i / 2 & 1] = add2(S[i / 2 & 1], e);
+      if (ENT) E[i / 2 & 1] = fma2(e, z, E[i / 2 & 1]);
+    }
+  }
+  const float2 s = halves(add2(S[0], S[1]));
+  a.S += s.x + s.y;
+  if (ENT) {
+    const float2 e = halves(add2(E[0], E[1]));
+    a.E += e.x + e.y;
+  }
+}
+// The gradient of a vector's elements.  e (c0 + c1 u) with e = 2^u; without ENT c0 e.
+template <bool ENT, typename T>
+__device__ __forceinline__ void grad_vector(uint4 w, float (&h)[Vec<T>::V], float cs, float mc, float c0, float c1, float nothing) {
+  float f[Vec<T>::V];
+  Vec<T>::unpack(ENT ? Vec<T>::above_or(w, nothing) : w, f);
+#pragma unroll
+  for (int i = 0; i < Vec<T>::V; i += 2) {
+    const F2 z = fma2(pair(f[i], f[i + 1]), pair(cs, cs), pair(-mc, -mc));
+    const float2 q = halves(z);
+    const F2 e = pair(exp2_fast(q.x), exp2_fast(q.y));
+    const float2 g = halves(mul2(e, ENT ? fma2(z, pair(c1, c1), pair(c0, c0)) : pair(c0, c0)));
+    h[i] = g.x;
+    h[i + 1] = g.y;
+  }
+}
+// ... and to where it goes: a vector, or single elements where the gradient's rows lie otherwise than the logits'
+template <typename T>
+__device__ __forceinline__ void put_vector(T* o, bool even, int accumulate, float (&h)[Vec<T>::V]) {
+  if (even) {
+    if (accumulate) {
+      float d[Vec<T>::V];
+      Vec<T>::unpack(*(const uint4*)o, d);
+#pragma unroll
+      for (int i = 0; i < Vec<T>::V; ++i) h[i] += d[i];
+    }
+    *(uint4*)o = Vec<T>::pack(h);
+  } else {
+#pragma unroll
+    for (int i = 0; i < Vec<T>::V; ++i) st_f(o + i, accumulate ? h[i] + ld_f(o + i) : h[i]);
+  }
+}
 
 // What the row's results are made of
 struct RowSums {
@@ -283,6 +373,158 @@ struct RowSums {
   __device__ float log_p(float x, float scale) const { return some ? (x - m) * scale - kLn2 * low : -INFINITY; }
   __device__ float lse(float scale) const { return some ? m * scale + kLn2 * low : -INFINITY; }
 };
+
+// A row's vectors [vb, ve), batch after batch: f(v0, w) gets the thread's vectors v0 + u * NT + tid, -inf behind the last.
+// A block feeds them through shared memory, kAheadBatches copies (cp.async) in front of the one that is worked on; a thread
+// reads what it has copied itself, so nothing is waited for together.  Where all of them fit (`slots` batches) they stay, and
+// a second pass reads them there, else again from global memory.  A warp loads them into registers.
+template <int NT>
+struct Feed {
+  static constexpr uint32_t U = NT == 32 ? 8 : 4, kBatch = U * NT;
+  static constexpr int kAheadBatches = 3;
+  const uint4* xv;
+  uint32_t vb, ve, tid, slots;
+  uint4* mem;
+  template <typename T, bool AGAIN, typename F>
+  __device__ __forceinline__ void run(F&& f) {
+    uint4 w[U];
+    if constexpr (NT == 32) {
+      for (uint32_t v0 = vb; v0 < ve; v0 += kBatch) {
+#pragma unroll
+        for (uint32_t u = 0; u < U; ++u) {
+          const uint32_t v = v0 + u * NT + tid;
+          w[u] = v < ve ? xv[v] : Vec<T>::none();
+        }
+        f(v0, w);
+      }
+    } else {
+      const uint32_t n = (ve - vb + kBatch - 1) / kBatch;
+      auto take = [&](uint32_t v0, const uint4* slot) {
+#pragma unroll
+        for (uint32_t u = 0; u < U; ++u) w[u] = v0 + u * NT + tid < ve ? slot[u * NT + tid] : Vec<T>::none();
+      };
+      if (AGAIN && n <= slots) {
+        for (uint32_t i = 0; i < n; ++i) {
+          take(vb + i * kBatch, mem + i * kBatch);
+          f(vb + i * kBatch, w);
+        }
+        return;
+      }
+      uint32_t put = 0, get = 0;
+      auto copy = [&](uint32_t i) {
+        if (i < n) {
+          const uint32_t v0 = vb + i * kBatch + tid;
+#pragma unroll
+          for (uint32_t u = 0; u < U; ++u)
+            if (v0 + u * NT < ve)
+              asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(mem + put * kBatch + u * NT + tid)),
+                           "l"(xv + v0 + u * NT) : "memory");
+          if (++put == slots) put = 0;
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+      };
+#pragma unroll
+      for (int i = 0; i < kAheadBatches; ++i) copy(i);
+      for (uint32_t i = 0; i < n; ++i) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(kAheadBatches - 1) : "memory");
+        take(vb + i * kBatch, mem + get * kBatch);
+        if (++get == slots) get = 0;
+        f(vb + i * kBatch, w);
+        copy(i + kAheadBatches);   // into the slot that has just been read, where there are no more
+      }
+    }
+  }
+};
+// Batches that a block's share of a row has room for: all of them where they fit into `most` bytes, else as many as are ahead
+inline uint32_t feed_slots(size_t row_bytes, uint32_t parts, size_t most) {
+  constexpr size_t batch = Feed<kRowThreads>::kBatch * 16, ahead = Feed<kRowThreads>::kAheadBatches;
+  const size_t n = (row_bytes / 16 / parts + 1 + Feed<kRowThreads>::kBatch - 1) / Feed<kRowThreads>::kBatch;
+  return (uint32_t)(n * batch <= most || n < ahead ? n : ahead);
+}
+constexpr size_t kMostFeed = 96 * 1024;
+
+// ---- many rows: blocks that stay, eight warps that stream and one that does what a row needs besides
+// The streaming warps take one row's vectors after the other's: their copies (cp.async, three batches ahead) go on into the
+// next row, so that loads are in flight while a row is finished.  The ninth warp prepares a row while the one in front of it
+// is streamed (label, lists, masks), and finishes a row while the next one is.
+constexpr uint32_t kStreamThreads = kRowThreads + 32, kStreamBlocks = 3;   // of an SM
+enum { kBarReady = 1, kBarSums = 3, kBarResult = 5, kBarFree = 7 };        // and the row's parity; 9: Group<256>
+__device__ __forceinline__ void bar_arrive(uint32_t id) { __syncwarp(); __threadfence_block(); asm volatile("bar.arrive %0, %1;" ::"r"(id), "n"(kStreamThreads) : "memory"); }
+__device__ __forceinline__ void bar_wait(uint32_t id) { __syncwarp(); asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(kStreamThreads) : "memory"); }
+
+template <typename T, bool TWICE>   // TWICE: every row's vectors are streamed twice in a row
+struct Stream {
+  static constexpr uint32_t U = 4, kBatch = U * kRowThreads, kAhead = 3, kBytes = kBatch * 16, kVec = kRowThreads * 16;
+  const T* x;
+  const Rows* at;
+  size_t r, stride;        // of the row that is copied
+  const uint4 *first, *from;   // this thread's first vector of it, and the one to be copied next
+  uint32_t nv, left;       // vectors of the row, and those that are left
+  uint32_t ring, put, get; // this thread's place in shared memory: kAhead batches
+  bool second;
+  __device__ void row() {
+    if (r < at->rows) {
+      const T* p = x + at->offset(r);
+      const Strip<T> b(p, at->C);
+      first = from = (const uint4*)(p + b.head) + threadIdx.x;
+      nv = left = b.nv;
+    } else {
+      left = 0;
+    }
+  }
+  __device__ __forceinline__ void copy() {
+    if (left >= kBatch) {
+#pragma unroll
+      for (uint32_t u = 0; u < U; ++u) copy_async(put + u * kVec, from + u * kRowThreads);
+      left -= kBatch;
+      from += kBatch;
+    } else {
+#pragma unroll
+      for (uint32_t u = 0; u < U; ++u)
+        if (u * kRowThreads + threadIdx.x < left) copy_async(put + u * kVec, from + u * kRowThreads);
+      left = 0;
+    }
+    put = put == ring + (kAhead - 1) * kBytes ? ring : put + kBytes;
+    commit_copies();
+    if (left == 0) {
+      if (TWICE && !second) {
+        second = true;
+        from = first;
+        left = r < at->rows ? nv : 0;
+      } else {
+        second = false;
+        r += stride;
+        row();
+      }
+    }
+  }
+  __device__ Stream(const T* x_, const Rows& at_, void* mem)
+      : x(x_), at(&at_), r(blockIdx.x), stride(gridDim.x), first(nullptr), from(nullptr), nv(0), left(0), ring(shared_address(mem) + threadIdx.x * 16), put(ring), get(ring), second(false) {
+    row();
+#pragma unroll
+    for (uint32_t i = 0; i < kAhead; ++i) copy();
+  }
+  // f(v0, w, full) for the batches of a row of n vectors: the ones that were copied first.  full: all threads have all of theirs
+  template <typename F> __device__ __forceinline__ void run(uint32_t n, F&& f) {
+    for (uint32_t v0 = 0; v0 < n; v0 += kBatch) {
+      uint4 w[U];
+      wait_copies<kAhead - 1>();
+#pragma unroll
+      for (uint32_t u = 0; u < U; ++u) w[u] = load_shared(get + u * kVec);
+      if (v0 + kBatch <= n) {
+        f(v0, w, true);
+      } else {
+#pragma unroll
+        for (uint32_t u = 0; u < U; ++u)
+          if (v0 + u * kRowThreads + threadIdx.x >= n) w[u] = Vec<T>::none();
+        f(v0, w, false);
+      }
+      get = get == ring + (kAhead - 1) * kBytes ? ring : get + kBytes;
+      copy();   // into the slot that has just been read
+    }
+  }
+};
+inline unsigned stream_grid(size_t rows) { return (unsigned)(rows < kStreamBlocks * kNumSMs ? rows : kStreamBlocks * kNumSMs); }
 
 // Plain loops over a row in any layout: what the fast pass does not serve
 template <typename G, typename T, bool ENT>
@@ -408,6 +650,8 @@ __device__ void plain_position(const P& x, float cs, RowSums& s, float& E) {
   s.low = s.L = s.some ? log2f(S) : 0.f;
 }
 
+// Rows enough for blocks that stay: at least one for each
+inline bool stream_worth(size_t rows) { return rows >= kStreamBlocks * kNumSMs; }
 // Blocks of a row: few rows share the machine, a part at least 8 KB
 inline uint32_t row_parts(size_t rows, size_t row_bytes) {
   uint32_t n = 1;
@@ -416,7 +660,7 @@ inline uint32_t row_parts(size_t rows, size_t row_bytes) {
 }
 // `units` blocks, or clusters of n blocks; a kernel's blocks go on to further rows where there are more
 template <typename P>
-void launch_row_kernel(void (*kernel)(P), const P& p, size_t units, uint32_t n, size_t smem, cudaStream_t s) {
+void launch_row_kernel(void (*kernel)(P, uint32_t), const P& p, uint32_t slots, size_t units, uint32_t n, size_t smem, cudaStream_t s) {
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute at[2];
   cfg.gridDim = (unsigned)((units < (1u << 20) ? units : (1u << 20)) * n);
@@ -430,7 +674,7 @@ void launch_row_kernel(void (*kernel)(P), const P& p, size_t units, uint32_t n, 
     cfg.numAttrs = 1;
   }
   launch_attr(cfg, at);
-  cudaLaunchKernelEx(&cfg, kernel, p);   // an error is what launch_status() returns
+  cudaLaunchKernelEx(&cfg, kernel, p, slots);   // an error is what launch_status() returns
 }
 
 }  // namespace adk
