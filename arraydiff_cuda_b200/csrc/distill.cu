@@ -253,6 +253,19 @@ __global__ void __launch_bounds__(256) distill_any(DistillP p) {
   }
 }
 
+// The elements of a vector whose bits are set become -inf
+template <typename T>
+__device__ __forceinline__ void leave_out(uint4& w, uint32_t bits) {
+  constexpr int V = Vec<T>::V;
+  uint32_t* q = &w.x;
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+    if (bits >> i & 1) {
+      if (V == 4) q[i] = 0xff800000u;
+      else q[i / 2] = i & 1 ? (q[i / 2] & 0xffffu) | 0xff800000u : (q[i / 2] & 0xffff0000u) | 0xff80u;
+    }
+}
+
 // ---------------------------------------------------------------- rows of many neighbouring classes
 // NT 32: a warp per row, eight vectors per lane and batch.  NT 256: a block per row, or a cluster of blocks, four vectors.
 // REST: the classes of the list are left out of the pass.
@@ -298,7 +311,8 @@ __global__ void __launch_bounds__(256) distill_rows(DistillP p, uint32_t slots) 
     Part a;
     a.clear();
     if (sc != kNoClass && apart) a.add<false>(ld_f(x + sc), p.cs);
-    Feed<NT> feed = {xv, b.vb, b.ve, g.tid, slots, (uint4*)dyn};
+    Feed<NT> feed(xv, b.vb, b.ve, g.tid, slots, (uint4*)dyn);
+    feed.template start<T>();
     feed.template run<T, false>([&](uint32_t v0, uint4 (&w)[U]) {
       typename X::Max most;
       if (REST) {
@@ -311,30 +325,12 @@ __global__ void __launch_bounds__(256) distill_rows(DistillP p, uint32_t slots) 
         }
         if (any) {
 #pragma unroll
-          for (int u = 0; u < U; ++u) {
-            uint32_t* q = &w[u].x;
-#pragma unroll
-            for (int i = 0; i < V; ++i)
-              if (out[u] >> i & 1) {
-                if (V == 4) q[i] = 0xff800000u;
-                else q[i / 2] = i & 1 ? (q[i / 2] & 0xffffu) | 0xff800000u : (q[i / 2] & 0xffff0000u) | 0xff80u;
-              }
-          }
+          for (int u = 0; u < U; ++u) leave_out<T>(w[u], out[u]);
         }
       }
 #pragma unroll
       for (int u = 0; u < U; ++u) most = u ? X::max(most, X::max(w[u])) : X::max(w[u]);
-      a.reach<false>(X::value(most), p.cs);
-      float S[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (v0 + u * NT >= b.ve) break;
-        float f[V];
-        X::unpack(w[u], f);
-#pragma unroll
-        for (int i = 0; i < V; ++i) S[i & 3] += exp2_fast(fmaf(f[i], p.cs, -a.mc));
-      }
-      a.S += (S[0] + S[1]) + (S[2] + S[3]);
+      add_vectors<false, U, T>(a, w, (int)((b.ve - v0 + NT - 1) / NT), X::value(most), p.cs, 0.f);
     });
     a.join<false, 32>(p.cs);
     if (NT != 32) {
@@ -380,29 +376,14 @@ __global__ void __launch_bounds__(256) distill_rows(DistillP p, uint32_t slots) 
       }
       if (p.accumulate) g.sync();
       if (sc != kNoClass) st_f(o + sc, grad(ld_f(x + sc)) + (p.accumulate ? ld_f(o + sc) : 0.f));
-      uint4* ov = (uint4*)(o + b.head);
       feed.template run<T, true>([&](uint32_t v0, const uint4 (&w)[U]) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           const uint32_t v = v0 + u * NT + g.tid;
           if (v >= b.ve) break;
           float h[V];
-          X::unpack(w[u], h);
-#pragma unroll
-          for (int i = 0; i < V; ++i) h[i] = grad(h[i]);
-          if (even) {
-            if (p.accumulate) {
-              float q[V];
-              X::unpack(ov[v], q);
-#pragma unroll
-              for (int i = 0; i < V; ++i) h[i] += q[i];
-            }
-            ov[v] = X::pack(h);
-          } else {
-            T* os = o + b.class_of(v);
-#pragma unroll
-            for (int i = 0; i < V; ++i) st_f(os + i, p.accumulate ? h[i] + ld_f(os + i) : h[i]);
-          }
+          grad_vector<false, T>(w[u], h, p.cs, mc, coef, 0.f, 0.f);
+          put_vector<T>(o + b.class_of(v), even, p.accumulate, h);
         }
       });
       g.sync();
@@ -414,6 +395,271 @@ __global__ void __launch_bounds__(256) distill_rows(DistillP p, uint32_t slots) 
     }
     if (parts_n > 1) cluster.sync();   // what the others read of this block's
     else g.sync();
+  }
+}
+
+// Many rows of many classes: see Stream.  Two rows are in hand, by parity.
+struct __align__(16) DistillSlot {
+  List list;
+  float old[kMostTop], grad[kMostTop];   // what the gradient of an entry's class is added to, and that gradient
+  Part parts[kRowWarps];
+  float mc, coef;
+  uint32_t singles;                      // which of the row's single elements are listed
+  bool strange;
+};
+template <typename T, bool REST, bool BWD>
+__global__ void __launch_bounds__(kStreamThreads, kStreamBlocks) distill_stream(DistillP p, uint32_t mask_bytes) {
+  typedef Stream<T, BWD> Str;
+  constexpr int U = Str::U, V = Vec<T>::V;
+  typedef Vec<T> X;
+  extern __shared__ __align__(16) uint8_t dyn[];   // batches of vectors, then two masks: a byte per vector
+  __shared__ DistillSlot slot[2];
+  __shared__ Key red[kRowWarps];
+  __shared__ Distilled shared;
+  grid_dependency();
+  const uint32_t C = p.x.C, k = p.top, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  uint8_t* masks = dyn + Str::kAhead * Str::kBytes;
+  if (warp < kRowWarps) {
+    Str stream((const T*)p.logits, p.x, dyn);
+    uint32_t i = 0;
+    for (size_t r = blockIdx.x; r < p.x.rows; r += gridDim.x, ++i) {
+      DistillSlot& q = slot[i & 1];
+      const T* x = (const T*)p.logits + p.x.offset(r);
+      const Strip<T> b(x, C);
+      const uint8_t* mask = masks + (i & 1) * mask_bytes + tid;
+      bar_wait(kBarReady + (i & 1));
+      Part a;
+      a.clear();
+      stream.run(b.nv, [&](uint32_t v0, uint4 (&w)[U], bool full) {
+        if (REST) {
+          uint32_t out[U], any = 0;
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            out[u] = full || v0 + u * kRowThreads + tid < b.nv ? mask[v0 + u * kRowThreads] : 0;
+            any |= out[u];
+          }
+          if (any) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) leave_out<T>(w[u], out[u]);
+          }
+        }
+        typename X::Max most = X::max(w[0]);
+#pragma unroll
+        for (int u = 1; u < U; ++u) most = X::max(most, X::max(w[u]));
+        add_vectors<false, U, T>(a, w, full ? U : (int)((b.nv - v0 + kRowThreads - 1) / kRowThreads), X::value(most), p.cs, 0.f);
+      });
+      a.join<false, 32>(p.cs);
+      if (lane == 0) q.parts[warp] = a;
+      bar_arrive(kBarSums + (i & 1));
+      if constexpr (BWD) {
+        bar_wait(kBarResult + (i & 1));
+        T* o = (T*)p.dlogits + p.g.offset(r);
+        const bool even = (((uintptr_t)o ^ (uintptr_t)x) & 15u) == 0, plain = q.strange;
+        const float mc = q.mc, coef = q.coef;
+        T* to = o + b.head + tid * V;   // this thread's vector of the batch
+        stream.run(b.nv, [&](uint32_t v0, uint4 (&w)[U], bool full) {
+          if (!plain) {
+            if (full && even && !p.accumulate) {
+#pragma unroll
+              for (int u = 0; u < U; ++u) {
+                float h[V];
+                grad_vector<false, T>(w[u], h, p.cs, mc, coef, 0.f, 0.f);
+                *(uint4*)(to + u * kRowThreads * V) = X::pack(h);
+              }
+            } else {
+#pragma unroll
+              for (int u = 0; u < U; ++u) {
+                if (v0 + u * kRowThreads + tid >= b.nv) break;
+                float h[V];
+                grad_vector<false, T>(w[u], h, p.cs, mc, coef, 0.f, 0.f);
+                put_vector<T>(to + u * kRowThreads * V, even, p.accumulate, h);
+              }
+            }
+          }
+          to += Str::kBatch * V;
+        });
+        Group<kRowThreads> g(red);
+        if (plain) {
+          plain_row<kRowThreads, T, true>(g, p, r, q.list, &shared);
+        } else {
+          g.sync();   // the list's classes over what the loop wrote
+          if (tid < k && q.list.cls[tid] < C) st_f(o + q.list.cls[tid], q.grad[tid]);
+        }
+        if (r + 2 * (size_t)gridDim.x < p.x.rows) bar_arrive(kBarFree + (i & 1));   // there is a row to come in this slot
+      }
+    }
+  } else {
+    struct Row {   // what this warp keeps of a row between its two turns
+      uint32_t cls;
+      float single, old, Q, mk, K, dloss;
+      bool apart;
+    };
+    auto prepare = [&](size_t r, uint32_t i) {
+      Row w = {kNoClass, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, true};
+      if (r >= p.x.rows) return w;
+      if (BWD && i >= 2) bar_wait(kBarFree + (i & 1));
+      DistillSlot& q = slot[i & 1];
+      uint8_t* mask = masks + (i & 1) * mask_bytes;
+      const T* x = (const T*)p.logits + p.x.offset(r);
+      const T* o = (const T*)p.dlogits + (BWD ? p.g.offset(r) : 0);
+      const Strip<T> b(x, C);
+      uint32_t cls[4];
+      float a[4], xs[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t j = lane + 32 * e;
+        cls[e] = j < k ? p.top_class[r * k + j] : kNoClass;
+        a[e] = j < k ? p.top_logit[r * k + j] * p.ts : 0.f;
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t j = lane + 32 * e;
+        const bool in = cls[e] < C;
+        xs[e] = in ? ld_f(x + cls[e]) : 0.f;
+        if (!in) a[e] = -INFINITY;
+        if (BWD && p.accumulate) q.old[j] = in ? ld_f(o + cls[e]) : 0.f;
+        q.list.cls[j] = cls[e];
+        q.list.x[j] = xs[e];
+      }
+      w.cls = lane < 2 * V ? b.single(lane) : kNoClass;
+      if (w.cls != kNoClass) {
+        w.single = ld_f(x + w.cls);
+        if (BWD && p.accumulate) w.old = ld_f(o + w.cls);
+      }
+      if (BWD) w.dloss = p.dloss[r];
+      float shift = 0.f;
+      if (p.rest) {
+        if (p.top_lse) shift = (float)(p.top_lse[r] * kLog2e);
+      } else {
+        float am = warp_max(fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3])));
+        if (am == -INFINITY) am = 0.f;
+        const float z = warp_sum((exp2f(a[0] - am) + exp2f(a[1] - am)) + (exp2f(a[2] - am) + exp2f(a[3] - am)));
+        shift = z != 0.f ? am + log2f(z) : 0.f;
+      }
+      // which classes are listed, and whether one of them stands twice
+      bool twice = false;
+      if (REST) {
+        for (uint32_t v = lane; v < (b.nv + 15) / 16; v += 32) ((uint4*)mask)[v] = make_uint4(0, 0, 0, 0);
+        if (lane == 0) q.singles = 0;
+        __syncwarp();
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t c = cls[e];
+          if (c >= C) continue;
+          if (c >= b.head && c < b.head + b.nv * V) {
+            const uint32_t v = (c - b.head) / V, bit = 1u << (v % 4 * 8 + (c - b.head) % V);
+            twice |= (atomicOr((uint32_t*)mask + v / 4, bit) & bit) != 0;
+          } else {
+            const uint32_t bit = 1u << (c < b.head ? c : V + (c - b.head - b.nv * V));
+            twice |= (atomicOr(&q.singles, bit) & bit) != 0;
+          }
+        }
+        twice = __any_sync(0xffffffffu, twice);
+        __syncwarp();
+        w.apart = !(q.singles >> lane & 1u);
+      }
+      if (BWD && !REST) twice = true;   // looked for below
+      bool first[4] = {true, true, true, true};
+      if (twice) {
+        __syncwarp();
+        uint32_t more = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (32 * e >= (int)k) break;
+          uint32_t before = 0, all = 0;
+          for (uint32_t f = 0; f < k; f += 4) {
+            const uint4 c = *(const uint4*)&q.list.cls[f];
+            const uint32_t j = lane + 32 * e;
+            all += (c.x == cls[e]) + (c.y == cls[e]) + (c.z == cls[e]) + (c.w == cls[e]);
+            before += (c.x == cls[e] && f < j) + (c.y == cls[e] && f + 1 < j) + (c.z == cls[e] && f + 2 < j) + (c.w == cls[e] && f + 3 < j);
+          }
+          first[e] = before == 0;
+          more += cls[e] < C && all > 1;
+        }
+        twice = __any_sync(0xffffffffu, more != 0);
+      }
+      if (REST) {
+        float mk = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) mk = cls[e] < C ? fmaxf(mk, xs[e]) : mk;
+        mk = warp_max(mk);
+        w.mk = mk == -INFINITY ? 0.f : mk;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (cls[e] < C && first[e]) w.K += exp2_fast((xs[e] - w.mk) * p.cs);
+        w.K = warp_sum(w.K);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        a[e] -= shift;
+        q.list.a[lane + 32 * e] = a[e];
+        w.Q += exp2f(a[e]);
+      }
+      w.Q = warp_sum(w.Q);
+      if (lane == 0) q.list.twice = twice;
+      bar_arrive(kBarReady + (i & 1));
+      return w;
+    };
+    uint32_t i = 0;
+    Row now = prepare(blockIdx.x, 0);
+    for (size_t r = blockIdx.x; r < p.x.rows; r += gridDim.x, ++i) {
+      const Row next = prepare(r + gridDim.x, i + 1);
+      DistillSlot& q = slot[i & 1];
+      bar_wait(kBarSums + (i & 1));
+      Part a;
+      a.clear();
+      if (lane < kRowWarps) a = q.parts[lane];
+      if (now.cls != kNoClass && now.apart) a.add<false>(now.single, p.cs);
+      a.join<false, 32>(p.cs);
+      const bool strange = a.strange(p.cs);
+      const float off = a.m == -INFINITY ? 0.f : fmaf(-a.m, p.cs, a.mc);
+      float loss;
+      const Distilled d = row_sums(p, a.m, off, a.S, now.mk, now.K, now.Q, loss);
+      const float f = now.dloss * p.scale;
+      if (!strange) {
+        float terms = 0.f, w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t j = lane + 32 * e;
+          const float v = q.list.a[j];
+          w[e] = exp2f(v);
+          terms += d.term(w[e], v, q.list.x[j], p.scale);
+        }
+        if (BWD) {
+          __syncwarp();
+#pragma unroll
+          for (int e = 0; e < 4; ++e) q.list.a[lane + 32 * e] = w[e];
+          __syncwarp();
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t j = lane + 32 * e;
+            if (j < k) q.grad[j] = listed_grad(p, d, q.list, j, f) + (p.accumulate ? q.old[j] : 0.f);
+          }
+          if (lane == 0) {
+            q.mc = a.mc;
+            q.coef = f * d.out;
+            q.strange = false;
+          }
+          // before the list's, which the streaming threads write behind this barrier
+          if (now.cls != kNoClass) st_f((T*)p.dlogits + p.g.offset(r) + now.cls, f * d.out * exp2_fast(fmaf(now.single, p.cs, -a.mc)) + now.old);
+          bar_arrive(kBarResult + (i & 1));
+        }
+        loss += warp_sum(terms);
+        if (lane == 0 && p.loss) p.loss[r] = d.some ? loss + 0.f * d.L : 0.f;
+      } else {
+        // the plain loops want the list as it is fetched
+        Group<32> g(nullptr);
+        __syncwarp();
+        fetch_list<32, T>(g, p, r, (const T*)p.logits + p.x.offset(r), 1, q.list);
+        if (BWD) {
+          if (lane == 0) q.strange = true;
+          bar_arrive(kBarResult + (i & 1));
+        } else {
+          plain_row<32, T, false>(g, p, r, q.list, &shared);
+        }
+      }
+      now = next;
+    }
   }
 }
 
@@ -578,6 +824,19 @@ static int distill_args(const ad_distill_args* a, bool bwd, DistillP& p) {
 
 template <int NT, typename T, bool REST, bool BWD>
 static int launch_rows(const DistillP& p, uint32_t n, size_t mask, cudaStream_t s) {
+  if (NT != 32 && stream_worth(p.x.rows)) {
+    typedef Stream<T, BWD> Str;
+    const size_t bytes = REST ? (p.x.C / Vec<T>::V + 15) / 16 * 16 : 0, smem = Str::kAhead * Str::kBytes + 2 * bytes;
+    if (bytes <= kMostMask / 2) {
+      auto kernel = distill_stream<T, REST, BWD>;
+      if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(Str::kAhead * Str::kBytes + kMostMask)) != cudaSuccess) {
+        cudaGetLastError();
+        return AD_ERR_CUDA;
+      }
+      launch(kernel, stream_grid(p.x.rows, smem), kStreamThreads, smem, s, p, (uint32_t)bytes);
+      return AD_OK;
+    }
+  }
   auto kernel = distill_rows<NT, T, REST, BWD>;
   const uint32_t slots = NT == 32 ? 0 : feed_slots((size_t)p.x.C * sizeof(T), n, BWD ? kMostFeed : 0);
   const size_t smem = slots * Feed<NT>::kBatch * 16 + mask;

@@ -30,28 +30,38 @@ struct LogprobP {
 
 // ---------------------------------------------------------------- top classes
 struct TopMem {
-  Key *list, *cand;   // the result, in order; what is at or in front of the bound
-  uint32_t cap, *n;   // room in cand, and how many there are (more than cap: not all are there)
+  Key *list, *cand;   // the result, in order; what reaches the bound
+  uint32_t cap;       // room in cand
   __host__ __device__ static constexpr uint32_t room(uint32_t k) { return 64 + 9 * k; }   // k vectors of equal elements and the single ones fit
-  __device__ void push(float v, uint32_t c) const {
-    const uint32_t at = atomicAdd(n, 1u);
-    if (at < cap) cand[at] = key_of(v, c);
-  }
 };
+// One warp: places for `mine` things of each lane behind `n` that are there already, which is increased by all of them
+__device__ __forceinline__ uint32_t places(uint32_t mine, uint32_t& n) {
+  const uint32_t lane = threadIdx.x & 31;
+  uint32_t upto = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t q = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= (uint32_t)o) upto += q;
+  }
+  const uint32_t at = n + upto - mine;
+  n += __shfl_sync(0xffffffffu, upto, 31);
+  return at;
+}
 
 // One warp: of 256 shares' maxima, eight per lane (keys, 0 for none), the k-th, or less; 0: fewer than k
 template <int SHIFT>
-__device__ uint32_t kth_share(const uint32_t (&kv)[8], uint32_t k, uint32_t* mem) {
+__device__ uint32_t kth_share(const uint32_t (&kv)[8], uint32_t k) {
   if (k <= 16) {   // the k-th of the lanes' largest: little less
-    uint32_t best = kv[0], at = 0;
+    uint32_t best = kv[0], t = 0;
 #pragma unroll
     for (int i = 1; i < 8; ++i) best = max(best, kv[i]);
-    mem[threadIdx.x & 31] = best;
-    __syncwarp();
-#pragma unroll
-    for (int i = 0; i < 32; ++i) at += mem[i] > best;
-    __syncwarp();
-    return __reduce_min_sync(0xffffffffu, at < k ? best : 0xffffffffu);
+    for (uint32_t n = 0; n < k;) {
+      t = __reduce_max_sync(0xffffffffu, best);
+      if (t == 0) break;
+      n += __popc(__ballot_sync(0xffffffffu, best == t));
+      if (best == t) best = 0;
+    }
+    return t;
   }
   uint32_t t = 0;
   for (uint32_t bit = 1u << (31 - SHIFT); bit; bit >>= 1) {
@@ -63,27 +73,56 @@ __device__ uint32_t kth_share(const uint32_t (&kv)[8], uint32_t k, uint32_t* mem
   return t == 0 ? 0u : SHIFT ? t << SHIFT | (t >> (31 - SHIFT) ? 0u : (1u << SHIFT) - 1) : t;   // the bits that a key's sign tells
 }
 
-// The list out of the candidates: each one's place is the number of those in front of it
-template <int NT>
-__device__ void sort_candidates(Group<NT>& g, const TopMem& t, uint32_t n, uint32_t k) {
-  Key least = 0;
-  if (n > 64 + 2 * k) {   // many equal or clustered ones: the k-th first, bit by bit
-    for (Key bit = 1ull << 63; bit; bit >>= 1) {
-      uint32_t m = 0;
-      for (uint32_t i = g.tid; i < n; i += NT) m += t.cand[i] >= (least | bit);
-      if (g.sum(m) >= k) least |= bit;
+// One warp: the list out of n candidates, each one's place being the number of those in front of it.  Q of them per lane and pass.
+template <int Q>
+__device__ __forceinline__ void sort_candidates(const TopMem& t, uint32_t n, uint32_t k, Key least) {
+  const uint32_t lane = threadIdx.x & 31;
+  for (uint32_t i0 = 0; i0 < n; i0 += 32 * Q) {
+    Key key[Q];
+    uint32_t at[Q];
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+      key[q] = i0 + q * 32 + lane < n ? t.cand[i0 + q * 32 + lane] : 0;
+      at[q] = 0;
     }
-  }
-  for (uint32_t i = g.tid; i < n; i += NT) {
-    const Key key = t.cand[i];
-    if (key < least) continue;
-    uint32_t at = 0;
 #pragma unroll 4
-    for (uint32_t j = 0; j < n; ++j) at += t.cand[j] > key;
-    if (at < k) t.list[at] = key;
+    for (uint32_t j = 0; j < n; ++j) {
+      const Key other = t.cand[j];
+#pragma unroll
+      for (int q = 0; q < Q; ++q) at[q] += other > key[q];
+    }
+#pragma unroll
+    for (int q = 0; q < Q; ++q)
+      if (key[q] >= least && key[q] && at[q] < k) t.list[at[q]] = key[q];
   }
-  for (uint32_t i = n + g.tid; i < k; i += NT) t.list[i] = 0;
-  g.sync();
+}
+__device__ void sort_candidates(const TopMem& t, uint32_t n, uint32_t k) {
+  const uint32_t lane = threadIdx.x & 31;
+  __syncwarp();
+  Key least = 0;
+  if (n <= 32) {
+    sort_candidates<1>(t, n, k, 0);
+  } else {
+    if (n > 64 + 2 * k) {   // many equal or clustered ones: the k-th first, bit by bit, and only those up to it
+      for (Key bit = 1ull << 63; bit; bit >>= 1) {
+        uint32_t m = 0;
+        for (uint32_t i = lane; i < n; i += 32) m += t.cand[i] >= (least | bit);
+        if (__reduce_add_sync(0xffffffffu, m) >= k) least |= bit;
+      }
+      uint32_t kept = 0;
+      for (uint32_t i0 = 0; i0 < n; i0 += 32) {
+        const Key key = i0 + lane < n ? t.cand[i0 + lane] : 0;
+        __syncwarp();
+        const uint32_t at = places(key >= least && key, kept);
+        if (key >= least && key) t.cand[at] = key;   // not behind where it was
+        __syncwarp();
+      }
+      n = kept;
+    }
+    sort_candidates<4>(t, n, k, least);
+  }
+  for (uint32_t i = n + lane; i < k; i += 32) t.list[i] = 0;
+  __syncwarp();
 }
 
 // One class after the other, from classes [lo, hi): for rows that the bound does not serve
@@ -104,30 +143,22 @@ __device__ void rounds(Group<NT>& g, const TopMem& t, const T* x, int64_t st, ui
   g.sync();
 }
 
-// One warp: pushes the elements of a strip that equal v, in order of their classes, until there are r of them
+// One warp: adds the first r elements of a strip that equal v, in order of their classes, to the n candidates
 template <typename T>
-__device__ void push_equal(const TopMem& t, const Strip<T>& b, const T* x, float v, uint32_t r) {
+__device__ void add_equal(const TopMem& t, const Strip<T>& b, const T* x, float v, uint32_t r, uint32_t& n) {
   constexpr uint32_t V = Vec<T>::V;
-  const uint32_t lane = threadIdx.x & 31;
-  uint32_t have = 0;
-  for (uint32_t c0 = b.begin(); c0 < b.end() && have < r; c0 += 32 * V) {
-    uint32_t n = 0, hits = 0;
+  const uint32_t lane = threadIdx.x & 31, most = n + r;
+  for (uint32_t c0 = b.begin(); c0 < b.end() && n < most; c0 += 32 * V) {
+    uint32_t hits = 0;
     for (uint32_t i = 0; i < V; ++i) {
       const uint32_t c = c0 + lane * V + i;
-      if (c < b.end() && ld_f(x + c) == v) { hits |= 1u << i; ++n; }
+      if (c < b.end() && ld_f(x + c) == v) hits |= 1u << i;
     }
-    uint32_t before = n;   // of the lanes up to this one
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const uint32_t q = __shfl_up_sync(0xffffffffu, before, o);
-      if (lane >= (uint32_t)o) before += q;
-    }
-    uint32_t at = have + before - n;
+    uint32_t at = places(__popc(hits), n);
     for (uint32_t i = 0; i < V; ++i)
-      if (hits >> i & 1 && at++ < r) t.push(v, c0 + lane * V + i);
-    have += __shfl_sync(0xffffffffu, before, 31);
+      if (hits >> i & 1 && at++ < most) t.cand[at - 1] = key_of(v, c0 + lane * V + i);
   }
-  __syncwarp();
+  if (n > most) n = most;
 }
 
 // The maxima of what a thread has taken at a time: batches of four vectors, `1 << shift` of them together, as the upper
@@ -138,6 +169,8 @@ struct Maxima {
 };
 constexpr uint32_t kMostSlots = 16;
 __device__ __forceinline__ uint32_t half_key(uint32_t h) { return h & 0x8000u ? 0xffffu ^ h : h | 0x8000u; }   // value_key >> 16
+
+template <int N> struct Loads { static constexpr int value = N; };
 
 // One warp: a strip's list out of its 256 shares, of which lane i has number 32 j + i in kv[j]: the key of its largest value, 0
 // for none.  Share s is the vectors vb + s + 256 n, xv[0] being vector vb.  `single`: a single element of the strip in this
@@ -150,14 +183,13 @@ __device__ void select_top(const TopMem& t, uint32_t k, const uint32_t (&kv)[8],
   constexpr uint32_t kWork = 2048;
   Group<32> g(nullptr);
   const uint32_t lane = g.tid, below = (1u << lane) - 1;
-  const uint32_t tv = kth_share<X::kKeyShift>(kv, k, (uint32_t*)t.cand);
+  const uint32_t tv = kth_share<X::kKeyShift>(kv, k);
   const float bound = tv ? key_value(tv) : -INFINITY;
   const uint32_t nv = b.ve - b.vb, per = mx.m ? mx.slots : (nv + 255) / 256;
   // all elements of the shares that reach the bound; where that is too many, those above it, and of the equal ones the first
   for (int strict = 0; strict < 2; ++strict) {
     auto reaches = [&](float v) { return strict ? v > bound : v >= bound; };
-    if (lane == 0) *t.n = 0;
-    uint32_t ns = 0;
+    uint32_t ns = 0, n = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const bool in = kv[i] && (strict ? kv[i] > tv : kv[i] >= tv);
@@ -169,62 +201,82 @@ __device__ void select_top(const TopMem& t, uint32_t k, const uint32_t (&kv)[8],
     uint32_t vectors = ns * per;   // of the shares, or (maxima) of their slots that reach it
     uint16_t* list = work + 256;
     if (mx.m) {
-      uint32_t n = 0;
-      for (uint32_t i0 = 0; i0 < ns * per; i0 += 32) {
+      uint32_t found = 0;
+      for (uint32_t i0 = 0; i0 < vectors; i0 += 32) {
         const uint32_t i = i0 + lane, s = i / per, slot = i - s * per;
         bool in = false;
         uint16_t at = 0;
-        if (i < ns * per) {
+        if (i < vectors) {
           at = (uint16_t)(slot * 256 + work[s]);
           in = half_key(mx.m[at]) >= tv >> 16;
         }
         const uint32_t who = __ballot_sync(0xffffffffu, in);
-        if (in && n + __popc(who & below) < kWork - 256) list[n + __popc(who & below)] = at;
-        n += __popc(who);
+        if (in && found + __popc(who & below) < kWork - 256) list[found + __popc(who & below)] = at;
+        found += __popc(who);
       }
-      if (n > kWork - 256 && !strict) continue;
-      if (n > kWork - 256) n = 0, *t.n = t.cap + 1;
-      vectors = n * (4u << mx.shift);
+      if (found > kWork - 256) continue;
+      vectors = found * (4u << mx.shift);
       __syncwarp();
     }
-    for (uint32_t i0 = 0; i0 < vectors; i0 += 128) {   // four loads at a time
-      uint4 w[4];
-      uint32_t at[4];
+    auto vector_of = [&](uint32_t i) -> uint32_t {
+      if (i >= vectors) return nv;
+      if (mx.m) {
+        const uint32_t e = list[i >> (2 + mx.shift)], sub = i & ((4u << mx.shift) - 1);
+        return (((e >> 8) << (2 + mx.shift)) + sub) * 256 + (e & 255);
+      }
+      const uint32_t s = i / per;
+      return (i - s * per) * 256 + work[s];
+    };
+    auto look = [&](auto loads, uint32_t i0) {   // so many loads at a time
+      constexpr int Q = decltype(loads)::value;
+      uint4 w[Q];
+      uint32_t at[Q], hits[Q], mine = 0;
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const uint32_t i = i0 + q * 32 + lane;
-        uint32_t v = nv;
-        if (i < vectors) {
-          if (mx.m) {
-            const uint32_t e = list[i >> (2 + mx.shift)], sub = i & ((4u << mx.shift) - 1);
-            v = (((e >> 8) << (2 + mx.shift)) + sub) * 256 + (e & 255);
-          } else {
-            const uint32_t s = i / per;
-            v = (i - s * per) * 256 + work[s];
-          }
-        }
-        at[q] = v;
-        w[q] = v < nv ? xv[v] : X::none();
+      for (int q = 0; q < Q; ++q) {
+        at[q] = vector_of(i0 + q * 32 + lane);
+        w[q] = at[q] < nv ? xv[at[q]] : X::none();
       }
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
+      for (int q = 0; q < Q; ++q) {
+        hits[q] = 0;
         if (at[q] < nv && reaches(X::value(X::max(w[q])))) {
           float f[V];
           X::unpack(w[q], f);
 #pragma unroll
-          for (int j = 0; j < V; ++j)
-            if (reaches(f[j])) t.push(f[j], b.class_of(b.vb + at[q]) + j);
+          for (int j = 0; j < V; ++j) hits[q] |= reaches(f[j]) ? 1u << j : 0u;
         }
-      if (__any_sync(0xffffffffu, *(volatile uint32_t*)t.n > t.cap)) break;
+        mine += __popc(hits[q]);
+      }
+      uint32_t to = places(mine, n);
+#pragma unroll
+      for (int q = 0; q < Q; ++q)
+        if (hits[q]) {
+          float f[V];
+          X::unpack(w[q], f);
+          const uint32_t c0 = b.class_of(b.vb + at[q]);
+#pragma unroll
+          for (int j = 0; j < V; ++j)
+            if (hits[q] >> j & 1) {
+              if (to < t.cap) t.cand[to] = key_of(f[j], c0 + j);
+              ++to;
+            }
+        }
+    };
+    for (uint32_t i0 = 0; i0 < vectors && n <= t.cap;) {
+      if (vectors - i0 <= 32) {
+        look(Loads<1>(), i0);
+        i0 += 32;
+      } else {
+        look(Loads<4>(), i0);
+        i0 += 128;
+      }
     }
-    if (sc != kNoClass && reaches(single)) t.push(single, sc);
-    __syncwarp();
-    const uint32_t n = *t.n;
-    if (n <= t.cap && strict) {
-      if (n < k) push_equal<T>(t, b, x, bound, k - n);
-    }
+    const bool in = sc != kNoClass && reaches(single);
+    const uint32_t to = places(in, n);
+    if (in && to < t.cap) t.cand[to] = key_of(single, sc);
     if (n <= t.cap) {
-      sort_candidates<32>(g, t, *t.n, k);
+      if (strict && n < k) add_equal<T>(t, b, x, bound, k - n, n);
+      sort_candidates(t, n, k);
       return;
     }
     __syncwarp();
@@ -288,7 +340,7 @@ __global__ void __launch_bounds__(256) logprob_any(LogprobP p) {
   grid_dependency();
   __shared__ Key list[8][kMostTop];
   Group<32> g(nullptr);
-  TopMem t = {list[threadIdx.x >> 5], nullptr, 0, nullptr};
+  TopMem t = {list[threadIdx.x >> 5], nullptr, 0};
   const size_t warp = ((size_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5, nw = ((size_t)gridDim.x * blockDim.x) >> 5;
   for (size_t r = warp; r < p.x.rows; r += nw) plain_row<32, T, BWD>(g, p, r, t);
 }
@@ -338,8 +390,9 @@ struct Label {
   uint32_t l, lv;
   float xl, thr0;
   bool low;   // its logit is -inf, nothing is below: all classes in front of it count, whatever they hold
-  __device__ void fetch(const LogprobP& p, size_t r, const T* x, const Strip<T>& b) {
-    l = p.label ? p.label[r] : kNoClass;
+  __device__ void fetch(const LogprobP& p, size_t r, const T* x, const Strip<T>& b) { fetch(p, p.label ? p.label[r] : kNoClass, x, b, 0); }
+  __device__ void fetch(const LogprobP& p, uint32_t l_, const T* x, const Strip<T>& b, int) {
+    l = l_;
     xl = l < p.x.C ? ld_f(x + l) : 0.f;
     low = xl == -INFINITY;
     lv = l < b.head ? 0 : (l - b.head) / Vec<T>::V;
@@ -386,7 +439,7 @@ __global__ void __launch_bounds__(256) logprob_rows(LogprobP p, uint32_t slots) 
   extern __shared__ __align__(16) Key dyn[];   // batches of vectors, then what the top classes need
   __shared__ Key red[kRowWarps];
   __shared__ Part parts[kRowWarps], whole;
-  __shared__ uint32_t sv[NT == 32 ? 1 : 256], count[kRowWarps];
+  __shared__ uint32_t sv[NT == 32 ? 1 : 256];
   __shared__ uint16_t work[NT == 32 ? kRowWarps : 1][TOP ? 256 : 1];
   grid_dependency();
   cg::cluster_group cluster = cg::this_cluster();
@@ -394,7 +447,7 @@ __global__ void __launch_bounds__(256) logprob_rows(LogprobP p, uint32_t slots) 
   Group<NT> g(red);
   const uint32_t C = p.x.C, warp = threadIdx.x >> 5;
   const float nothing = as_nothing(p.cs);
-  TopMem t = {nullptr, nullptr, TopMem::room(p.top), &count[NT == 32 ? warp : 0]};
+  TopMem t = {nullptr, nullptr, TopMem::room(p.top)};
   if (TOP) {
     t.list = dyn + (size_t)slots * Feed<NT>::kBatch * 2 + (NT == 32 ? (size_t)warp * (p.top + t.cap) : 0);
     t.cand = t.list + p.top;
@@ -405,13 +458,14 @@ __global__ void __launch_bounds__(256) logprob_rows(LogprobP p, uint32_t slots) 
     const T* x = (const T*)p.logits + p.x.offset(r);
     const Strip<T> b(x, C, part, parts_n);
     const uint4* xv = (const uint4*)(x + b.head);
-    Feed<NT> feed = {xv, b.vb, b.ve, g.tid, slots, (uint4*)dyn};
+    Feed<NT> feed(xv, b.vb, b.ve, g.tid, slots, (uint4*)dyn);
     S scan;
     scan.clear();
     Part& a = scan.a;
     const uint32_t cls = g.tid < 2 * V ? b.single(g.tid) : kNoClass;
     const float single = cls != kNoClass ? ld_f(x + cls) : 0.f;
     Label<T> label;
+    feed.template start<T>();
     label.fetch(p, r, x, b);
     feed.template run<T, false>([&](uint32_t v0, const uint4 (&w)[U]) { scan.batch(v0, w, false, b, g.tid, p.cs, nothing, label.lv, label.xl, label.thr0); });
     if (TOP && NT != 32) sv[g.tid] = b.vb + g.tid < b.ve ? value_key(a.m) : 0u;
@@ -535,7 +589,6 @@ __global__ void __launch_bounds__(kStreamThreads, kStreamBlocks) logprob_stream(
   extern __shared__ __align__(16) uint4 ring[];   // batches of vectors, then what the top classes need
   __shared__ LogprobSlot<T> slot[2];
   __shared__ Key red[kRowWarps];
-  __shared__ uint32_t count;
   __shared__ uint16_t work[TOP ? 2048 : 1];
   grid_dependency();
   const uint32_t shift = slot_shift<T>(p.x.C), slots = (p.x.C / V + (Str::kBatch << shift) - 1) / (Str::kBatch << shift);
@@ -609,7 +662,7 @@ __global__ void __launch_bounds__(kStreamThreads, kStreamBlocks) logprob_stream(
       }
     }
   } else {
-    TopMem t = {nullptr, nullptr, TopMem::room(p.top), &count};
+    TopMem t = {nullptr, nullptr, TopMem::room(p.top)};
     t.list = (Key*)(maxima + (TOP ? 2 * slots * 256 : 0));
     t.cand = t.list + p.top;
     struct Row {   // what this warp keeps of a row between its two turns
@@ -617,6 +670,7 @@ __global__ void __launch_bounds__(kStreamThreads, kStreamBlocks) logprob_stream(
       float single, old;
       Factors f;
     };
+    uint32_t coming = p.label && blockIdx.x < p.x.rows ? p.label[blockIdx.x] : kNoClass;   // the label of the row to be prepared next
     auto prepare = [&](size_t r, uint32_t i) {
       Row w = {kNoClass, 0, 0.f, 0.f, {}};
       if (r >= p.x.rows) return w;
@@ -625,7 +679,9 @@ __global__ void __launch_bounds__(kStreamThreads, kStreamBlocks) logprob_stream(
       const T* x = (const T*)p.logits + p.x.offset(r);
       const Strip<T> b(x, C);
       Label<T> label;
-      label.fetch(p, r, x, b);
+      label.fetch(p, coming, x, b, 0);
+      const size_t after = r + gridDim.x;
+      coming = p.label && after < p.x.rows ? p.label[after] : kNoClass;
       w.cls = lane < 2 * V ? b.single(lane) : kNoClass;
       if (w.cls != kNoClass) {
         w.single = ld_f(x + w.cls);
@@ -942,7 +998,7 @@ static int launch_rows(const LogprobP& p, cudaStream_t s) {
       cudaGetLastError();
       return AD_ERR_CUDA;
     }
-    launch(kernel, stream_grid(p.x.rows), kStreamThreads, smem, s, p);
+    launch(kernel, stream_grid(p.x.rows, smem), kStreamThreads, smem, s, p);
     return AD_OK;
   }
   auto kernel = logprob_rows<NT, T, ENT, RANK, TOP, BWD>;

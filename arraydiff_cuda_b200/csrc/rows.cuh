@@ -385,49 +385,62 @@ struct Feed {
   const uint4* xv;
   uint32_t vb, ve, tid, slots;
   uint4* mem;
+  uint32_t put, get;
+  uint4 w[U];
+  __device__ Feed(const uint4* xv_, uint32_t vb_, uint32_t ve_, uint32_t tid_, uint32_t slots_, uint4* mem_) : xv(xv_), vb(vb_), ve(ve_), tid(tid_), slots(slots_), mem(mem_) {}
+  __device__ uint32_t batches() const { return (ve - vb + kBatch - 1) / kBatch; }
+  __device__ __forceinline__ void copy(uint32_t i) {
+    if (i < batches()) {
+      const uint32_t v0 = vb + i * kBatch + tid;
+#pragma unroll
+      for (uint32_t u = 0; u < U; ++u)
+        if (v0 + u * NT < ve) copy_async(shared_address(mem + put * kBatch + u * NT + tid), xv + v0 + u * NT);
+      if (++put == slots) put = 0;
+    }
+    commit_copies();
+  }
+  template <typename T> __device__ __forceinline__ void load(uint32_t v0) {
+#pragma unroll
+    for (uint32_t u = 0; u < U; ++u) {
+      const uint32_t v = v0 + u * NT + tid;
+      w[u] = v < ve ? xv[v] : Vec<T>::none();
+    }
+  }
+  template <typename T> __device__ __forceinline__ void take(uint32_t v0, const uint4* slot) {
+#pragma unroll
+    for (uint32_t u = 0; u < U; ++u) w[u] = v0 + u * NT + tid < ve ? load_shared(shared_address(slot + u * NT + tid)) : Vec<T>::none();
+  }
+  // the first loads of a pass
+  template <typename T> __device__ __forceinline__ void start() {
+    if constexpr (NT == 32) {
+      load<T>(vb);
+    } else {
+      put = get = 0;
+#pragma unroll
+      for (int i = 0; i < kAheadBatches; ++i) copy(i);
+    }
+  }
   template <typename T, bool AGAIN, typename F>
   __device__ __forceinline__ void run(F&& f) {
-    uint4 w[U];
     if constexpr (NT == 32) {
+      if (AGAIN) load<T>(vb);
       for (uint32_t v0 = vb; v0 < ve; v0 += kBatch) {
-#pragma unroll
-        for (uint32_t u = 0; u < U; ++u) {
-          const uint32_t v = v0 + u * NT + tid;
-          w[u] = v < ve ? xv[v] : Vec<T>::none();
-        }
+        if (v0 != vb) load<T>(v0);
         f(v0, w);
       }
     } else {
-      const uint32_t n = (ve - vb + kBatch - 1) / kBatch;
-      auto take = [&](uint32_t v0, const uint4* slot) {
-#pragma unroll
-        for (uint32_t u = 0; u < U; ++u) w[u] = v0 + u * NT + tid < ve ? slot[u * NT + tid] : Vec<T>::none();
-      };
+      const uint32_t n = batches();
       if (AGAIN && n <= slots) {
         for (uint32_t i = 0; i < n; ++i) {
-          take(vb + i * kBatch, mem + i * kBatch);
+          take<T>(vb + i * kBatch, mem + i * kBatch);
           f(vb + i * kBatch, w);
         }
         return;
       }
-      uint32_t put = 0, get = 0;
-      auto copy = [&](uint32_t i) {
-        if (i < n) {
-          const uint32_t v0 = vb + i * kBatch + tid;
-#pragma unroll
-          for (uint32_t u = 0; u < U; ++u)
-            if (v0 + u * NT < ve)
-              asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(mem + put * kBatch + u * NT + tid)),
-                           "l"(xv + v0 + u * NT) : "memory");
-          if (++put == slots) put = 0;
-        }
-        asm volatile("cp.async.commit_group;" ::: "memory");
-      };
-#pragma unroll
-      for (int i = 0; i < kAheadBatches; ++i) copy(i);
+      if (AGAIN) start<T>();
       for (uint32_t i = 0; i < n; ++i) {
-        asm volatile("cp.async.wait_group %0;" ::"n"(kAheadBatches - 1) : "memory");
-        take(vb + i * kBatch, mem + get * kBatch);
+        wait_copies<kAheadBatches - 1>();
+        take<T>(vb + i * kBatch, mem + get * kBatch);
         if (++get == slots) get = 0;
         f(vb + i * kBatch, w);
         copy(i + kAheadBatches);   // into the slot that has just been read, where there are no more
@@ -505,7 +518,7 @@ struct Stream {
     for (uint32_t i = 0; i < kAhead; ++i) copy();
   }
   // f(v0, w, full) for the batches of a row of n vectors: the ones that were copied first.  full: all threads have all of theirs
-  template <typename F> __device__ __forceinline__ void run(uint32_t n, F&& f) {
+  template <typename F> __device__ __forceinline__ void run(uint32_t n, F&& f) {   // f may change w
     for (uint32_t v0 = 0; v0 < n; v0 += kBatch) {
       uint4 w[U];
       wait_copies<kAhead - 1>();
@@ -524,7 +537,11 @@ struct Stream {
     }
   }
 };
-inline unsigned stream_grid(size_t rows) { return (unsigned)(rows < kStreamBlocks * kNumSMs ? rows : kStreamBlocks * kNumSMs); }
+// Blocks that are resident together, each with `smem` bytes and up to 8 KB that the kernels have besides
+inline unsigned stream_grid(size_t rows, size_t smem) {
+  const size_t room = 227 * 1024 / (smem + 9 * 1024), n = (room < kStreamBlocks ? (room ? room : 1) : kStreamBlocks) * kNumSMs;
+  return (unsigned)(rows < n ? rows : n);
+}
 
 // Plain loops over a row in any layout: what the fast pass does not serve
 template <typename G, typename T, bool ENT>
