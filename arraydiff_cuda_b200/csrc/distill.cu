@@ -399,43 +399,52 @@ __global__ void __launch_bounds__(256) distill_rows(DistillP p, uint32_t slots) 
 }
 
 // Many rows of many classes: see Stream.  Two rows are in hand, by parity.
+template <int W>
 struct __align__(16) DistillSlot {
   List list;
   float old[kMostTop], grad[kMostTop];   // what the gradient of an entry's class is added to, and that gradient
-  Part parts[kRowWarps];
+  Part parts[W];
   float mc, coef;
   uint32_t singles;                      // which of the row's single elements are listed
   bool strange;
 };
 template <typename T, bool REST, bool BWD>
-__global__ void __launch_bounds__(kStreamThreads, kStreamBlocks) distill_stream(DistillP p, uint32_t mask_bytes) {
-  typedef Stream<T, BWD> Str;
+__global__ void __launch_bounds__(Crew<8>::kThreads, Crew<8>::kBlocks) distill_stream(DistillP p, RingPlan plan, uint32_t mask_bytes) {
+  constexpr int W = 8;
+  typedef Crew<W> Team;
+  typedef Stream<T, W, BWD> Str;
   constexpr int U = Str::U, V = Vec<T>::V;
+  constexpr uint32_t NS = Str::NS;
   typedef Vec<T> X;
   extern __shared__ __align__(16) uint8_t dyn[];   // batches of vectors, then two masks: a byte per vector
-  __shared__ DistillSlot slot[2];
-  __shared__ Key red[kRowWarps];
+  __shared__ DistillSlot<W> slot[2];
+  __shared__ Key red[W];
+  __shared__ Part whole[2];
   __shared__ Distilled shared;
   grid_dependency();
+  cg::cluster_group cluster = cg::this_cluster();
+  const uint32_t parts = BWD ? cluster.num_blocks() : 1, part = BWD ? cluster.block_rank() : 0, row0 = blockIdx.x / parts, stride = gridDim.x / parts;
+  const uint32_t rows = (uint32_t)p.x.rows;
   const uint32_t C = p.x.C, k = p.top, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  uint8_t* masks = dyn + Str::kAhead * Str::kBytes;
-  if (warp < kRowWarps) {
-    Str stream((const T*)p.logits, p.x, dyn);
+  uint8_t* masks = dyn + plan.bytes;
+  if (warp < W) {
+    Str stream((const T*)p.logits, p.x, dyn, plan.slots, plan.twice != 0, row0, stride, part, parts);
     uint32_t i = 0;
-    for (size_t r = blockIdx.x; r < p.x.rows; r += gridDim.x, ++i) {
-      DistillSlot& q = slot[i & 1];
+    for (uint32_t r = row0; r < rows; r += stride, ++i) {
+      DistillSlot<W>& q = slot[i & 1];
       const T* x = (const T*)p.logits + p.x.offset(r);
-      const Strip<T> b(x, C);
+      const Strip<T> b(x, C, part, parts);
+      const uint32_t nv = b.ve - b.vb;
       const uint8_t* mask = masks + (i & 1) * mask_bytes + tid;
-      bar_wait(kBarReady + (i & 1));
+      Team::wait(kBarReady + (i & 1));
       Part a;
       a.clear();
-      stream.run(b.nv, [&](uint32_t v0, uint4 (&w)[U], bool full) {
+      auto sums = [&](uint32_t v0, uint4 (&w)[U], bool full) {
         if (REST) {
           uint32_t out[U], any = 0;
 #pragma unroll
           for (int u = 0; u < U; ++u) {
-            out[u] = full || v0 + u * kRowThreads + tid < b.nv ? mask[v0 + u * kRowThreads] : 0;
+            out[u] = full || v0 + u * NS + tid < nv ? mask[v0 + u * NS] : 0;
             any |= out[u];
           }
           if (any) {
@@ -446,46 +455,50 @@ __global__ void __launch_bounds__(kStreamThreads, kStreamBlocks) distill_stream(
         typename X::Max most = X::max(w[0]);
 #pragma unroll
         for (int u = 1; u < U; ++u) most = X::max(most, X::max(w[u]));
-        add_vectors<false, U, T>(a, w, full ? U : (int)((b.nv - v0 + kRowThreads - 1) / kRowThreads), X::value(most), p.cs, 0.f);
-      });
+        add_vectors<false, U, T>(a, w, full ? U : (int)((nv - v0 + NS - 1) / NS), X::value(most), p.cs, 0.f);
+      };
+      if (BWD && !plan.twice) stream.look(nv, sums);
+      else stream.run(nv, sums);
       a.join<false, 32>(p.cs);
       if (lane == 0) q.parts[warp] = a;
-      bar_arrive(kBarSums + (i & 1));
+      Team::arrive(kBarSums + (i & 1));
       if constexpr (BWD) {
-        bar_wait(kBarResult + (i & 1));
+        __syncwarp();
+        if (parts > 1) cluster.sync();
+        Team::wait(kBarResult + (i & 1));
         T* o = (T*)p.dlogits + p.g.offset(r);
         const bool even = (((uintptr_t)o ^ (uintptr_t)x) & 15u) == 0, plain = q.strange;
         const float mc = q.mc, coef = q.coef;
-        T* to = o + b.head + tid * V;   // this thread's vector of the batch
-        stream.run(b.nv, [&](uint32_t v0, uint4 (&w)[U], bool full) {
+        T* to = o + b.class_of(b.vb) + tid * V;   // this thread's vector of the batch
+        stream.run(nv, [&](uint32_t v0, uint4 (&w)[U], bool full) {
           if (!plain) {
             if (full && even && !p.accumulate) {
 #pragma unroll
               for (int u = 0; u < U; ++u) {
                 float h[V];
                 grad_vector<false, T>(w[u], h, p.cs, mc, coef, 0.f, 0.f);
-                *(uint4*)(to + u * kRowThreads * V) = X::pack(h);
+                __stcs((uint4*)(to + u * NS * V), X::pack(h));
               }
             } else {
 #pragma unroll
               for (int u = 0; u < U; ++u) {
-                if (v0 + u * kRowThreads + tid >= b.nv) break;
+                if (v0 + u * NS + tid >= nv) break;
                 float h[V];
                 grad_vector<false, T>(w[u], h, p.cs, mc, coef, 0.f, 0.f);
-                put_vector<T>(to + u * kRowThreads * V, even, p.accumulate, h);
+                put_vector<T>(to + u * NS * V, even, p.accumulate, h);
               }
             }
           }
           to += Str::kBatch * V;
         });
-        Group<kRowThreads> g(red);
+        Group<(int)NS> g(red);
         if (plain) {
-          plain_row<kRowThreads, T, true>(g, p, r, q.list, &shared);
+          if (part == 0) plain_row<(int)NS, T, true>(g, p, r, q.list, &shared);
         } else {
           g.sync();   // the list's classes over what the loop wrote
-          if (tid < k && q.list.cls[tid] < C) st_f(o + q.list.cls[tid], q.grad[tid]);
+          if (tid < k && q.list.cls[tid] >= b.begin() && q.list.cls[tid] < b.end()) st_f(o + q.list.cls[tid], q.grad[tid]);
         }
-        if (r + 2 * (size_t)gridDim.x < p.x.rows) bar_arrive(kBarFree + (i & 1));   // there is a row to come in this slot
+        if (r + 2 * stride < rows) Team::arrive(kBarFree + (i & 1));   // there is a row to come in this slot
       }
     }
   } else {
@@ -494,15 +507,15 @@ __global__ void __launch_bounds__(kStreamThreads, kStreamBlocks) distill_stream(
       float single, old, Q, mk, K, dloss;
       bool apart;
     };
-    auto prepare = [&](size_t r, uint32_t i) {
+    auto prepare = [&](uint32_t r, uint32_t i) {
       Row w = {kNoClass, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, true};
-      if (r >= p.x.rows) return w;
-      if (BWD && i >= 2) bar_wait(kBarFree + (i & 1));
-      DistillSlot& q = slot[i & 1];
+      if (r >= rows) return w;
+      if (BWD && i >= 2) Team::wait(kBarFree + (i & 1));
+      DistillSlot<W>& q = slot[i & 1];
       uint8_t* mask = masks + (i & 1) * mask_bytes;
       const T* x = (const T*)p.logits + p.x.offset(r);
       const T* o = (const T*)p.dlogits + (BWD ? p.g.offset(r) : 0);
-      const Strip<T> b(x, C);
+      const Strip<T> b(x, C, part, parts);
       uint32_t cls[4];
       float a[4], xs[4];
 #pragma unroll
@@ -539,21 +552,25 @@ __global__ void __launch_bounds__(kStreamThreads, kStreamBlocks) distill_stream(
       // which classes are listed, and whether one of them stands twice
       bool twice = false;
       if (REST) {
-        for (uint32_t v = lane; v < (b.nv + 15) / 16; v += 32) ((uint4*)mask)[v] = make_uint4(0, 0, 0, 0);
+        for (uint32_t v = lane; v < (b.ve - b.vb + 15) / 16; v += 32) ((uint4*)mask)[v] = make_uint4(0, 0, 0, 0);
         if (lane == 0) q.singles = 0;
         __syncwarp();
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const uint32_t c = cls[e];
           if (c >= C) continue;
-          if (c >= b.head && c < b.head + b.nv * V) {
-            const uint32_t v = (c - b.head) / V, bit = 1u << (v % 4 * 8 + (c - b.head) % V);
-            twice |= (atomicOr((uint32_t*)mask + v / 4, bit) & bit) != 0;
+          const uint32_t v = (c - b.head) / V;
+          if (c >= b.head && v < b.nv) {
+            if (v >= b.vb && v < b.ve) {   // this block's part
+              const uint32_t at = v - b.vb, bit = 1u << (at % 4 * 8 + (c - b.head) % V);
+              twice |= (atomicOr((uint32_t*)mask + at / 4, bit) & bit) != 0;
+            }
           } else {
             const uint32_t bit = 1u << (c < b.head ? c : V + (c - b.head - b.nv * V));
             twice |= (atomicOr(&q.singles, bit) & bit) != 0;
           }
         }
+        if (parts > 1) twice = true;   // the other parts are not known: looked for below
         twice = __any_sync(0xffffffffu, twice);
         __syncwarp();
         w.apart = !(q.singles >> lane & 1u);
@@ -597,20 +614,28 @@ __global__ void __launch_bounds__(kStreamThreads, kStreamBlocks) distill_stream(
       }
       w.Q = warp_sum(w.Q);
       if (lane == 0) q.list.twice = twice;
-      bar_arrive(kBarReady + (i & 1));
+      Team::arrive(kBarReady + (i & 1));
       return w;
     };
     uint32_t i = 0;
-    Row now = prepare(blockIdx.x, 0);
-    for (size_t r = blockIdx.x; r < p.x.rows; r += gridDim.x, ++i) {
-      const Row next = prepare(r + gridDim.x, i + 1);
-      DistillSlot& q = slot[i & 1];
-      bar_wait(kBarSums + (i & 1));
+    Row now = prepare(row0, 0);
+    for (uint32_t r = row0; r < rows; r += stride, ++i) {
+      const Row next = prepare(r + stride, i + 1);
+      DistillSlot<W>& q = slot[i & 1];
+      Team::wait(kBarSums + (i & 1));
       Part a;
       a.clear();
-      if (lane < kRowWarps) a = q.parts[lane];
+      if (lane < W) a = q.parts[lane];
       if (now.cls != kNoClass && now.apart) a.add<false>(now.single, p.cs);
       a.join<false, 32>(p.cs);
+      if (parts > 1) {
+        if (lane == 0) whole[i & 1] = a;
+        __syncwarp();
+        cluster.sync();
+        a.clear();
+        if (lane % 8 < parts) a = *cluster.map_shared_rank(&whole[i & 1], lane % 8);
+        a.join<false, 8>(p.cs);
+      }
       const bool strange = a.strange(p.cs);
       const float off = a.m == -INFINITY ? 0.f : fmaf(-a.m, p.cs, a.mc);
       float loss;
@@ -642,10 +667,10 @@ __global__ void __launch_bounds__(kStreamThreads, kStreamBlocks) distill_stream(
           }
           // before the list's, which the streaming threads write behind this barrier
           if (now.cls != kNoClass) st_f((T*)p.dlogits + p.g.offset(r) + now.cls, f * d.out * exp2_fast(fmaf(now.single, p.cs, -a.mc)) + now.old);
-          bar_arrive(kBarResult + (i & 1));
+          Team::arrive(kBarResult + (i & 1));
         }
         loss += warp_sum(terms);
-        if (lane == 0 && p.loss) p.loss[r] = d.some ? loss + 0.f * d.L : 0.f;
+        if (lane == 0 && part == 0 && p.loss) p.loss[r] = d.some ? loss + 0.f * d.L : 0.f;
       } else {
         // the plain loops want the list as it is fetched
         Group<32> g(nullptr);
@@ -653,7 +678,7 @@ __global__ void __launch_bounds__(kStreamThreads, kStreamBlocks) distill_stream(
         fetch_list<32, T>(g, p, r, (const T*)p.logits + p.x.offset(r), 1, q.list);
         if (BWD) {
           if (lane == 0) q.strange = true;
-          bar_arrive(kBarResult + (i & 1));
+          Team::arrive(kBarResult + (i & 1));
         } else {
           plain_row<32, T, false>(g, p, r, q.list, &shared);
         }
@@ -661,6 +686,8 @@ __global__ void __launch_bounds__(kStreamThreads, kStreamBlocks) distill_stream(
       now = next;
     }
   }
+  __syncwarp();
+  if (parts > 1) cluster.sync();   // nobody leaves while its sums are still read
 }
 
 // ---------------------------------------------------------------- a thread per position
@@ -824,17 +851,14 @@ static int distill_args(const ad_distill_args* a, bool bwd, DistillP& p) {
 
 template <int NT, typename T, bool REST, bool BWD>
 static int launch_rows(const DistillP& p, uint32_t n, size_t mask, cudaStream_t s) {
-  if (NT != 32 && stream_worth(p.x.rows)) {
-    typedef Stream<T, BWD> Str;
-    const size_t bytes = REST ? (p.x.C / Vec<T>::V + 15) / 16 * 16 : 0, smem = Str::kAhead * Str::kBytes + 2 * bytes;
-    if (bytes <= kMostMask / 2) {
-      auto kernel = distill_stream<T, REST, BWD>;
-      if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(Str::kAhead * Str::kBytes + kMostMask)) != cudaSuccess) {
-        cudaGetLastError();
-        return AD_ERR_CUDA;
-      }
-      launch(kernel, stream_grid(p.x.rows, smem), kStreamThreads, smem, s, p, (uint32_t)bytes);
-      return AD_OK;
+  if constexpr (NT != 32) {
+    constexpr int W = 8;
+    auto bytes = [&](uint32_t parts) { return REST ? (p.x.C / Vec<T>::V / parts + 1 + 15) / 16 * 16 : (size_t)0; };   // of a mask
+    const RingPlan plan = ring_plan<T, W, BWD>(p.x.C, [&](uint32_t parts) { return 2 * bytes(parts) < kMostMask ? 2 * bytes(parts) : kMostMask; });
+    const size_t one = bytes(plan.parts);
+    if (one <= kMostMask / 2 && stream_worth<W>(p.x.rows, plan.parts)) {
+      static StreamLaunch shared;
+      return launch_stream<W>(distill_stream<T, REST, BWD>, shared, p.x.rows, plan.parts, plan.bytes + 2 * one, s, p, plan, (uint32_t)one);
     }
   }
   auto kernel = distill_rows<NT, T, REST, BWD>;

@@ -303,7 +303,7 @@ __device__ void plain_row(Group<NT>& g, const LogprobP& p, size_t r, const TopMe
   const float xl = l < C ? ld_f(x + l * st) : 0.f;
   RowSums s;
   float E;
-  plain_sums<Group<NT>, T, true>(g, x, st, C, p.cs, s, E);
+  plain_sums<NT, T, true>(g, x, st, C, p.cs, s, E);
   const float H = s.some ? kLn2 * (s.L - E / s.S) : 0.f;
   if (g.tid == 0) put_row(p, s, r, H, l, xl);
   if constexpr (!BWD) {
@@ -347,9 +347,9 @@ __global__ void __launch_bounds__(256) logprob_any(LogprobP p) {
 
 // ---------------------------------------------------------------- rows of many neighbouring classes
 // What a thread finds in its vectors: sums, classes in front of the label, its shares of the row
-template <int NT, typename T, bool ENT, bool RANK, bool TOP>
+template <int NT, typename T, bool ENT, bool RANK, bool TOP, int U_ = NT == 32 ? 8 : 4>
 struct Scan {
-  static constexpr int U = NT == 32 ? 8 : 4, SH = NT == 32 ? 8 : 1;
+  static constexpr int U = U_, SH = NT == 32 ? 8 : 1;
   typedef Vec<T> X;
   Part a;
   uint32_t km[SH];   // maxima of the eight shares of a lane, as keys; a thread's own share has a.m
@@ -572,93 +572,105 @@ __host__ __device__ inline uint32_t slot_shift(uint32_t C) {
   return s;
 }
 // Many rows of many classes: see Stream.  Two rows are in hand, by parity.
-template <typename T>
+template <typename T, int W>
 struct LogprobSlot {
   Label<T> label;
-  Part parts[kRowWarps];
+  Part parts[W];
   uint32_t sv[256];
   Factors f;
   float mc;
   bool strange;
 };
 template <typename T, bool ENT, bool RANK, bool TOP, bool BWD>
-__global__ void __launch_bounds__(kStreamThreads, kStreamBlocks) logprob_stream(LogprobP p) {
-  typedef Scan<kRowThreads, T, ENT, RANK, TOP> S;
-  typedef Stream<T, BWD> Str;
+__global__ void __launch_bounds__(Crew<8>::kThreads, Crew<8>::kBlocks) logprob_stream(LogprobP p, RingPlan plan) {
+  constexpr int W = 8;
+  typedef Crew<W> Team;
+  typedef Stream<T, W, BWD> Str;
   constexpr int U = Str::U, V = Vec<T>::V;
+  constexpr uint32_t NS = Str::NS;
+  typedef Scan<(int)NS, T, ENT, RANK, TOP, U> S;
   extern __shared__ __align__(16) uint4 ring[];   // batches of vectors, then what the top classes need
-  __shared__ LogprobSlot<T> slot[2];
-  __shared__ Key red[kRowWarps];
+  __shared__ LogprobSlot<T, W> slot[2];
+  __shared__ Key red[W];
+  __shared__ Part whole[2];
   __shared__ uint16_t work[TOP ? 2048 : 1];
   grid_dependency();
+  cg::cluster_group cluster = cg::this_cluster();
+  const uint32_t parts = BWD ? cluster.num_blocks() : 1, part = BWD ? cluster.block_rank() : 0, row0 = blockIdx.x / parts, stride = gridDim.x / parts;
+  const uint32_t rows = (uint32_t)p.x.rows;
   const uint32_t shift = slot_shift<T>(p.x.C), slots = (p.x.C / V + (Str::kBatch << shift) - 1) / (Str::kBatch << shift);
-  uint16_t* maxima = (uint16_t*)(ring + Str::kAhead * Str::kBatch);   // [2][slots][256]
+  uint16_t* maxima = (uint16_t*)((uint8_t*)ring + plan.bytes);   // [2][slots][256]
   const uint32_t C = p.x.C, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const float nothing = as_nothing(p.cs);
-  if (warp < kRowWarps) {
-    Str stream((const T*)p.logits, p.x, ring);
+  if (warp < W) {
+    Str stream((const T*)p.logits, p.x, ring, plan.slots, plan.twice != 0, row0, stride, part, parts);
     uint32_t i = 0;
-    for (size_t r = blockIdx.x; r < p.x.rows; r += gridDim.x, ++i) {
-      LogprobSlot<T>& q = slot[i & 1];
+    for (uint32_t r = row0; r < rows; r += stride, ++i) {
+      LogprobSlot<T, W>& q = slot[i & 1];
       const T* x = (const T*)p.logits + p.x.offset(r);
-      const Strip<T> b(x, C);
-      bar_wait(kBarReady + (i & 1));
+      const Strip<T> b(x, C, part, parts);
+      Team::wait(kBarReady + (i & 1));
       const uint32_t lv = q.label.lv;
       const float xl = q.label.xl, thr0 = q.label.thr0;
       S scan;
       scan.clear();
       uint16_t* mine = maxima + (i & 1) * slots * 256 + tid;
       float most = -INFINITY;
-      stream.run(b.nv, [&](uint32_t v0, const uint4 (&w)[U], bool full) {
-        const float bm = scan.batch(v0, w, full, b, tid, p.cs, nothing, lv, xl, thr0);
+      auto sums = [&](uint32_t v0, const uint4 (&w)[U], bool full) {
+        const float bm = scan.batch(b.vb + v0, w, full, b, tid, p.cs, nothing, lv, xl, thr0);
         if (TOP) {   // the slot's maximum so far
           const uint32_t n = v0 / Str::kBatch;
           most = (n & ((1u << shift) - 1)) ? fmaxf(most, bm) : bm;
           mine[(n >> shift) * 256] = (uint16_t)(__float_as_uint(most + 0.f) >> 16);
         }
-      });
-      if (TOP) q.sv[tid] = tid < b.nv ? value_key(scan.a.m) : 0u;
+      };
+      const uint32_t nv = b.ve - b.vb;
+      if (BWD && !plan.twice) stream.look(nv, sums);
+      else stream.run(nv, sums);
+      if (TOP) q.sv[tid] = tid < nv ? value_key(scan.a.m) : 0u;
       scan.a.template join<ENT, 32>(p.cs);
       if (lane == 0) q.parts[warp] = scan.a;
-      bar_arrive(kBarSums + (i & 1));
+      Team::arrive(kBarSums + (i & 1));
       if constexpr (BWD) {
-        bar_wait(kBarResult + (i & 1));
+        __syncwarp();
+        if (parts > 1) cluster.sync();
+        Team::wait(kBarResult + (i & 1));
         T* o = (T*)p.dlogits + p.g.offset(r);
         const bool even = (((uintptr_t)o ^ (uintptr_t)x) & 15u) == 0, plain = q.strange;
-        const Factors f = q.f;
-        const float mc = q.mc;
+        const float c0 = q.f.c0, c1 = q.f.c1, mc = q.mc;
         // the thread that has the label's vector writes its class once more
-        const uint32_t l = q.label.l < C && q.label.l >= b.head && lv < b.nv && lv % kRowThreads == tid ? lv : kNoClass;
-        const float gl = f.grad<ENT>(xl, p.cs, mc) + f.dl, old = l != kNoClass && p.accumulate ? ld_f(o + q.label.l) : 0.f;
-        T* to = o + b.head + tid * V;   // this thread's vector of the batch
-        stream.run(b.nv, [&](uint32_t v0, const uint4 (&w)[U], bool full) {
+        const uint32_t l = q.label.l < C && q.label.l >= b.head && lv >= b.vb && lv < b.ve && (lv - b.vb) % NS == tid ? lv - b.vb : kNoClass;
+        float gl = 0.f;
+        if (l != kNoClass) gl = q.f.template grad<ENT>(xl, p.cs, mc) + q.f.dl + (p.accumulate ? ld_f(o + q.label.l) : 0.f);
+        T* to = o + b.class_of(b.vb) + tid * V;   // this thread's vector of the batch
+        stream.run(nv, [&](uint32_t v0, const uint4 (&w)[U], bool full) {
           if (!plain) {
             if (full && even && !p.accumulate) {
 #pragma unroll
               for (int u = 0; u < U; ++u) {
                 float h[V];
-                grad_vector<ENT, T>(w[u], h, p.cs, mc, f.c0, f.c1, nothing);
-                *(uint4*)(to + u * kRowThreads * V) = Vec<T>::pack(h);
+                grad_vector<ENT, T>(w[u], h, p.cs, mc, c0, c1, nothing);
+                __stcs((uint4*)(to + u * NS * V), Vec<T>::pack(h));
               }
             } else {
 #pragma unroll
               for (int u = 0; u < U; ++u) {
-                if (v0 + u * kRowThreads + tid >= b.nv) break;
+                if (v0 + u * NS + tid >= nv) break;
                 float h[V];
-                grad_vector<ENT, T>(w[u], h, p.cs, mc, f.c0, f.c1, nothing);
-                put_vector<T>(to + u * kRowThreads * V, even, p.accumulate, h);
+                grad_vector<ENT, T>(w[u], h, p.cs, mc, c0, c1, nothing);
+                put_vector<T>(to + u * NS * V, even, p.accumulate, h);
               }
             }
-            if (l - v0 < Str::kBatch) st_f(o + q.label.l, gl + old);
+            if (l - v0 < Str::kBatch) st_f(o + q.label.l, gl);
           }
           to += Str::kBatch * V;
         });
-        if (plain) {
-          Group<kRowThreads> g(red);
+        if (plain && part == 0) {
+          Group<(int)NS> g(red);
           const TopMem none = {};
-          plain_row<kRowThreads, T, true>(g, p, r, none);
+          plain_row<(int)NS, T, true>(g, p, r, none);
         }
-        if (r + 2 * (size_t)gridDim.x < p.x.rows) bar_arrive(kBarFree + (i & 1));   // there is a row to come in this slot
+        if (r + 2 * stride < rows) Team::arrive(kBarFree + (i & 1));   // there is a row to come in this slot
       }
     }
   } else {
@@ -670,18 +682,17 @@ __global__ void __launch_bounds__(kStreamThreads, kStreamBlocks) logprob_stream(
       float single, old;
       Factors f;
     };
-    uint32_t coming = p.label && blockIdx.x < p.x.rows ? p.label[blockIdx.x] : kNoClass;   // the label of the row to be prepared next
-    auto prepare = [&](size_t r, uint32_t i) {
+    uint32_t coming = p.label && row0 < rows ? p.label[row0] : kNoClass;   // the label of the row to be prepared next
+    auto prepare = [&](uint32_t r, uint32_t i) {
       Row w = {kNoClass, 0, 0.f, 0.f, {}};
-      if (r >= p.x.rows) return w;
-      if (BWD && i >= 2) bar_wait(kBarFree + (i & 1));
-      LogprobSlot<T>& q = slot[i & 1];
+      if (r >= rows) return w;
+      if (BWD && i >= 2) Team::wait(kBarFree + (i & 1));
+      LogprobSlot<T, W>& q = slot[i & 1];
       const T* x = (const T*)p.logits + p.x.offset(r);
-      const Strip<T> b(x, C);
+      const Strip<T> b(x, C, part, parts);
       Label<T> label;
       label.fetch(p, coming, x, b, 0);
-      const size_t after = r + gridDim.x;
-      coming = p.label && after < p.x.rows ? p.label[after] : kNoClass;
+      coming = p.label && r + stride < rows ? p.label[r + stride] : kNoClass;
       w.cls = lane < 2 * V ? b.single(lane) : kNoClass;
       if (w.cls != kNoClass) {
         w.single = ld_f(x + w.cls);
@@ -691,24 +702,32 @@ __global__ void __launch_bounds__(kStreamThreads, kStreamBlocks) logprob_stream(
       if (BWD) w.f.fetch(p, r, label.l);
       if (lane == 0) q.label = label;
       __syncwarp();
-      bar_arrive(kBarReady + (i & 1));
+      Team::arrive(kBarReady + (i & 1));
       return w;
     };
     uint32_t i = 0;
-    Row now = prepare(blockIdx.x, 0);
-    for (size_t r = blockIdx.x; r < p.x.rows; r += gridDim.x, ++i) {
-      const Row next = prepare(r + gridDim.x, i + 1);
-      LogprobSlot<T>& q = slot[i & 1];
+    Row now = prepare(row0, 0);
+    for (uint32_t r = row0; r < rows; r += stride, ++i) {
+      const Row next = prepare(r + stride, i + 1);
+      LogprobSlot<T, W>& q = slot[i & 1];
       const T* x = (const T*)p.logits + p.x.offset(r);
-      const Strip<T> b(x, C);
+      const Strip<T> b(x, C, part, parts);
       const Label<T> label = q.label;
-      bar_wait(kBarSums + (i & 1));
+      Team::wait(kBarSums + (i & 1));
       Part a;
       a.clear();
-      if (lane < kRowWarps) a = q.parts[lane];
+      if (lane < W) a = q.parts[lane];
       if (now.cls != kNoClass) a.add<ENT>(now.single, p.cs);
       if (RANK) a.cnt += now.own + (now.cls != kNoClass && label.single_counts(now.single, now.cls));
       a.join<ENT, 32>(p.cs);
+      if (parts > 1) {
+        if (lane == 0) whole[i & 1] = a;
+        __syncwarp();
+        cluster.sync();
+        a.clear();
+        if (lane % 8 < parts) a = *cluster.map_shared_rank(&whole[i & 1], lane % 8);
+        a.join<ENT, 8>(p.cs);
+      }
       const bool strange = a.strange(p.cs);
       RowSums s;
       s.set(a.m, a.mc, a.S, p.cs);
@@ -721,7 +740,7 @@ __global__ void __launch_bounds__(kStreamThreads, kStreamBlocks) logprob_stream(
           q.mc = s.mc;
           q.strange = strange;
         }
-        bar_arrive(kBarResult + (i & 1));
+        Team::arrive(kBarResult + (i & 1));
         if (!strange && now.cls != kNoClass)
           st_f((T*)p.dlogits + p.g.offset(r) + now.cls, f.grad<ENT>(now.single, p.cs, s.mc) + (now.cls == label.l ? f.dl : 0.f) + now.old);
       }
@@ -729,7 +748,7 @@ __global__ void __launch_bounds__(kStreamThreads, kStreamBlocks) logprob_stream(
         Group<32> g(nullptr);
         if (!BWD) plain_row<32, T, false>(g, p, r, t);
       } else {
-        if (lane == 0) {
+        if (lane == 0 && part == 0) {
           put_row(p, s, r, H, label.l, label.xl);
           if (RANK) p.rank[r] = label.rank(a.cnt, C);
         }
@@ -746,6 +765,8 @@ __global__ void __launch_bounds__(kStreamThreads, kStreamBlocks) logprob_stream(
       now = next;
     }
   }
+  __syncwarp();
+  if (parts > 1) cluster.sync();   // nobody leaves while its sums are still read
 }
 
 // ---------------------------------------------------------------- a thread per position
@@ -988,18 +1009,15 @@ template <int NT, typename T, bool ENT, bool RANK, bool TOP, bool BWD>
 static int launch_rows(const LogprobP& p, cudaStream_t s) {
   const size_t bytes = (size_t)p.x.C * sizeof(T), list = p.top + TopMem::room(p.top);
   // the limits belong to the functions: the most that they take
-  if (NT != 32 && stream_worth(p.x.rows)) {
-    auto kernel = logprob_stream<T, ENT, RANK, TOP, BWD>;
-    typedef Stream<T, BWD> Str;
-    constexpr size_t ring = Str::kAhead * Str::kBytes;
-    const uint32_t shift = slot_shift<T>(p.x.C), slots = (p.x.C / Vec<T>::V + (Str::kBatch << shift) - 1) / (Str::kBatch << shift);
-    const size_t smem = ring + (TOP ? list * sizeof(Key) + 2 * slots * 256 * 2 : 0);
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(ring + 2 * kMostSlots * 256 * 2 + sizeof(Key) * (kMostTop + TopMem::room(kMostTop)))) != cudaSuccess) {
-      cudaGetLastError();
-      return AD_ERR_CUDA;
+  if constexpr (NT != 32) {
+    constexpr int W = 8;
+    const uint32_t shift = slot_shift<T>(p.x.C), slots = (p.x.C / Vec<T>::V + (1024u << shift) - 1) / (1024u << shift);
+    const size_t besides = TOP ? list * sizeof(Key) + 2 * slots * 256 * 2 : 0;
+    const RingPlan plan = ring_plan<T, W, BWD>(p.x.C, [&](uint32_t) { return besides; });
+    if (stream_worth<W>(p.x.rows, plan.parts)) {
+      static StreamLaunch shared;
+      return launch_stream<W>(logprob_stream<T, ENT, RANK, TOP, BWD>, shared, p.x.rows, plan.parts, plan.bytes + besides, s, p, plan);
     }
-    launch(kernel, stream_grid(p.x.rows, smem), kStreamThreads, smem, s, p);
-    return AD_OK;
   }
   auto kernel = logprob_rows<NT, T, ENT, RANK, TOP, BWD>;
   const uint32_t n = NT == 32 ? 1 : row_parts(p.x.rows, bytes), slots = NT == 32 ? 0 : feed_slots(bytes, n, BWD ? kMostFeed : 0);

@@ -109,7 +109,7 @@ typedef unsigned long long Key;   // value, then the complement of the class; 0:
 __device__ __forceinline__ Key key_of(float v, uint32_t c) { return (Key)value_key(v) << 32 | (uint32_t)~c; }
 __device__ __forceinline__ uint32_t key_class(Key k) { return ~(uint32_t)k; }
 
-// ---- threads that work on one row: a warp, or a block of 256 with `red` (10 words of shared memory)
+// ---- threads that work on one row: a warp, or NT threads of a block with `red` (8 bytes for each warp)
 template <int NT> struct Group;
 template <> struct Group<32> {
   uint32_t tid = threadIdx.x & 31;
@@ -125,11 +125,11 @@ template <> struct Group<32> {
   }
 };
 constexpr int kRowThreads = 256, kRowWarps = kRowThreads / 32;
-template <> struct Group<kRowThreads> {
+template <int NT> struct Group {
   uint32_t tid = threadIdx.x;
   Key* red;   // one per warp
   __device__ explicit Group(void* r) : red((Key*)r) {}
-  __device__ void sync() { __syncwarp(); asm volatile("bar.sync 9, 256;" ::: "memory"); }   // these threads alone: a block may have more
+  __device__ void sync() { __syncwarp(); asm volatile("bar.sync 9, %0;" ::"n"(NT) : "memory"); }   // these threads alone: a block may have more
   template <typename V, typename F>
   __device__ V all(V w, F f) {   // of the warps' values, in order
     sync();
@@ -137,14 +137,15 @@ template <> struct Group<kRowThreads> {
     sync();
     V v = *(V*)&red[0];
 #pragma unroll
-    for (int i = 1; i < kRowWarps; ++i) v = f(v, *(V*)&red[i]);
+    for (int i = 1; i < NT / 32; ++i) v = f(v, *(V*)&red[i]);
     return v;
   }
   __device__ float max(float v) { return all(warp_max(v), [](float a, float b) { return fmaxf(a, b); }); }
   __device__ float sum(float v) { return all(warp_sum(v), [](float a, float b) { return a + b; }); }
   __device__ uint32_t sum(uint32_t v) { return all(__reduce_add_sync(0xffffffffu, v), [](uint32_t a, uint32_t b) { return a + b; }); }
-  __device__ Key max(Key v) { return all(Group<32>(nullptr).max(v), [](Key a, Key b) { return a > b ? a : b; }); }
+  __device__ Key max(Key v);
 };
+template <int NT> __device__ Key Group<NT>::max(Key v) { return all(Group<32>(nullptr).max(v), [](Key a, Key b) { return a > b ? a : b; }); }
 
 // ---- 16 bytes of a row
 template <typename T> struct Vec;
@@ -456,98 +457,202 @@ inline uint32_t feed_slots(size_t row_bytes, uint32_t parts, size_t most) {
 }
 constexpr size_t kMostFeed = 96 * 1024;
 
-// ---- many rows: blocks that stay, eight warps that stream and one that does what a row needs besides
-// The streaming warps take one row's vectors after the other's: their copies (cp.async, three batches ahead) go on into the
-// next row, so that loads are in flight while a row is finished.  The ninth warp prepares a row while the one in front of it
-// is streamed (label, lists, masks), and finishes a row while the next one is.
-constexpr uint32_t kStreamThreads = kRowThreads + 32, kStreamBlocks = 3;   // of an SM
-enum { kBarReady = 1, kBarSums = 3, kBarResult = 5, kBarFree = 7 };        // and the row's parity; 9: Group<256>
-__device__ __forceinline__ void bar_arrive(uint32_t id) { __syncwarp(); __threadfence_block(); asm volatile("bar.arrive %0, %1;" ::"r"(id), "n"(kStreamThreads) : "memory"); }
-__device__ __forceinline__ void bar_wait(uint32_t id) { __syncwarp(); asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(kStreamThreads) : "memory"); }
+// ---- many rows: blocks that stay, W warps that stream and one that does what a row needs besides
+// The streaming warps take one row's vectors after the other's: their copies (cp.async) go on into the next rows, so that
+// loads are in flight while a row is finished.  The last warp prepares a row while the one in front of it is streamed (label,
+// lists, masks), and finishes a row while the next one is.
+// Three blocks of an SM with eight streaming warps each.  Backward every row is passed over twice: a row (or a block's part
+// of it) that fits into the ring stays there for the second pass, each batch of which makes room for one of the next row;
+// other rows are copied again, out of the L2.  One block of an SM with sixteen warps and 192 KB of ring was slower (4096 rows
+// of 64 KB: 149 us for 122): nothing else fills the SM while a row's sums are joined.
+enum { kBarReady = 1, kBarSums = 3, kBarResult = 5, kBarFree = 7 };   // and the row's parity; 9: Group<W * 32>
+// The sums of the blocks of a cluster: whole[parity] is this block's, the one in the same place the others'.  All threads of
+// all blocks meet in between, and the next row's meeting comes before whole[parity] is written again.
+template <int W> struct Crew {
+  static constexpr uint32_t kStreaming = W * 32, kThreads = W * 32 + 32, kBlocks = 3;   // blocks of an SM
+  __device__ static void arrive(uint32_t id) {
+    __syncwarp();
+    __threadfence_block();
+    asm volatile("bar.arrive %0, %1;" ::"r"(id), "n"(kThreads) : "memory");
+  }
+  __device__ static void wait(uint32_t id) {
+    __syncwarp();
+    asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(kThreads) : "memory");
+  }
+};
+template <int N> __device__ __forceinline__ void wait_for_copies(uint32_t n) {   // until at most n are on their way
+  if constexpr (N == 0) wait_copies<0>();
+  else if (n >= N) wait_copies<N>();
+  else wait_for_copies<N - 1>(n);
+}
 
-template <typename T, bool TWICE>   // TWICE: every row's vectors are streamed twice in a row
+template <typename T, int W, bool BWD>
 struct Stream {
-  static constexpr uint32_t U = 4, kBatch = U * kRowThreads, kAhead = 3, kBytes = kBatch * 16, kVec = kRowThreads * 16;
+  static constexpr uint32_t U = 4, NS = W * 32, kBatch = U * NS, kBytes = kBatch * 16, kVec = NS * 16, kMostSlots = 6, kForward = 3;
   const T* x;
-  const Rows* at;
-  size_t r, stride;        // of the row that is copied
-  const uint4 *first, *from;   // this thread's first vector of it, and the one to be copied next
-  uint32_t nv, left;       // vectors of the row, and those that are left
-  uint32_t ring, put, get; // this thread's place in shared memory: kAhead batches
-  bool second;
+  const Rows& at;
+  uint32_t r, stride, part, parts;   // the row that is copied; this block's part of it
+  const uint4* from;       // this thread's vector to be copied next
+  uint32_t left;           // vectors of the row that are left
+  uint32_t ring, end, put, get; // this thread's places in shared memory
+  uint32_t held;           // batches that are copied or on their way
+  bool twice, second;      // rows are copied for each of two passes
   __device__ void row() {
-    if (r < at->rows) {
-      const T* p = x + at->offset(r);
-      const Strip<T> b(p, at->C);
-      first = from = (const uint4*)(p + b.head) + threadIdx.x;
-      nv = left = b.nv;
-    } else {
-      left = 0;
+    left = 0;
+    if (r < at.rows) {
+      const T* p = x + at.offset(r);
+      const Strip<T> b(p, at.C, part, parts);
+      from = (const uint4*)(p + b.head) + b.vb + threadIdx.x;
+      left = b.ve - b.vb;
     }
   }
   __device__ __forceinline__ void copy() {
+    if (left == 0) {
+      if (!BWD) commit_copies();   // there are always as many groups behind a batch
+      return;
+    }
     if (left >= kBatch) {
 #pragma unroll
-      for (uint32_t u = 0; u < U; ++u) copy_async(put + u * kVec, from + u * kRowThreads);
+      for (uint32_t u = 0; u < U; ++u) copy_async(put + u * kVec, from + u * NS);
       left -= kBatch;
       from += kBatch;
     } else {
 #pragma unroll
       for (uint32_t u = 0; u < U; ++u)
-        if (u * kRowThreads + threadIdx.x < left) copy_async(put + u * kVec, from + u * kRowThreads);
+        if (u * NS + threadIdx.x < left) copy_async(put + u * kVec, from + u * NS);
       left = 0;
     }
-    put = put == ring + (kAhead - 1) * kBytes ? ring : put + kBytes;
     commit_copies();
+    ++held;
+    put = put + kBytes == end ? ring : put + kBytes;
     if (left == 0) {
-      if (TWICE && !second) {
+      if (twice && !second) {
         second = true;
-        from = first;
-        left = r < at->rows ? nv : 0;
       } else {
         second = false;
         r += stride;
-        row();
       }
+      row();
     }
   }
-  __device__ Stream(const T* x_, const Rows& at_, void* mem)
-      : x(x_), at(&at_), r(blockIdx.x), stride(gridDim.x), first(nullptr), from(nullptr), nv(0), left(0), ring(shared_address(mem) + threadIdx.x * 16), put(ring), get(ring), second(false) {
+  __device__ Stream(const T* x_, const Rows& at_, void* mem, uint32_t slots, bool twice_, uint32_t first, uint32_t stride_, uint32_t part_, uint32_t parts_)
+      : x(x_), at(at_), r(first), stride(stride_), part(part_), parts(parts_), from(nullptr), left(0), ring(shared_address(mem) + threadIdx.x * 16),
+        end(ring + slots * kBytes), put(ring), get(ring), held(0), twice(twice_), second(false) {
     row();
-#pragma unroll
-    for (uint32_t i = 0; i < kAhead; ++i) copy();
+    for (uint32_t i = 0; i < slots; ++i) copy();
   }
-  // f(v0, w, full) for the batches of a row of n vectors: the ones that were copied first.  full: all threads have all of theirs
-  template <typename F> __device__ __forceinline__ void run(uint32_t n, F&& f) {   // f may change w
+  template <typename F> __device__ __forceinline__ void take(uint32_t at, uint32_t v0, uint32_t n, F&& f) {
+    uint4 w[U];
+#pragma unroll
+    for (uint32_t u = 0; u < U; ++u) w[u] = load_shared(at + u * kVec);
+    if (v0 + kBatch <= n) {
+      f(v0, w, true);
+    } else {
+#pragma unroll
+      for (uint32_t u = 0; u < U; ++u)
+        if (v0 + u * NS + threadIdx.x >= n) w[u] = Vec<T>::none();
+      f(v0, w, false);
+    }
+  }
+  // f(v0, w, full) for the batches of a row of n vectors; full: all threads have all of theirs.  f may change w.
+  // The batches that have been there longest, and their room for further ones
+  template <typename F> __device__ __forceinline__ void run(uint32_t n, F&& f) {
     for (uint32_t v0 = 0; v0 < n; v0 += kBatch) {
-      uint4 w[U];
-      wait_copies<kAhead - 1>();
-#pragma unroll
-      for (uint32_t u = 0; u < U; ++u) w[u] = load_shared(get + u * kVec);
-      if (v0 + kBatch <= n) {
-        f(v0, w, true);
-      } else {
-#pragma unroll
-        for (uint32_t u = 0; u < U; ++u)
-          if (v0 + u * kRowThreads + threadIdx.x >= n) w[u] = Vec<T>::none();
-        f(v0, w, false);
-      }
-      get = get == ring + (kAhead - 1) * kBytes ? ring : get + kBytes;
-      copy();   // into the slot that has just been read
+      if (BWD) wait_for_copies<kMostSlots - 1>(held - 1);
+      else wait_copies<kForward - 1>();
+      take(get, v0, n, f);
+      get = get + kBytes == end ? ring : get + kBytes;
+      --held;
+      copy();   // into the slot that has just been read, where there are no more
+    }
+  }
+  // ... which stay where they are, for run() to have them once more (all of a row: not where it is copied twice)
+  template <typename F> __device__ __forceinline__ void look(uint32_t n, F&& f) {
+    uint32_t there = get, newer = held;
+    for (uint32_t v0 = 0; v0 < n; v0 += kBatch) {
+      wait_for_copies<kMostSlots - 1>(--newer);
+      take(there, v0, n, f);
+      there = there + kBytes == end ? ring : there + kBytes;
     }
   }
 };
-// Blocks that are resident together, each with `smem` bytes and up to 8 KB that the kernels have besides
-inline unsigned stream_grid(size_t rows, size_t smem) {
-  const size_t room = 227 * 1024 / (smem + 9 * 1024), n = (room < kStreamBlocks ? (room ? room : 1) : kStreamBlocks) * kNumSMs;
-  return (unsigned)(rows < n ? rows : n);
+// How the blocks of a call are laid out: blocks that share a row (a cluster), batches of a ring, whether rows are copied twice
+struct RingPlan {
+  uint32_t parts, slots, twice;
+  size_t bytes;
+};
+// besides(parts): bytes of shared memory that a block needs for other things.  Backward: the rows that are in hand together
+// have to stay in the L2 for the second pass, or in the ring where they fit.  444 rows of 200 KB did not (1001 of them read 1.7
+// times, 107 us), 222 rows shared by two blocks each do (95); of 400 KB four blocks each (2000 rows: 401 -> 352 us).  Sharing costs
+// a meeting per row: 444 rows of 131 KB take 223 us unshared (4096 of them) and 232 by twos.
+constexpr size_t kRowsInL2 = 60 << 20;
+template <typename T, int W, bool BWD, typename F>
+inline RingPlan ring_plan(uint32_t C, F&& besides) {
+  typedef Stream<T, W, BWD> Str;
+  RingPlan p = {1, Str::kForward, 0, 0};
+  if (BWD) {
+    constexpr size_t blocks = Crew<W>::kBlocks * kNumSMs;
+    while (p.parts < 8 && blocks / p.parts * (size_t)C * sizeof(T) > kRowsInL2) p.parts *= 2;
+    const long long room = (227 * 1024 / (long long)Crew<W>::kBlocks - 9 * 1024 - (long long)besides(p.parts)) / (long long)Str::kBytes;
+    const size_t need = (C / Vec<T>::V / p.parts + 1 + Str::kBatch - 1) / Str::kBatch;
+    p.slots = (uint32_t)(room < 3 ? 3 : room < (long long)Str::kMostSlots ? room : Str::kMostSlots);
+    p.twice = need > p.slots;
+  }
+  p.bytes = (size_t)p.slots * Str::kBytes;
+  return p;
+}
+// What the launches of one kernel share: on which devices (a bit each) its limit is raised, and how many clusters of a size
+// (1, 2, 4, 8 blocks) and of blocks of so much shared memory (KB) the machine holds at a time, as last asked
+struct StreamLaunch {
+  unsigned raised;
+  unsigned long long held[4];   // shared memory << 32 | clusters
+};
+constexpr size_t kMostRing = 218 * 1024;   // dynamic shared memory of the blocks that stay
+template <int W, typename... P, typename... A>
+inline int launch_stream(void (*kernel)(P...), StreamLaunch& l, size_t rows, uint32_t parts, size_t smem, cudaStream_t s, A... args) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (!(__atomic_load_n(&l.raised, __ATOMIC_RELAXED) & (1u << (dev & 31)))) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMostRing) != cudaSuccess) {
+      cudaGetLastError();
+      return AD_ERR_CUDA;
+    }
+    __atomic_fetch_or(&l.raised, 1u << (dev & 31), __ATOMIC_RELAXED);
+  }
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute at[2];
+  cfg.blockDim = Crew<W>::kThreads;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cfg.gridDim = parts;
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = parts;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  // as many clusters as are resident together, which is less than three blocks per SM: a cluster stays within one group of SMs
+  const int i = parts == 1 ? 0 : parts == 2 ? 1 : parts == 4 ? 2 : 3;
+  unsigned long long held = __atomic_load_n(&l.held[i], __ATOMIC_RELAXED);
+  if (held >> 32 != smem) {
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n < 1) {
+      cudaGetLastError();
+      return AD_ERR_CUDA;
+    }
+    held = (unsigned long long)smem << 32 | (unsigned)n;
+    __atomic_store_n(&l.held[i], held, __ATOMIC_RELAXED);
+  }
+  const size_t n = (uint32_t)held;
+  cfg.gridDim = (unsigned)((rows < n ? rows : n) * parts);
+  launch_attr(cfg, at);
+  cudaLaunchKernelEx(&cfg, kernel, P(args)...);   // an error is what launch_status() returns
+  return AD_OK;
 }
 
 // Plain loops over a row in any layout: what the fast pass does not serve
-template <typename G, typename T, bool ENT>
-__device__ void plain_sums(G& g, const T* x, int64_t st, uint32_t C, float cs, RowSums& s, float& E) {
-  const uint32_t NT = sizeof(G) == sizeof(Group<32>) ? 32 : kRowThreads;
-  float m = -INFINITY, S = 0.f;
+template <int NT, typename T, bool ENT>
+__device__ void plain_sums(Group<NT>& g, const T* x, int64_t st, uint32_t C, float cs, RowSums& s, float& E) {
+    float m = -INFINITY, S = 0.f;
   for (uint32_t c = g.tid; c < C; c += NT) m = fmaxf(m, ld_f(x + c * st));
   m = g.max(m);
   if (m == -INFINITY) m = 0.f;
@@ -668,7 +773,7 @@ __device__ void plain_position(const P& x, float cs, RowSums& s, float& E) {
 }
 
 // Rows enough for blocks that stay: at least one for each
-inline bool stream_worth(size_t rows) { return rows >= kStreamBlocks * kNumSMs; }
+template <int W> inline bool stream_worth(size_t rows, uint32_t parts) { return rows * parts >= Crew<W>::kBlocks * kNumSMs && rows < (1u << 31); }
 // Blocks of a row: few rows share the machine, a part at least 8 KB
 inline uint32_t row_parts(size_t rows, size_t row_bytes) {
   uint32_t n = 1;
