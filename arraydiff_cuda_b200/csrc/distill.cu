@@ -708,8 +708,8 @@ __global__ void __launch_bounds__(kPositions) distill_positions(DistillP p) {
     const size_t r0 = blk * kPositions, r = r0 + threadIdx.x;
     const uint32_t n = (uint32_t)(p.x.rows - r0 < kPositions ? p.x.rows - r0 : kPositions);
     if (MODE) {
-      copy_tile<T, TM>((const T*)p.logits, p.x, r0, n, tile);
-      if (BWD && p.accumulate) copy_tile<T, TM>((const T*)p.dlogits, p.g, r0, n, olds);
+      copy_tile<T>(TM == 2, (const T*)p.logits, p.x, r0, n, tile);
+      if (BWD && p.accumulate) copy_tile<T>(TM == 2, (const T*)p.dlogits, p.g, r0, n, olds);
       __syncthreads();
     }
     if (r < p.x.rows) {
@@ -744,7 +744,7 @@ __global__ void __launch_bounds__(kPositions) distill_positions(DistillP p) {
       a.clear();
       for (uint32_t c = 0; c < C; c += 8) {
         float f[8], bm;
-        x.batch(c, f);
+        x.batch(c, C, f);
         if (p.rest) {
           const uint32_t w = bits[(c >> 5) * kPositions] >> (c & 31);
 #pragma unroll
@@ -784,7 +784,7 @@ __global__ void __launch_bounds__(kPositions) distill_positions(DistillP p) {
         // the classes outside of the list; those of the list keep their logits for the loop behind it
         for (uint32_t c = 0; c < C; c += 8) {
           float h[8];
-          x.batch(c, h);
+          x.batch(c, C, h);
           const uint32_t w = bits[(c >> 5) * kPositions] >> (c & 31);
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
@@ -807,7 +807,7 @@ __global__ void __launch_bounds__(kPositions) distill_positions(DistillP p) {
     }
     if (MODE && BWD) {
       __syncthreads();
-      write_tile<T, TM>((T*)p.dlogits, p.g, r0, n, tile);
+      write_tile<T>(TM == 2, (T*)p.dlogits, p.g, r0, n, tile);
     }
     if (MODE) __syncthreads();
   }
@@ -895,7 +895,7 @@ static int launch_distill(const DistillP& p, cudaStream_t s) {
   const size_t mask = p.rest ? (vectors / n + 17) / 16 * 16 : 0;
   if (mode == 0 && (p.x.C > kMostBits || (BWD && p.g.HW == 0))) mode = -1;
   if (mode > 0 && BWD && p.g.step != 1) mode = -1;
-  if (mode == 2 && BWD && p.accumulate && position_mode<T>(p.g, p.dlogits) != 2) mode = 1;
+  if (mode == 2 && BWD && position_mode<T>(p.g, p.dlogits) != 2) mode = 1;
   if (mode == 0) rc = launch_positions<T, 0, BWD>(p, s);
   else if (mode == 1) rc = launch_positions<T, 1, BWD>(p, s);
   else if (mode == 2) rc = launch_positions<T, 2, BWD>(p, s);

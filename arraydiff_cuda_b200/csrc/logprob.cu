@@ -7,33 +7,13 @@
 // Backward: the sums as in the forward pass, then the row once more (out of the L2 or L1) for the gradient.
 #include <cooperative_groups.h>
 
-#include "rows.cuh"
+#include "logprob.cuh"
 
 namespace cg = cooperative_groups;
 
 namespace adk {
 
-struct LogprobP {
-  Rows x, g;
-  const void *logits;
-  void* dlogits;
-  float scale, cs;
-  const uint32_t* label;
-  float *lse, *entropy, *logp;
-  uint32_t *rank, *top_class;
-  float* top_logp;
-  uint32_t top;
-  const float *dlse, *dentropy, *dlogp;
-  int accumulate;
-};
-
-
 // ---------------------------------------------------------------- top classes
-struct TopMem {
-  Key *list, *cand;   // the result, in order; what reaches the bound
-  uint32_t cap;       // room in cand
-  __host__ __device__ static constexpr uint32_t room(uint32_t k) { return 64 + 9 * k; }   // k vectors of equal elements and the single ones fit
-};
 // One warp: places for `mine` things of each lane behind `n` that are there already, which is increased by all of them
 __device__ __forceinline__ uint32_t places(uint32_t mine, uint32_t& n) {
   const uint32_t lane = threadIdx.x & 31;
@@ -123,24 +103,6 @@ __device__ void sort_candidates(const TopMem& t, uint32_t n, uint32_t k) {
   }
   for (uint32_t i = n + lane; i < k; i += 32) t.list[i] = 0;
   __syncwarp();
-}
-
-// One class after the other, from classes [lo, hi): for rows that the bound does not serve
-template <int NT, typename T>
-__device__ void rounds(Group<NT>& g, const TopMem& t, const T* x, int64_t st, uint32_t lo, uint32_t hi, uint32_t k) {
-  Key last = ~0ull;
-  for (uint32_t i = 0; i < k; ++i) {
-    Key best = 0;
-    if (last)
-      for (uint32_t c = lo + g.tid; c < hi; c += NT) {
-        const float v = ld_f(x + c * st);
-        const Key key = v == v ? key_of(v, c) : 0;
-        if (key < last && key > best) best = key;
-      }
-    best = last = g.max(best);
-    if (g.tid == 0) t.list[i] = best;
-  }
-  g.sync();
 }
 
 // One warp: adds the first r elements of a strip that equal v, in order of their classes, to the n candidates
@@ -284,16 +246,6 @@ __device__ void select_top(const TopMem& t, uint32_t k, const uint32_t (&kv)[8],
   rounds<32, T>(g, t, x, 1, b.begin(), b.end(), k);
 }
 
-__device__ __forceinline__ void put_top(const LogprobP& p, const RowSums& s, size_t r, uint32_t at, Key key) {
-  if (p.top_class) p.top_class[r * p.top + at] = key ? key_class(key) : kNoClass;
-  if (p.top_logp) p.top_logp[r * p.top + at] = key ? s.log_p(key_value((uint32_t)(key >> 32)), p.scale) : -INFINITY;
-}
-__device__ __forceinline__ void put_row(const LogprobP& p, const RowSums& s, size_t r, float H, uint32_t l, float xl) {
-  if (p.lse) p.lse[r] = s.lse(p.scale);
-  if (p.entropy) p.entropy[r] = H;
-  if (p.logp) p.logp[r] = l < p.x.C ? s.log_p(xl, p.scale) : 0.f;
-}
-
 // ---------------------------------------------------------------- any layout, any numbers: plain loops over one row
 template <int NT, typename T, bool BWD>
 __device__ void plain_row(Group<NT>& g, const LogprobP& p, size_t r, const TopMem& t) {
@@ -407,28 +359,6 @@ struct Label {
   __device__ bool single_counts(float v, uint32_t c) const { return low ? c > l && v > xl : in_front(v, c, xl, l); }
   __device__ uint32_t rank(uint32_t cnt, uint32_t C) const { return l < C ? cnt + (low ? l : 0u) : kNoClass; }
 };
-// The gradient's factors: e (c0 + c1 u) with e = 2^u is scale p (A - dentropy (log p + H)); dl: what the label's class has besides
-struct Factors {
-  float c0, c1, dl, dh, dz;
-  __device__ void fetch(const LogprobP& p, size_t r, uint32_t l) {
-    dl = p.dlogp && l < p.x.C ? p.dlogp[r] : 0.f;
-    dh = p.dentropy ? p.dentropy[r] : 0.f;
-    dz = p.dlse ? p.dlse[r] : 0.f;
-  }
-  template <bool ENT> __device__ void set(const LogprobP& p, const RowSums& s, float H) {
-    if (!s.some) dl = 0.f;
-    const float A = dz - dl, k = s.some ? p.scale / s.S : 0.f;
-    c1 = ENT ? -k * dh * kLn2 : 0.f;
-    c0 = ENT ? k * (A - dh * (H - kLn2 * s.L)) : k * A;
-    dl *= p.scale;
-  }
-  template <bool ENT> __device__ float grad(float x, float cs, float mc) const {
-    float u = fmaf(x, cs, -mc);
-    if (ENT) u = above_nothing(u);
-    return exp2_fast(u) * (ENT ? fmaf(c1, u, c0) : c0);
-  }
-};
-
 // NT 32: a warp per row, eight vectors per lane and batch.  NT 256: for few rows, a block or a cluster of blocks per row.
 // ENT: the entropy is asked for.  RANK: the label's rank.  TOP: top classes.  BWD: the gradient.
 template <int NT, typename T, bool ENT, bool RANK, bool TOP, bool BWD>
@@ -769,195 +699,6 @@ __global__ void __launch_bounds__(Crew<8>::kThreads, Crew<8>::kBlocks) logprob_s
   if (parts > 1) cluster.sync();   // nobody leaves while its sums are still read
 }
 
-// ---------------------------------------------------------------- a thread per position
-// The first KT classes of those seen so far.  16-bit values: value and class in one word, the list sorted by exchanges.
-template <typename T, int KT> struct Firsts;
-template <int KT> struct Firsts<__nv_bfloat16, KT> {
-  uint32_t k[KT] = {};
-  __device__ void add(float v, uint32_t c) {
-    uint32_t t = v == v ? (value_key(v) & 0xffff0000u) | (0xffffu - c) : 0u;
-#pragma unroll
-    for (int i = 0; i < KT; ++i) {
-      const uint32_t hi = max(k[i], t);
-      t = min(k[i], t);
-      k[i] = hi;
-    }
-  }
-  __device__ Key key(int i) const {
-    if (!k[i]) return 0;
-    const uint32_t v = k[i] & 0xffff0000u;
-    return (Key)(v >> 31 ? v : v | 0xffffu) << 32 | (uint32_t)~(0xffffu - (k[i] & 0xffffu));
-  }
-};
-template <int KT> struct Firsts<float, KT> {   // classes come in ascending order
-  uint32_t k[KT] = {}, c[KT] = {};
-  __device__ void add(float v, uint32_t cls) {
-    uint32_t t = v == v ? value_key(v) : 0u;
-    bool g = false;   // from the place that it takes on, everything moves by one
-#pragma unroll
-    for (int i = 0; i < KT; ++i) {
-      g |= t > k[i];
-      const uint32_t tk = g ? k[i] : t, tc = g ? c[i] : cls;
-      k[i] = g ? t : k[i];
-      c[i] = g ? cls : c[i];
-      t = tk;
-      cls = tc;
-    }
-  }
-  __device__ Key key(int i) const { return k[i] ? (Key)k[i] << 32 | (uint32_t)~c[i] : 0; }
-};
-
-// KT: room for the top classes in registers (0: none, or more than eight: one round over the classes for each)
-template <typename T, int MODE, int KT>
-__global__ void __launch_bounds__(kPositions) logprob_positions(LogprobP p) {
-  grid_dependency();
-  extern __shared__ __align__(16) uint8_t tiles[];
-  T* tile = (T*)tiles;
-  const uint32_t C = p.x.C;
-  const size_t blocks = (p.x.rows + kPositions - 1) / kPositions;
-  for (size_t blk = blockIdx.x; blk < blocks; blk += gridDim.x) {
-    const size_t r0 = blk * kPositions, r = r0 + threadIdx.x;
-    if (MODE) {
-      copy_tile<T, MODE>((const T*)p.logits, p.x, r0, (uint32_t)(p.x.rows - r0 < kPositions ? p.x.rows - r0 : kPositions), tile);
-      __syncthreads();
-    }
-    if (r < p.x.rows) {
-      const Position<T, MODE> x = {MODE ? tile + threadIdx.x * tile_pitch<T, MODE>(C) : (const T*)p.logits + p.x.offset(r), p.x.step, C};
-      const uint32_t l = p.label ? p.label[r] : kNoClass;
-      const float xl = l < C ? x.get(l) : 0.f;
-      Part a;
-      a.clear();
-      Firsts<T, KT ? KT : 1> top;
-      for (uint32_t c = 0; c < C; c += 8) {
-        float f[8], bm;
-        x.batch(c, f);
-        bm = fmaxf(fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3])), fmaxf(fmaxf(f[4], f[5]), fmaxf(f[6], f[7])));
-        a.reach<true>(bm, p.cs);
-        float S[2] = {0.f, 0.f}, E[2] = {0.f, 0.f};
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float u = above_nothing(fmaf(f[i], p.cs, -a.mc)), e = exp2_fast(u);
-          S[i & 1] += e;
-          E[i & 1] = fmaf(e, u, E[i & 1]);
-        }
-        a.S += S[0] + S[1];
-        a.E += E[0] + E[1];
-        if (p.rank) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) a.cnt += c + i < C && in_front(f[i], c + i, xl, l);
-        }
-        if (KT) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (c + i < C) top.add(f[i], c + i);
-        }
-      }
-      RowSums s;
-      if (a.strange(p.cs)) plain_position<true>(x, p.cs, s, a.E);
-      else {
-        a.refer<true>(Part::reference(a.m, p.cs));
-        s.set(a.m, a.mc, a.S, p.cs);
-      }
-      put_row(p, s, r, s.some ? kLn2 * (s.L - a.E / s.S) : 0.f, l, xl);
-      if (p.rank) p.rank[r] = l < C ? a.cnt : kNoClass;
-      if (KT) {
-#pragma unroll
-        for (int i = 0; i < KT; ++i)
-          if ((uint32_t)i < p.top) put_top(p, s, r, i, top.key(i));
-      } else {
-        Key last = ~0ull;
-        for (uint32_t i = 0; i < p.top; ++i) {
-          Key best = 0;
-          if (last)
-            for (uint32_t c = 0; c < C; ++c) {
-              const float v = x.get(c);
-              const Key key = v == v ? key_of(v, c) : 0;
-              if (key < last && key > best) best = key;
-            }
-          put_top(p, s, r, i, best);
-          last = best;
-        }
-      }
-    }
-    if (MODE) __syncthreads();
-  }
-}
-
-template <typename T, int MODE, bool ENT>
-__global__ void __launch_bounds__(kPositions) logprob_positions_bwd(LogprobP p) {
-  grid_dependency();
-  extern __shared__ __align__(16) uint8_t tiles[];
-  const uint32_t C = p.x.C;
-  T *tile = (T*)tiles, *olds = tile + kPositions * tile_pitch<T, MODE ? MODE : 1>(C);   // what the gradient is added to
-  const size_t blocks = (p.x.rows + kPositions - 1) / kPositions;
-  for (size_t blk = blockIdx.x; blk < blocks; blk += gridDim.x) {
-    const size_t r0 = blk * kPositions, r = r0 + threadIdx.x;
-    const uint32_t n = (uint32_t)(p.x.rows - r0 < kPositions ? p.x.rows - r0 : kPositions);
-    if (MODE) {
-      copy_tile<T, MODE>((const T*)p.logits, p.x, r0, n, tile);
-      if (p.accumulate) copy_tile<T, MODE>((const T*)p.dlogits, p.g, r0, n, olds);
-      __syncthreads();
-    }
-    if (r < p.x.rows) {
-      const uint32_t at = threadIdx.x * tile_pitch<T, MODE ? MODE : 1>(C);
-      const Position<T, MODE> x = {MODE ? tile + at : (const T*)p.logits + p.x.offset(r), p.x.step, C};
-      const Position<T, MODE> o = {MODE ? tile + at : (T*)p.dlogits + p.g.offset(r), p.g.step, C};
-      const Position<T, MODE> old = {MODE ? olds + at : (T*)p.dlogits + p.g.offset(r), p.g.step, C};
-      const uint32_t l = p.label ? p.label[r] : kNoClass;
-      const float xl = l < C ? x.get(l) : 0.f;
-      Part a;
-      a.clear();
-      for (uint32_t c = 0; c < C; c += 8) {
-        float f[8], bm;
-        x.batch(c, f);
-        bm = fmaxf(fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3])), fmaxf(fmaxf(f[4], f[5]), fmaxf(f[6], f[7])));
-        a.reach<ENT>(bm, p.cs);
-        float S[2] = {0.f, 0.f}, E[2] = {0.f, 0.f};
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          float u = fmaf(f[i], p.cs, -a.mc);
-          if (ENT) u = above_nothing(u);
-          const float e = exp2_fast(u);
-          S[i & 1] += e;
-          if (ENT) E[i & 1] = fmaf(e, u, E[i & 1]);
-        }
-        a.S += S[0] + S[1];
-        if (ENT) a.E += E[0] + E[1];
-      }
-      RowSums s;
-      const bool strange = a.strange(p.cs);
-      if (strange) plain_position<ENT>(x, p.cs, s, a.E);
-      else {
-        a.refer<ENT>(Part::reference(a.m, p.cs));
-        s.set(a.m, a.mc, a.S, p.cs);
-      }
-      const float H = s.some ? kLn2 * (s.L - a.E / s.S) : 0.f;
-      put_row(p, s, r, H, l, xl);
-      const float dl = p.dlogp && l < C && s.some ? p.dlogp[r] : 0.f, dh = p.dentropy ? p.dentropy[r] : 0.f;
-      const float A = (p.dlse ? p.dlse[r] : 0.f) - dl, k = s.some ? p.scale / s.S : 0.f;
-      const float c1 = ENT ? -k * dh * kLn2 : 0.f, c0 = ENT ? k * (A - dh * (H - kLn2 * s.L)) : k * A;
-      const float mc = s.mc;
-      for (uint32_t c = 0; c < C; c += 8) {
-        float f[8];
-        x.batch(c, f);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          float u = strange ? (f[i] - s.m) * p.cs : fmaf(f[i], p.cs, -mc);
-          if (ENT) u = above_nothing(u);
-          f[i] = exp2_fast(u) * (ENT ? fmaf(c1, u, c0) : c0);
-          if (c + i == l) f[i] += p.scale * dl;
-          if (c + i < C) o.set(c + i, p.accumulate ? f[i] + old.get(c + i) : f[i]);
-        }
-      }
-    }
-    if (MODE) {
-      __syncthreads();
-      write_tile<T, MODE>((T*)p.dlogits, p.g, r0, n, tile);
-      __syncthreads();
-    }
-  }
-}
-
 static int logprob_args(const ad_logprob_args* a, bool bwd, LogprobP& p) {
   if (!a) return AD_ERR_BAD_ARG;
   p = {};
@@ -1047,39 +788,10 @@ static int launch_bwd(const LogprobP& p, cudaStream_t s) {
   return p.entropy || p.dentropy ? launch_rows<NT, T, true, false, false, true>(p, s) : launch_rows<NT, T, false, false, false, true>(p, s);
 }
 
-template <typename P>
-static int launch_positions(void (*kernel)(P), const P& p, size_t smem, cudaStream_t s) {
-  // the limit belongs to the function: the most that it takes
-  if (smem > 48 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * (kFewClasses * 4 + 16) * kPositions) != cudaSuccess) {
-    cudaGetLastError();
-    return AD_ERR_CUDA;
-  }
-  launch(kernel, position_blocks(p.x.rows), kPositions, smem, s, p);
-  return AD_OK;
-}
-template <typename T, int MODE>
-static int positions_fwd(const LogprobP& p, cudaStream_t s) {
-  const size_t smem = tile_bytes<T, MODE>(p.x.C);
-  if (p.top == 0 || p.top > 8) return launch_positions(logprob_positions<T, MODE, 0>, p, smem, s);
-  if (p.top == 1) return launch_positions(logprob_positions<T, MODE, 1>, p, smem, s);
-  if (p.top <= 3) return launch_positions(logprob_positions<T, MODE, 3>, p, smem, s);
-  return launch_positions(logprob_positions<T, MODE, 8>, p, smem, s);
-}
-template <typename T, int MODE>
-static int positions_bwd(const LogprobP& p, cudaStream_t s) {
-  const size_t smem = tile_bytes<T, MODE>(p.x.C) * (p.accumulate ? 2 : 1);
-  return p.entropy || p.dentropy ? launch_positions(logprob_positions_bwd<T, MODE, true>, p, smem, s) : launch_positions(logprob_positions_bwd<T, MODE, false>, p, smem, s);
-}
-
 template <typename T, bool BWD>
 static int launch_logprob(const LogprobP& p, cudaStream_t s) {
-  int rc, mode = position_mode<T>(p.x, p.logits);
-  if (BWD && mode == 0 && p.g.HW == 0) mode = -1;   // the gradient of an image of one position, packed
-  if (BWD && mode == 2 && p.accumulate && position_mode<T>(p.g, p.dlogits) != 2) mode = 1;
-  if (mode > 0 && BWD && p.g.step != 1) mode = -1;
-  if (mode == 0) rc = BWD ? positions_bwd<T, 0>(p, s) : positions_fwd<T, 0>(p, s);
-  else if (mode == 1) rc = BWD ? positions_bwd<T, 1>(p, s) : positions_fwd<T, 1>(p, s);
-  else if (mode == 2) rc = BWD ? positions_bwd<T, 2>(p, s) : positions_fwd<T, 2>(p, s);
+  int rc = BWD ? logprob_positions_bwd<T>(p, s) : logprob_positions<T>(p, s);
+  if (rc != AD_ERR_UNSUPPORTED) {}
   else if (p.x.step != 1 || (BWD && p.g.step != 1)) rc = launch_any<T, BWD>(p, s);
   else if (p.x.C * sizeof(T) <= 8192) rc = BWD ? launch_bwd<32, T>(p, s) : launch_fwd<32, T>(p, s);
   else rc = BWD ? launch_bwd<256, T>(p, s) : launch_fwd<256, T>(p, s);

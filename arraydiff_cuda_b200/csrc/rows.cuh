@@ -679,65 +679,129 @@ struct Position {
   int64_t step;   // MODE 0
   uint32_t C;
   __device__ float get(uint32_t c) const { return ld_f(MODE == 0 ? x + c * step : x + c); }
-  // classes [c, c + 8), -inf behind the last one
-  __device__ void batch(uint32_t c, float (&f)[8]) const {
+  // classes [c, c + 8), -inf from `hi` on (MODE 2: hi is C, a multiple of the vector)
+  __device__ void batch(uint32_t c, uint32_t hi, float (&f)[8]) const {
     constexpr uint32_t V = Vec<T>::V;
     if (MODE == 2) {
       Vec<T>::unpack(*(const uint4*)(x + c), f);
-      if (V == 4) Vec<T>::unpack(c + 4 < C ? *(const uint4*)(x + c + 4) : Vec<T>::none(), f + 8 - V);
-    } else if (c + 8 <= C) {
+      if (V == 4) Vec<T>::unpack(c + 4 < hi ? *(const uint4*)(x + c + 4) : Vec<T>::none(), f + 8 - V);
+    } else if (c + 8 <= hi) {
 #pragma unroll
       for (uint32_t i = 0; i < 8; ++i) f[i] = get(c + i);
     } else {
 #pragma unroll
-      for (uint32_t i = 0; i < 8; ++i) f[i] = c + i < C ? get(c + i) : -INFINITY;
+      for (uint32_t i = 0; i < 8; ++i) f[i] = c + i < hi ? get(c + i) : -INFINITY;
     }
   }
   __device__ void set(uint32_t c, float v) const { st_f(const_cast<T*>(MODE == 0 ? x + c * step : x + c), v); }
 };
 constexpr uint32_t kPositions = 128;         // of a block
 constexpr uint32_t kFewClasses = 64;         // of rows in shared memory
+constexpr uint32_t kSharedPlanes = 16;       // classes in planes from which four warps share them
 // MODE 1, 2: elements from one row to the next in shared memory
 template <typename T, int MODE> __host__ __device__ inline uint32_t tile_pitch(uint32_t C) { return MODE == 2 ? (C / Vec<T>::V | 1u) * Vec<T>::V : C; }
-template <typename T, int MODE>
-__device__ __forceinline__ void copy_tile(const T* from, const Rows& g, size_t r0, uint32_t n, T* tile) {
+template <typename T>
+__device__ __forceinline__ void copy_tile(bool vec, const T* from, const Rows& g, size_t r0, uint32_t n, T* tile) {
   constexpr uint32_t V = Vec<T>::V;
   const T* src = from + r0 * (size_t)g.pitch;
-  auto async = [](void* d, const void* s) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(d)), "l"(s) : "memory");
-  };
-  if (MODE == 2) {
+  if (vec) {
     const uint32_t q = g.C / V, to = tile_pitch<T, 2>(g.C);
     for (uint32_t i = threadIdx.x; i < n * q; i += kPositions) {
       const uint32_t row = i / q, col = i - row * q;
-      async(tile + row * to + col * V, src + row * (size_t)g.pitch + col * V);
+      copy_async(shared_address(tile + row * to + col * V), src + row * (size_t)g.pitch + col * V);
     }
   } else if (g.pitch == (int64_t)g.C) {
     const uint32_t e = n * g.C, v = ((uintptr_t)src & 15u) == 0 ? e / V : 0;
-    for (uint32_t i = threadIdx.x; i < v; i += kPositions) async(tile + i * V, src + i * V);
+    for (uint32_t i = threadIdx.x; i < v; i += kPositions) copy_async(shared_address(tile + i * V), src + i * V);
     for (uint32_t i = v * V + threadIdx.x; i < e; i += kPositions) tile[i] = src[i];
   } else {
     for (uint32_t i = threadIdx.x; i < n * g.C; i += kPositions) tile[i] = src[i / g.C * (size_t)g.pitch + i % g.C];
   }
-  asm volatile("cp.async.wait_all;" ::: "memory");
+  commit_copies();
+  wait_copies<0>();
 }
-template <typename T, int MODE>
-__device__ __forceinline__ void write_tile(T* to, const Rows& g, size_t r0, uint32_t n, const T* tile) {
+template <typename T>
+__device__ __forceinline__ void write_tile(bool vec, T* to, const Rows& g, size_t r0, uint32_t n, const T* tile) {
   constexpr uint32_t V = Vec<T>::V;
   T* dst = to + r0 * (size_t)g.pitch;
-  const uint32_t tp = tile_pitch<T, MODE>(g.C);
-  if (MODE == 2 && ((uintptr_t)dst & 15u) == 0 && g.pitch % V == 0) {
-    const uint32_t q = g.C / V;
+  if (vec) {
+    const uint32_t q = g.C / V, tp = tile_pitch<T, 2>(g.C);
     for (uint32_t i = threadIdx.x; i < n * q; i += kPositions) {
       const uint32_t row = i / q, col = i - row * q;
       *(uint4*)(dst + row * (size_t)g.pitch + col * V) = *(const uint4*)(tile + row * tp + col * V);
     }
-  } else if (MODE == 1 && g.pitch == (int64_t)g.C) {
+  } else if (g.pitch == (int64_t)g.C) {
     const uint32_t e = n * g.C, v = ((uintptr_t)dst & 15u) == 0 ? e / V : 0;
     for (uint32_t i = threadIdx.x; i < v; i += kPositions) ((uint4*)dst)[i] = ((const uint4*)tile)[i];
     for (uint32_t i = v * V + threadIdx.x; i < e; i += kPositions) dst[i] = tile[i];
   } else {
-    for (uint32_t i = threadIdx.x; i < n * g.C; i += kPositions) dst[i / g.C * (size_t)g.pitch + i % g.C] = tile[i / g.C * tp + i % g.C];
+    for (uint32_t i = threadIdx.x; i < n * g.C; i += kPositions) dst[i / g.C * (size_t)g.pitch + i % g.C] = tile[i];
+  }
+}
+// A row of up to CM classes (C rounded up to a multiple of 4) in registers, -inf behind the last
+template <typename T, int CM>
+__device__ __forceinline__ void load_few(const T* x, uint32_t C, bool vec, float (&v)[CM]) {
+  constexpr int V = Vec<T>::V;
+  if constexpr (CM % V == 0) {
+    if (vec) {
+#pragma unroll
+      for (int c = 0; c < CM; c += V) {
+        float f[V];
+        Vec<T>::unpack(*(const uint4*)(x + c), f);
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[c + i] = f[i];
+      }
+      return;
+    }
+  }
+#pragma unroll
+  for (uint32_t c = 0; c < CM; ++c) v[c] = c + 4 < CM || c < C ? ld_f(x + c) : -INFINITY;
+}
+template <typename T, int CM>
+__device__ __forceinline__ void store_few(T* x, uint32_t C, bool vec, const float (&v)[CM]) {
+  constexpr int V = Vec<T>::V;
+  if constexpr (CM % V == 0) {
+    if (vec) {
+#pragma unroll
+      for (int c = 0; c < CM; c += V) {
+        float f[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) f[i] = v[c + i];
+        *(uint4*)(x + c) = Vec<T>::pack(f);
+      }
+      return;
+    }
+  }
+#pragma unroll
+  for (uint32_t c = 0; c < CM; ++c)
+    if (c + 4 < CM || c < C) st_f(x + c, v[c]);
+}
+template <bool ENT, int CM>
+__device__ __forceinline__ void sum_few(Part& a, const float (&v)[CM], float cs) {
+  a.clear();
+#pragma unroll
+  for (int c = 0; c < CM; ++c) a.m = fmaxf(a.m, v[c]);
+  a.mc = Part::reference(a.m, cs);
+  const F2 cs2 = pair(cs, cs), mc2 = pair(-a.mc, -a.mc);
+  F2 S[2] = {0, 0}, E[2] = {0, 0};
+#pragma unroll
+  for (int c = 0; c < CM; c += 2) {
+    F2 z = fma2(pair(v[c], v[c + 1]), cs2, mc2);
+    float2 q = halves(z);
+    if (ENT) {
+      q.x = above_nothing(q.x);
+      q.y = above_nothing(q.y);
+      z = pair(q.x, q.y);
+    }
+    const F2 e = pair(exp2_fast(q.x), exp2_fast(q.y));
+    S[c / 2 & 1] = add2(S[c / 2 & 1], e);
+    if (ENT) E[c / 2 & 1] = fma2(e, z, E[c / 2 & 1]);
+  }
+  const float2 s = halves(add2(S[0], S[1]));
+  a.S = s.x + s.y;
+  if (ENT) {
+    const float2 e = halves(add2(E[0], E[1]));
+    a.E = e.x + e.y;
   }
 }
 // Bytes of such a tile, a multiple of 16
@@ -751,13 +815,13 @@ inline int position_mode(const Rows& g, const void* x) {
   if (g.step != 1 || g.C > kFewClasses) return -1;
   return g.C % Vec<T>::V == 0 && g.pitch % Vec<T>::V == 0 && aligned_to(x, 16) ? 2 : 1;
 }
-inline unsigned position_blocks(size_t rows) {
-  const size_t n = (rows + kPositions - 1) / kPositions;
+inline unsigned position_blocks(size_t rows, uint32_t places = kPositions) {
+  const size_t n = (rows + places - 1) / places;
   return (unsigned)(n < (1u << 20) ? n : (1u << 20));
 }
 // One position by plain loops over x_c - m
 template <bool ENT, typename P>
-__device__ void plain_position(const P& x, float cs, RowSums& s, float& E) {
+__device__ void plain_position_sums(const P& x, float cs, RowSums& s, float& E) {
   float m = -INFINITY, S = 0.f;
   for (uint32_t c = 0; c < x.C; ++c) m = fmaxf(m, x.get(c));
   if (m == -INFINITY) m = 0.f;
