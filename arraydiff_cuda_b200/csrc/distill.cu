@@ -7,26 +7,11 @@
 // however little of the row it is, and the row's sum is theirs and that of the list, each class of it once.
 #include <cooperative_groups.h>
 
-#include "rows.cuh"
+#include "distill.cuh"
 
 namespace cg = cooperative_groups;
 
 namespace adk {
-
-struct DistillP {
-  Rows x, g;
-  const void* logits;
-  void* dlogits;
-  float scale, cs;
-  uint32_t top;
-  int rest;
-  const uint32_t* top_class;
-  const float *top_logit, *top_lse;
-  float ts;              // top_scale * log2(e)
-  float* loss;
-  const float* dloss;
-  int accumulate;
-};
 
 constexpr size_t kMostMask = 120 * 1024;   // bytes of mask in shared memory
 
@@ -37,50 +22,6 @@ struct __align__(16) List {
   uint8_t first[kMostTop];          // no earlier entry has the class
   bool twice;                       // some class stands twice
 };
-
-// What is known of a row when its list and its classes have been summed
-struct Distilled {
-  float S, mt, L;      // the row's sum against mt, a maximum, and its log2
-  float off, offt;     // roundings of the references of the pass's sum and of S
-  float qr, Q;         // q_r, sum q + q_r
-  float out, rS;       // gradient outside of the list: dloss * scale * out * 2^u with u as in the pass; p of a listed class: 2^((x - mt) cs) rS
-  bool some;
-  __device__ float term(float q, float a, float x, float scale) const { return q != 0.f ? q * (kLn2 * (a + L + offt) - (x - mt) * scale) : 0.f; }
-};
-// R: the pass's sum, of all classes or (rest) of those outside of the list, against m * cs + off.  K: the list's share of the
-// row (rest), each class once, against mk.
-__device__ __forceinline__ Distilled row_sums(const DistillP& p, float m, float off, float R, float mk, float K, float Q, float& rest_loss) {
-  Distilled d;
-  float to = 0.f;
-  if (m == -INFINITY) m = 0.f;
-  d.S = R;
-  d.mt = m;
-  bool by_list = false;
-  if (K != 0.f) {
-    if (R == 0.f) {
-      d.S = K;
-      by_list = true;
-    } else if (m >= mk) {
-      d.S = R + K * exp2_fast((mk - m) * p.cs - off);
-    } else {
-      to = (mk - m) * p.cs - off;
-      d.S = K + R * exp2_fast(-to);
-      by_list = true;
-    }
-    if (by_list) d.mt = mk;
-  }
-  d.off = off;
-  d.offt = by_list ? 0.f : off;
-  d.some = d.S != 0.f;
-  d.L = d.some ? log2f(d.S) : 0.f;
-  d.qr = p.rest && R != 0.f ? fmaxf(1.f - Q, 0.f) : 0.f;
-  d.Q = Q + d.qr;
-  d.rS = d.some ? 1.f / d.S : 0.f;
-  d.out = d.some ? d.Q * d.rS * exp2_fast(-to) - (d.qr > 0.f ? d.qr / R : 0.f) : 0.f;
-  d.rS *= exp2_fast(-d.offt);
-  rest_loss = d.qr > 0.f ? d.qr * (kLn2 * (log2f(d.qr) - log2f(R) + d.L + (d.offt - off)) + (d.mt - m) * p.scale) : 0.f;
-  return d;
-}
 
 // One warp: the teacher's weights, the list's share of the row, and the loss
 __device__ __forceinline__ Distilled distill_row(const DistillP& p, size_t r, List& list, float m, float off, float R, float& loss) {
@@ -690,129 +631,6 @@ __global__ void __launch_bounds__(Crew<8>::kThreads, Crew<8>::kBlocks) distill_s
   if (parts > 1) cluster.sync();   // nobody leaves while its sums are still read
 }
 
-// ---------------------------------------------------------------- a thread per position
-// Rows of few classes in shared memory (MODE 1, 2), or classes in planes (MODE 0).  A bit per class tells which are listed.
-constexpr uint32_t kMostBits = 4096;   // classes of such a mask: a word of 32 for each thread and 32 classes
-
-template <typename T, int MODE, bool BWD>
-__global__ void __launch_bounds__(kPositions) distill_positions(DistillP p) {
-  grid_dependency();
-  extern __shared__ __align__(16) uint8_t tiles[];
-  const uint32_t C = p.x.C, k = p.top, words = (C + 31) / 32;
-  constexpr int TM = MODE ? MODE : 1;
-  const uint32_t tile_elems = MODE ? kPositions * tile_pitch<T, TM>(C) : 0;
-  uint32_t* bits = (uint32_t*)tiles + threadIdx.x;   // word w at [w * kPositions]
-  T *tile = (T*)(tiles + (size_t)words * kPositions * 4), *olds = tile + tile_elems;
-  const size_t blocks = (p.x.rows + kPositions - 1) / kPositions;
-  for (size_t blk = blockIdx.x; blk < blocks; blk += gridDim.x) {
-    const size_t r0 = blk * kPositions, r = r0 + threadIdx.x;
-    const uint32_t n = (uint32_t)(p.x.rows - r0 < kPositions ? p.x.rows - r0 : kPositions);
-    if (MODE) {
-      copy_tile<T>(TM == 2, (const T*)p.logits, p.x, r0, n, tile);
-      if (BWD && p.accumulate) copy_tile<T>(TM == 2, (const T*)p.dlogits, p.g, r0, n, olds);
-      __syncthreads();
-    }
-    if (r < p.x.rows) {
-      const uint32_t at = threadIdx.x * tile_pitch<T, TM>(C);
-      const Position<T, MODE> x = {MODE ? tile + at : (const T*)p.logits + p.x.offset(r), p.x.step, C};
-      const uint32_t* cls = p.top_class + r * k;
-      const float* t = p.top_logit + r * k;
-      auto listed = [&](uint32_t c) { return bits[(c >> 5) * kPositions] >> (c & 31) & 1u; };
-      // the list: its weights' sum, and a bit for each class
-      for (uint32_t w = 0; w < words; ++w) bits[w * kPositions] = 0;
-      float am = -INFINITY, shift, Q = 0.f, mk = -INFINITY, K = 0.f;
-      for (uint32_t j = 0; j < k; ++j)
-        if (cls[j] < C) {
-          bits[(cls[j] >> 5) * kPositions] |= 1u << (cls[j] & 31);
-          am = fmaxf(am, t[j] * p.ts);
-          mk = fmaxf(mk, x.get(cls[j]));
-        }
-      if (mk == -INFINITY) mk = 0.f;
-      if (p.rest) {
-        shift = p.top_lse ? (float)(p.top_lse[r] * kLog2e) : 0.f;
-      } else {
-        if (am == -INFINITY) am = 0.f;
-        float z = 0.f;
-        for (uint32_t j = 0; j < k; ++j)
-          if (cls[j] < C) z += exp2f(t[j] * p.ts - am);
-        shift = z != 0.f ? am + log2f(z) : 0.f;
-      }
-      for (uint32_t j = 0; j < k; ++j)
-        if (cls[j] < C) Q += exp2f(t[j] * p.ts - shift);
-      // the classes: with rest those outside of the list, and the list's, each once
-      Part a;
-      a.clear();
-      for (uint32_t c = 0; c < C; c += 8) {
-        float f[8], bm;
-        x.batch(c, C, f);
-        if (p.rest) {
-          const uint32_t w = bits[(c >> 5) * kPositions] >> (c & 31);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) f[i] = w >> i & 1u ? -INFINITY : f[i];
-        }
-        bm = fmaxf(fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3])), fmaxf(fmaxf(f[4], f[5]), fmaxf(f[6], f[7])));
-        a.reach<false>(bm, p.cs);
-        float S[2] = {0.f, 0.f};
-#pragma unroll
-        for (int i = 0; i < 8; ++i) S[i & 1] += exp2_fast(fmaf(f[i], p.cs, -a.mc));
-        a.S += S[0] + S[1];
-      }
-      const bool strange = a.strange(p.cs);
-      a.refer<false>(Part::reference(a.m, p.cs));
-      float off = a.m == -INFINITY ? 0.f : fmaf(-a.m, p.cs, a.mc);
-      if (strange) {
-        off = a.S = 0.f;
-        if (a.m == -INFINITY) a.m = 0.f;
-        for (uint32_t c = 0; c < C; ++c)
-          if (!p.rest || !listed(c)) a.S += exp2_fast((x.get(c) - a.m) * p.cs);
-      }
-      if (p.rest)
-        for (uint32_t c0 = 0; c0 < C; c0 += 32)
-          for (uint32_t w = bits[(c0 >> 5) * kPositions]; w; w &= w - 1) K += exp2_fast((x.get(c0 + __ffs(w) - 1) - mk) * p.cs);
-      float loss;
-      const Distilled d = row_sums(p, a.m, off, a.S, mk, K, Q, loss);
-      for (uint32_t j = 0; j < k; ++j)
-        if (cls[j] < C) {
-          const float v = t[j] * p.ts - shift;
-          loss += d.term(exp2f(v), v, x.get(cls[j]), p.scale);
-        }
-      if (p.loss) p.loss[r] = d.some ? loss + 0.f * d.L : 0.f;
-      if constexpr (BWD) {
-        const Position<T, MODE> o = {MODE ? tile + at : (T*)p.dlogits + p.g.offset(r), p.g.step, C};
-        const Position<T, MODE> old = {MODE ? olds + at : (T*)p.dlogits + p.g.offset(r), p.g.step, C};
-        const float f = p.dloss[r] * p.scale, coef = f * d.out;
-        // the classes outside of the list; those of the list keep their logits for the loop behind it
-        for (uint32_t c = 0; c < C; c += 8) {
-          float h[8];
-          x.batch(c, C, h);
-          const uint32_t w = bits[(c >> 5) * kPositions] >> (c & 31);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float u = strange ? (h[i] - a.m) * p.cs : fmaf(h[i], p.cs, -a.mc);
-            h[i] = coef * exp2_fast(u);
-            if (c + i < C && !(w >> i & 1u)) o.set(c + i, p.accumulate ? h[i] + old.get(c + i) : h[i]);
-          }
-        }
-        for (uint32_t j = 0; j < k; ++j) {
-          const uint32_t c = cls[j];
-          if (c >= C || !listed(c)) continue;   // no class, or written already
-          bits[(c >> 5) * kPositions] &= ~(1u << (c & 31));
-          float sum = 0.f;
-          for (uint32_t i = j; i < k; ++i)
-            if (cls[i] == c) sum += exp2f(t[i] * p.ts - shift);
-          const float v = d.some ? f * (exp2_fast((x.get(c) - d.mt) * p.cs) * d.rS * d.Q - sum) : 0.f;
-          o.set(c, p.accumulate ? v + old.get(c) : v);
-        }
-      }
-    }
-    if (MODE && BWD) {
-      __syncthreads();
-      write_tile<T>(TM == 2, (T*)p.dlogits, p.g, r0, n, tile);
-    }
-    if (MODE) __syncthreads();
-  }
-}
-
 static int distill_args(const ad_distill_args* a, bool bwd, DistillP& p) {
   if (!a) return AD_ERR_BAD_ARG;
   p = {};
@@ -873,33 +691,15 @@ static int launch_rows(const DistillP& p, uint32_t n, size_t mask, cudaStream_t 
   return AD_OK;
 }
 
-template <typename T, int MODE, bool BWD>
-static int launch_positions(const DistillP& p, cudaStream_t s) {
-  auto kernel = distill_positions<T, MODE, BWD>;
-  const size_t smem = (p.x.C + 31) / 32 * kPositions * 4 + tile_bytes<T, MODE>(p.x.C) * (BWD && p.accumulate ? 2 : 1);
-  // the limit belongs to the function: the most that it takes
-  constexpr int most = kPositions * (MODE ? 2 * 4 + 2 * (kFewClasses * 4 + 16) : kMostBits / 8);
-  if (smem > 48 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most) != cudaSuccess) {
-    cudaGetLastError();
-    return AD_ERR_CUDA;
-  }
-  launch(kernel, position_blocks(p.x.rows), kPositions, smem, s, p);
-  return AD_OK;
-}
-
 template <typename T, bool BWD>
 static int launch_distill(const DistillP& p, cudaStream_t s) {
-  int rc = AD_OK, mode = position_mode<T>(p.x, p.logits);
   const size_t vectors = p.x.C / Vec<T>::V;
   const uint32_t n = row_parts(p.x.rows, (size_t)p.x.C * sizeof(T));
   const size_t mask = p.rest ? (vectors / n + 17) / 16 * 16 : 0;
-  if (mode == 0 && (p.x.C > kMostBits || (BWD && p.g.HW == 0))) mode = -1;
-  if (mode > 0 && BWD && p.g.step != 1) mode = -1;
-  if (mode == 2 && BWD && position_mode<T>(p.g, p.dlogits) != 2) mode = 1;
-  if (mode == 0) rc = launch_positions<T, 0, BWD>(p, s);
-  else if (mode == 1) rc = launch_positions<T, 1, BWD>(p, s);
-  else if (mode == 2) rc = launch_positions<T, 2, BWD>(p, s);
+  int rc = distill_positions<T, BWD>(p, s);
+  if (rc != AD_ERR_UNSUPPORTED) {}
   else if (p.x.step != 1 || (BWD && p.g.step != 1) || mask > kMostMask) {
+    rc = AD_OK;
     launch(distill_any<T, BWD>, grid_for(p.x.rows, 8), 256, 0, s, p);
   } else if (p.x.C * sizeof(T) <= 8192) {
     const size_t all = p.rest ? kRowWarps * ((vectors + 15) / 16 * 16) : 0;

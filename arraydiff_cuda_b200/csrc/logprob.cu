@@ -256,7 +256,7 @@ __device__ void plain_row(Group<NT>& g, const LogprobP& p, size_t r, const TopMe
   RowSums s;
   float E;
   plain_sums<NT, T, true>(g, x, st, C, p.cs, s, E);
-  const float H = s.some ? kLn2 * (s.L - E / s.S) : 0.f;
+  const float H = s.entropy(E);
   if (g.tid == 0) put_row(p, s, r, H, l, xl);
   if constexpr (!BWD) {
     if (p.rank) {
@@ -424,7 +424,7 @@ __global__ void __launch_bounds__(256) logprob_rows(LogprobP p, uint32_t slots) 
     }
     RowSums s;
     s.set(a.m, a.mc, a.S, p.cs);
-    const float H = s.some ? kLn2 * (s.L - a.E / s.S) : 0.f;
+    const float H = s.entropy(a.E);
     if (g.tid == 0 && part == 0) {
       put_row(p, s, r, H, label.l, label.xl);
       if (RANK) p.rank[r] = label.rank(a.cnt, C);
@@ -661,7 +661,7 @@ __global__ void __launch_bounds__(Crew<8>::kThreads, Crew<8>::kBlocks) logprob_s
       const bool strange = a.strange(p.cs);
       RowSums s;
       s.set(a.m, a.mc, a.S, p.cs);
-      const float H = s.some ? kLn2 * (s.L - a.E / s.S) : 0.f;
+      const float H = s.entropy(a.E);
       if constexpr (BWD) {
         Factors f = now.f;
         f.set<ENT>(p, s, H);

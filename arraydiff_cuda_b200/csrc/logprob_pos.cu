@@ -10,10 +10,15 @@ namespace adk {
 
 // The first KT classes of those seen so far (NaN apart: such a row is done again).  16-bit values: value and class in one word, the list sorted by exchanges.
 template <typename T, int KT> struct Firsts;
+// The word orders values and, among equal ones, classes: of two the larger is in front.
+__device__ __forceinline__ uint32_t word_of(float v, uint32_t c) {
+  const uint32_t b = __float_as_uint(v + 0.f);
+  return b ^ ((uint32_t)((int)b >> 31) & 0x7fff0000u) ^ (0x8000ffffu - c);
+}
 template <int KT> struct Firsts<__nv_bfloat16, KT> {
   uint32_t k[KT] = {};
-  __device__ void add(float v, uint32_t c) {
-    uint32_t t = (value_key(v) & 0xffff0000u) | (0xffffu - c);
+  __device__ void add(float v, uint32_t c) { add(word_of(v, c)); }
+  __device__ void add(uint32_t t) {
 #pragma unroll
     for (int i = 0; i < KT; ++i) {
       const uint32_t hi = max(k[i], t);
@@ -46,13 +51,32 @@ template <int KT> struct Firsts<float, KT> {   // classes come in ascending orde
 };
 
 
+// Where a block's lists go: to shared memory, from where they leave in one piece (a position's own entries are parts of sectors:
+// 4,194,304 positions with three entries each wrote 2.4 times their bytes), or directly where they are too long for that
+struct ListOut {
+  uint32_t* cls;   // [positions][top], then as many log probabilities; NULL: directly
+  float* logp;
+  __device__ void put(const LogprobP& p, const RowSums& s, size_t r, uint32_t place, uint32_t at, Key key) const {
+    if (!cls) return put_top(p, s, r, at, key);
+    cls[place * p.top + at] = key ? key_class(key) : kNoClass;
+    logp[place * p.top + at] = key ? s.log_p(key_value((uint32_t)(key >> 32)), p.scale) : -INFINITY;
+  }
+  __device__ void flush(const LogprobP& p, size_t r0, uint32_t n) const {   // behind a barrier
+    if (!cls) return;
+    for (uint32_t i = threadIdx.x; i < n * p.top; i += kPositions) {
+      if (p.top_class) p.top_class[r0 * p.top + i] = cls[i];
+      if (p.top_logp) p.top_logp[r0 * p.top + i] = logp[i];
+    }
+  }
+};
+
 // One position by plain loops: any numbers, any length of list
 template <typename P>
-__device__ __noinline__ void plain_position(const LogprobP& p, const P& x, size_t r, uint32_t l, float xl) {
+__device__ __noinline__ void plain_position(const LogprobP& p, P x, size_t r, uint32_t l, float xl) {
   RowSums s;
   float E;
   plain_position_sums<true>(x, p.cs, s, E);
-  put_row(p, s, r, s.some ? kLn2 * (s.L - E / s.S) : 0.f, l, xl);
+  put_row(p, s, r, s.entropy(E), l, xl);
   if (p.rank) {
     uint32_t n = 0;
     for (uint32_t c = 0; c < x.C; ++c) n += in_front(x.get(c), c, xl, l);
@@ -60,7 +84,7 @@ __device__ __noinline__ void plain_position(const LogprobP& p, const P& x, size_
   }
 }
 template <typename P>
-__device__ __noinline__ void plain_list(const LogprobP& p, const P& x, const RowSums& s, size_t r) {
+__device__ __noinline__ void plain_list(const LogprobP& p, P x, RowSums s, size_t r, ListOut out, uint32_t place) {
   Key last = ~0ull;
   for (uint32_t i = 0; i < p.top; ++i) {
     Key best = 0;
@@ -70,27 +94,27 @@ __device__ __noinline__ void plain_list(const LogprobP& p, const P& x, const Row
         const Key key = v == v ? key_of(v, c) : 0;
         if (key < last && key > best) best = key;
       }
-    put_top(p, s, r, i, best);
+    out.put(p, s, r, place, i, best);
     last = best;
   }
 }
 // Both, as far as they are asked for
 template <typename P>
-__device__ __noinline__ void plain_all(const LogprobP& p, const P& x, size_t r, uint32_t l, float xl) {
+__device__ __noinline__ void plain_all(const LogprobP& p, P x, size_t r, uint32_t l, float xl, ListOut out, uint32_t place) {
   plain_position(p, x, r, l, xl);
   if (p.top) {
     RowSums s;
     float E;
     plain_position_sums<false>(x, p.cs, s, E);
-    plain_list(p, x, s, r);
+    plain_list(p, x, s, r, out, place);
   }
 }
 template <bool ENT, typename P>
-__device__ __noinline__ void plain_gradient(const LogprobP& p, const P& x, const P& o, const P& old, size_t r, uint32_t l, float xl) {
+__device__ __noinline__ void plain_gradient(const LogprobP& p, P x, P o, P old, size_t r, uint32_t l, float xl) {
   RowSums s;
   float E;
   plain_position_sums<ENT>(x, p.cs, s, E);
-  const float H = s.some ? kLn2 * (s.L - E / s.S) : 0.f;
+  const float H = s.entropy(E);
   put_row(p, s, r, H, l, xl);
   Factors f;
   f.fetch(p, r, l);
@@ -107,11 +131,14 @@ __device__ __noinline__ void plain_gradient(const LogprobP& p, const P& x, const
 // ---------------------------------------------------------------- up to 32 classes: a row in registers
 // CM: C rounded up to a multiple of 4.  vec: rows of whole vectors, an odd number of them apart in shared memory.
 template <typename T, int CM, int KT>
-__global__ void __launch_bounds__(kPositions) logprob_few(LogprobP p, int vec) {
+__global__ void __launch_bounds__(kPositions) logprob_few(const __grid_constant__ LogprobP p, int vec) {
   grid_dependency();
   extern __shared__ __align__(16) uint8_t tiles[];
+  __shared__ uint32_t cls[kPositions * KT];
+  __shared__ float logps[kPositions * KT];
   T* tile = (T*)tiles;
   const uint32_t C = p.x.C;
+  const ListOut out = {p.top <= KT ? cls : nullptr, logps};
   const size_t blocks = (p.x.rows + kPositions - 1) / kPositions;
   for (size_t blk = blockIdx.x; blk < blocks; blk += gridDim.x) {
     const size_t r0 = blk * kPositions, r = r0 + threadIdx.x;
@@ -127,37 +154,53 @@ __global__ void __launch_bounds__(kPositions) logprob_few(LogprobP p, int vec) {
       Part a;
       sum_few<true, CM>(a, v, p.cs);
       if (a.strange(p.cs)) {
-        plain_all(p, x, r, l, xl);
+        plain_all(p, x, r, l, xl, out, threadIdx.x);
       } else {
         RowSums s;
         s.set(a.m, a.mc, a.S, p.cs);
-        put_row(p, s, r, s.some ? kLn2 * (s.L - a.E / s.S) : 0.f, l, xl);
-        if (p.rank) {
-          uint32_t k = 0;
+        put_row(p, s, r, s.entropy(a.E), l, xl);
+        Firsts<T, KT> top;
+        uint32_t k = 0;
+        if constexpr (sizeof(T) == 2) {
+          if (p.rank || p.top) {
+            const uint32_t wl = word_of(xl, l < C ? l : 0xffffu);
 #pragma unroll
-          for (uint32_t c = 0; c < CM; ++c)
-            if (c + 4 < CM || c < C) k += in_front(v[c], c, xl, l);
-          p.rank[r] = l < C ? k : kNoClass;
+            for (uint32_t c = 0; c < CM; ++c)
+              if (c + 4 < CM || c < C) {
+                const uint32_t w = word_of(v[c], c);
+                k += w > wl;
+                top.add(w);
+              }
+          }
+        } else {
+          if (p.rank) {
+#pragma unroll
+            for (uint32_t c = 0; c < CM; ++c)
+              if (c + 4 < CM || c < C) k += in_front(v[c], c, xl, l);
+          }
+          if (p.top && p.top <= KT) {
+#pragma unroll
+            for (uint32_t c = 0; c < CM; ++c)
+              if (c + 4 < CM || c < C) top.add(v[c], c);
+          }
         }
-        if (p.top > 8) {
-          plain_list(p, x, s, r);
+        if (p.rank) p.rank[r] = l < C ? k : kNoClass;
+        if (p.top > KT) {
+          plain_list(p, x, s, r, out, threadIdx.x);
         } else if (p.top) {
-          Firsts<T, KT> top;
-#pragma unroll
-          for (uint32_t c = 0; c < CM; ++c)
-            if (c + 4 < CM || c < C) top.add(v[c], c);
 #pragma unroll
           for (int i = 0; i < KT; ++i)
-            if ((uint32_t)i < p.top) put_top(p, s, r, i, top.key(i));
+            if ((uint32_t)i < p.top) out.put(p, s, r, threadIdx.x, i, top.key(i));
         }
       }
     }
     __syncthreads();
+    out.flush(p, r0, n);
   }
 }
 
 template <typename T, int CM, bool ENT>
-__global__ void __launch_bounds__(kPositions) logprob_few_bwd(LogprobP p, int vec) {
+__global__ void __launch_bounds__(kPositions) logprob_few_bwd(const __grid_constant__ LogprobP p, int vec) {
   grid_dependency();
   extern __shared__ __align__(16) uint8_t tiles[];
   const uint32_t C = p.x.C, tp = vec ? tile_pitch<T, 2>(C) : C;
@@ -184,7 +227,7 @@ __global__ void __launch_bounds__(kPositions) logprob_few_bwd(LogprobP p, int ve
       } else {
         RowSums s;
         s.set(a.m, a.mc, a.S, p.cs);
-        const float H = s.some ? kLn2 * (s.L - a.E / s.S) : 0.f;
+        const float H = s.entropy(a.E);
         put_row(p, s, r, H, l, xl);
         f.set<ENT>(p, s, H);
         float gl = f.grad<ENT>(xl, p.cs, s.mc) + f.dl;   // the label's class, whose value replaces the one that the loop writes
@@ -223,9 +266,13 @@ __global__ void __launch_bounds__(kPositions) logprob_few_bwd(LogprobP p, int ve
 template <int MODE, int G> constexpr uint32_t kPlaces = MODE == 0 && G > 1 ? 32 : kPositions;   // positions of a block
 template <bool ENT, typename P, typename F>
 __device__ __forceinline__ void sum_classes(const P& x, Part& a, uint32_t lo, uint32_t hi, float cs, F&& also) {
+  float next[8];
+  x.batch(lo, hi, next);
   for (uint32_t c = lo; c < hi; c += 8) {
     float f[8];
-    x.batch(c, hi, f);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = next[i];
+    if (c + 8 < hi) x.batch(c + 8, hi, next);   // on its way while this one is worked on
     a.reach<ENT>(fmaxf(fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3])), fmaxf(fmaxf(f[4], f[5]), fmaxf(f[6], f[7]))), cs);
     float S[2] = {0.f, 0.f}, E[2] = {0.f, 0.f};
 #pragma unroll
@@ -263,11 +310,14 @@ __device__ __forceinline__ void join_warps(Part& a, Part (&all)[G][32], float cs
 }
 
 template <typename T, int MODE, int KT, int G>
-__global__ void __launch_bounds__(kPositions) logprob_positions_fwd(LogprobP p) {
+__global__ void __launch_bounds__(kPositions) logprob_positions_fwd(const __grid_constant__ LogprobP p) {
   grid_dependency();
   extern __shared__ __align__(16) uint8_t tiles[];
   __shared__ Part sums[G][32];
   __shared__ Key lists[G][KT ? KT : 1][32];
+  __shared__ uint32_t cls[KT ? kPlaces<MODE, G> * KT : 1];
+  __shared__ float logps[KT ? kPlaces<MODE, G> * KT : 1];
+  const ListOut out = {KT ? cls : nullptr, logps};
   T* tile = (T*)tiles;
   constexpr uint32_t N = kPlaces<MODE, G>;
   const uint32_t C = p.x.C, at = threadIdx.x % N, part = G > 1 ? threadIdx.x / N : 0;
@@ -306,19 +356,19 @@ __global__ void __launch_bounds__(kPositions) logprob_positions_fwd(LogprobP p) 
     }
     if (mine && part == 0) {
       if (a.strange(p.cs)) {
-        plain_all(p, x, r, l, xl);
+        plain_all(p, x, r, l, xl, out, at);
       } else {
         a.refer<true>(Part::reference(a.m, p.cs));
         RowSums s;
         s.set(a.m, a.mc, a.S, p.cs);
-        put_row(p, s, r, s.some ? kLn2 * (s.L - a.E / s.S) : 0.f, l, xl);
+        put_row(p, s, r, s.entropy(a.E), l, xl);
         if (p.rank) p.rank[r] = l < C ? a.cnt : kNoClass;
-        if (!KT) {
-          if (p.top) plain_list(p, x, s, r);
-        } else if (G == 1) {
+        if constexpr (KT == 0) {
+          if (p.top) plain_list(p, x, s, r, out, at);
+        } else if constexpr (G == 1) {
 #pragma unroll
           for (int i = 0; i < KT; ++i)
-            if ((uint32_t)i < p.top) put_top(p, s, r, i, top.key(i));
+            if ((uint32_t)i < p.top) out.put(p, s, r, at, i, top.key(i));
         } else {   // the warps' lists are in order
           uint32_t next[G] = {};
           for (uint32_t i = 0; i < p.top; ++i) {
@@ -331,17 +381,19 @@ __global__ void __launch_bounds__(kPositions) logprob_positions_fwd(LogprobP p) 
             }
 #pragma unroll
             for (int g = 0; g < G; ++g) next[g] += best && from == (uint32_t)g;
-            put_top(p, s, r, i, best);
+            out.put(p, s, r, at, i, best);
           }
         }
       }
     }
     __syncthreads();
+    out.flush(p, r0, (uint32_t)(p.x.rows - r0 < N ? p.x.rows - r0 : N));
+    if (KT) __syncthreads();
   }
 }
 
 template <typename T, int MODE, bool ENT, int G>
-__global__ void __launch_bounds__(kPositions) logprob_positions_grad(LogprobP p) {
+__global__ void __launch_bounds__(kPositions) logprob_positions_grad(const __grid_constant__ LogprobP p) {
   grid_dependency();
   extern __shared__ __align__(16) uint8_t tiles[];
   __shared__ Part sums[G][32];
@@ -379,12 +431,16 @@ __global__ void __launch_bounds__(kPositions) logprob_positions_grad(LogprobP p)
         a.refer<ENT>(Part::reference(a.m, p.cs));
         RowSums s;
         s.set(a.m, a.mc, a.S, p.cs);
-        const float H = s.some ? kLn2 * (s.L - a.E / s.S) : 0.f, mc = s.mc;
+        const float H = s.entropy(a.E), mc = s.mc;
         if (part == 0) put_row(p, s, r, H, l, xl);
         f.set<ENT>(p, s, H);
+        float next[8];
+        x.batch(lo, hi, next);
         for (uint32_t c = lo; c < hi; c += 8) {
           float h[8];
-          x.batch(c, hi, h);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) h[i] = next[i];
+          if (c + 8 < hi) x.batch(c + 8, hi, next);
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             h[i] = f.grad<ENT>(h[i], p.cs, mc);

@@ -266,8 +266,8 @@ struct Part {
   __device__ static float reference(float m, float cs) { return fmaxf(m * cs, kFloor); }
   template <bool ENT> __device__ void refer(float mcn) {
     const float d = mc - mcn, f = exp2_fast(d);
-    if (ENT) E = (E + d * S) * f;
-    S *= f;
+    if (ENT) E = __fmul_rn(fmaf(d, S, E), f);   // rounded alike wherever this is inlined: results do not depend on what else is asked for
+    S = __fmul_rn(S, f);
     mc = mcn;
   }
   // before elements of which bm is the largest
@@ -371,8 +371,9 @@ struct RowSums {
     L = some ? log2f(S) : 0.f;
     low = some ? L + fmaf(-m, cs, mc) : 0.f;
   }
-  __device__ float log_p(float x, float scale) const { return some ? (x - m) * scale - kLn2 * low : -INFINITY; }
-  __device__ float lse(float scale) const { return some ? m * scale + kLn2 * low : -INFINITY; }
+  __device__ float log_p(float x, float scale) const { return some ? fmaf(-kLn2, low, __fmul_rn(x - m, scale)) : -INFINITY; }
+  __device__ float entropy(float E) const { return some ? __fmul_rn(kLn2, L - __fdiv_rn(E, S)) : 0.f; }
+  __device__ float lse(float scale) const { return some ? fmaf(kLn2, low, __fmul_rn(m, scale)) : -INFINITY; }
 };
 
 // A row's vectors [vb, ve), batch after batch: f(v0, w) gets the thread's vectors v0 + u * NT + tid, -inf behind the last.
