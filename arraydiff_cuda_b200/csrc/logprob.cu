@@ -28,10 +28,21 @@ __device__ __forceinline__ uint32_t places(uint32_t mine, uint32_t& n) {
   return at;
 }
 
+// One warp: f(bit, place) for every bit that is set in the lanes' words, places one behind the other from n on
+template <typename F>
+__device__ __forceinline__ void each_bit(uint32_t bits, uint32_t& n, F&& f) {
+  const uint32_t below = (1u << (threadIdx.x & 31)) - 1;
+  for (uint32_t who; (who = __ballot_sync(0xffffffffu, bits != 0)) != 0; n += __popc(who))
+    if (bits) {
+      f((uint32_t)__ffs(bits) - 1, n + __popc(who & below));
+      bits &= bits - 1;
+    }
+}
+
 // One warp: of 256 shares' maxima, eight per lane (keys, 0 for none), the k-th, or less; 0: fewer than k
 template <int SHIFT>
 __device__ uint32_t kth_share(const uint32_t (&kv)[8], uint32_t k) {
-  if (k <= 16) {   // the k-th of the lanes' largest: little less
+  if (k <= (SHIFT ? 10 : 20)) {   // the k-th of the lanes' largest: little less, and sooner found than bit by bit
     uint32_t best = kv[0], t = 0;
 #pragma unroll
     for (int i = 1; i < 8; ++i) best = max(best, kv[i]);
@@ -144,37 +155,31 @@ __device__ void select_top(const TopMem& t, uint32_t k, const uint32_t (&kv)[8],
   constexpr int V = X::V;
   constexpr uint32_t kWork = 2048;
   Group<32> g(nullptr);
-  const uint32_t lane = g.tid, below = (1u << lane) - 1;
+  const uint32_t lane = g.tid;
   const uint32_t tv = kth_share<X::kKeyShift>(kv, k);
   const float bound = tv ? key_value(tv) : -INFINITY;
   const uint32_t nv = b.ve - b.vb, per = mx.m ? mx.slots : (nv + 255) / 256;
   // all elements of the shares that reach the bound; where that is too many, those above it, and of the equal ones the first
   for (int strict = 0; strict < 2; ++strict) {
     auto reaches = [&](float v) { return strict ? v > bound : v >= bound; };
-    uint32_t ns = 0, n = 0;
+    uint32_t ns = 0, n = 0, mine = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const bool in = kv[i] && (strict ? kv[i] > tv : kv[i] >= tv);
-      const uint32_t who = __ballot_sync(0xffffffffu, in);
-      if (in) work[ns + __popc(who & below)] = (uint16_t)(i * 32 + lane);
-      ns += __popc(who);
-    }
+    for (int i = 0; i < 8; ++i) mine |= kv[i] && (strict ? kv[i] > tv : kv[i] >= tv) ? 1u << i : 0u;
+    each_bit(mine, ns, [&](uint32_t i, uint32_t at) { work[at] = (uint16_t)(i * 32 + lane); });
     __syncwarp();
-    uint32_t vectors = ns * per;   // of the shares, or (maxima) of their slots that reach it
+    const uint32_t wide = per <= 1 ? 0 : 32 - __clz(per - 1);   // a share's vectors as a power of two
+    uint32_t vectors = ns << wide;   // of the shares, or (maxima) of their slots that reach it
     uint16_t* list = work + 256;
     if (mx.m) {
       uint32_t found = 0;
-      for (uint32_t i0 = 0; i0 < vectors; i0 += 32) {
-        const uint32_t i = i0 + lane, s = i / per, slot = i - s * per;
-        bool in = false;
-        uint16_t at = 0;
-        if (i < vectors) {
-          at = (uint16_t)(slot * 256 + work[s]);
-          in = half_key(mx.m[at]) >= tv >> 16;
-        }
-        const uint32_t who = __ballot_sync(0xffffffffu, in);
-        if (in && found + __popc(who & below) < kWork - 256) list[found + __popc(who & below)] = at;
-        found += __popc(who);
+      for (uint32_t i0 = 0; i0 < ns; i0 += 32) {
+        uint32_t slots = 0;
+        const uint32_t share = i0 + lane < ns ? work[i0 + lane] : 0;
+        if (i0 + lane < ns)
+          for (uint32_t q = 0; q < per; ++q) slots |= half_key(mx.m[q * 256 + share]) >= tv >> 16 ? 1u << q : 0u;
+        each_bit(slots, found, [&](uint32_t q, uint32_t at) {
+          if (at < kWork - 256) list[at] = (uint16_t)(q * 256 + share);
+        });
       }
       if (found > kWork - 256) continue;
       vectors = found * (4u << mx.shift);
@@ -186,13 +191,12 @@ __device__ void select_top(const TopMem& t, uint32_t k, const uint32_t (&kv)[8],
         const uint32_t e = list[i >> (2 + mx.shift)], sub = i & ((4u << mx.shift) - 1);
         return (((e >> 8) << (2 + mx.shift)) + sub) * 256 + (e & 255);
       }
-      const uint32_t s = i / per;
-      return (i - s * per) * 256 + work[s];
+      return (i & ((1u << wide) - 1)) * 256 + work[i >> wide];
     };
     auto look = [&](auto loads, uint32_t i0) {   // so many loads at a time
       constexpr int Q = decltype(loads)::value;
       uint4 w[Q];
-      uint32_t at[Q], hits[Q], mine = 0;
+      uint32_t at[Q];
 #pragma unroll
       for (int q = 0; q < Q; ++q) {
         at[q] = vector_of(i0 + q * 32 + lane);
@@ -200,29 +204,18 @@ __device__ void select_top(const TopMem& t, uint32_t k, const uint32_t (&kv)[8],
       }
 #pragma unroll
       for (int q = 0; q < Q; ++q) {
-        hits[q] = 0;
+        uint32_t hits = 0;
+        const uint32_t c0 = b.class_of(b.vb + at[q]);
         if (at[q] < nv && reaches(X::value(X::max(w[q])))) {
           float f[V];
           X::unpack(w[q], f);
 #pragma unroll
-          for (int j = 0; j < V; ++j) hits[q] |= reaches(f[j]) ? 1u << j : 0u;
+          for (int j = 0; j < V; ++j) hits |= reaches(f[j]) ? 1u << j : 0u;
         }
-        mine += __popc(hits[q]);
+        each_bit(hits, n, [&](uint32_t j, uint32_t to) {
+          if (to < t.cap) t.cand[to] = key_of(X::element(w[q], j), c0 + j);
+        });
       }
-      uint32_t to = places(mine, n);
-#pragma unroll
-      for (int q = 0; q < Q; ++q)
-        if (hits[q]) {
-          float f[V];
-          X::unpack(w[q], f);
-          const uint32_t c0 = b.class_of(b.vb + at[q]);
-#pragma unroll
-          for (int j = 0; j < V; ++j)
-            if (hits[q] >> j & 1) {
-              if (to < t.cap) t.cand[to] = key_of(f[j], c0 + j);
-              ++to;
-            }
-        }
     };
     for (uint32_t i0 = 0; i0 < vectors && n <= t.cap;) {
       if (vectors - i0 <= 32) {
@@ -233,9 +226,9 @@ __device__ void select_top(const TopMem& t, uint32_t k, const uint32_t (&kv)[8],
         i0 += 128;
       }
     }
-    const bool in = sc != kNoClass && reaches(single);
-    const uint32_t to = places(in, n);
-    if (in && to < t.cap) t.cand[to] = key_of(single, sc);
+    each_bit(sc != kNoClass && reaches(single) ? 1u : 0u, n, [&](uint32_t, uint32_t to) {
+      if (to < t.cap) t.cand[to] = key_of(single, sc);
+    });
     if (n <= t.cap) {
       if (strict && n < k) add_equal<T>(t, b, x, bound, k - n, n);
       sort_candidates(t, n, k);
@@ -362,7 +355,7 @@ struct Label {
 // NT 32: a warp per row, eight vectors per lane and batch.  NT 256: for few rows, a block or a cluster of blocks per row.
 // ENT: the entropy is asked for.  RANK: the label's rank.  TOP: top classes.  BWD: the gradient.
 template <int NT, typename T, bool ENT, bool RANK, bool TOP, bool BWD>
-__global__ void __launch_bounds__(256) logprob_rows(LogprobP p, uint32_t slots) {
+__global__ void __launch_bounds__(256, NT == 32 ? (TOP ? 2 : 4) : 3) logprob_rows(LogprobP p, uint32_t slots) {
   typedef Scan<NT, T, ENT, RANK, TOP> S;
   constexpr int U = S::U, V = Vec<T>::V;
   typedef Vec<T> X;
@@ -395,28 +388,44 @@ __global__ void __launch_bounds__(256) logprob_rows(LogprobP p, uint32_t slots) 
     const uint32_t cls = g.tid < 2 * V ? b.single(g.tid) : kNoClass;
     const float single = cls != kNoClass ? ld_f(x + cls) : 0.f;
     Label<T> label;
+    const uint32_t l = p.label ? p.label[r] : kNoClass;
     feed.template start<T>();
-    label.fetch(p, r, x, b);
+    label.fetch(p, l, x, b, 0);
     feed.template run<T, false>([&](uint32_t v0, const uint4 (&w)[U]) { scan.batch(v0, w, false, b, g.tid, p.cs, nothing, label.lv, label.xl, label.thr0); });
     if (TOP && NT != 32) sv[g.tid] = b.vb + g.tid < b.ve ? value_key(a.m) : 0u;
     if (cls != kNoClass) a.add<ENT>(single, p.cs);
     if (RANK) a.cnt += label.own_vector(b, x, C, g.tid) + (cls != kNoClass && label.single_counts(single, cls));
     a.join<ENT, 32>(p.cs);
+    const uint32_t k = p.top;
     if (NT != 32) {
       if ((g.tid & 31) == 0) parts[warp] = a;
       __syncthreads();
       a = parts[g.tid % kRowWarps];
       a.join<ENT, kRowWarps>(p.cs);
-      if (parts_n > 1) {
-        if (g.tid == 0) whole = a;
-        cluster.sync();
-        const uint32_t q = g.tid % 8;
-        if (q < parts_n) a = *cluster.map_shared_rank(&whole, q);
-        else a.clear();
-        a.join<ENT, 8>(p.cs);
+    }
+    if constexpr (TOP) {   // before the blocks of a cluster meet
+      if (NT == 32 || warp == 0) {
+        uint32_t kv[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) kv[i] = NT == 32 ? scan.km[i % S::SH] : sv[i * 32 + g.tid];
+        const Maxima none = {nullptr, 0, 0};
+        // a part that is in shared memory as a whole is looked at there
+        const uint4* vectors = NT != 32 && feed.batches() <= slots ? (const uint4*)dyn : xv + b.vb;
+        select_top<T>(t, k, kv, none, b, x, vectors, cls, single, work[NT == 32 ? warp : 0]);
       }
     }
+    if (parts_n > 1) {
+      if (g.tid == kRowThreads - 1) whole = a;
+      cluster.sync();
+      const uint32_t q = g.tid % 8;
+      if (q < parts_n) a = *cluster.map_shared_rank(&whole, q);
+      else a.clear();
+      a.join<ENT, 8>(p.cs);
+    } else if (TOP) {
+      g.sync();
+    }
     if (a.strange(p.cs)) {
+      if (parts_n > 1) cluster.sync();   // the others' sums have been read
       if (part == 0) plain_row<NT, T, BWD>(g, p, r, t);
       if (parts_n > 1) cluster.sync();
       else g.sync();
@@ -430,34 +439,30 @@ __global__ void __launch_bounds__(256) logprob_rows(LogprobP p, uint32_t slots) 
       if (RANK) p.rank[r] = label.rank(a.cnt, C);
     }
     if constexpr (TOP) {
-      const uint32_t k = p.top;
-      if (NT == 32 || warp == 0) {
-        uint32_t kv[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) kv[i] = NT == 32 ? scan.km[i % S::SH] : sv[i * 32 + g.tid];
-        const Maxima none = {nullptr, 0, 0};
-        select_top<T>(t, k, kv, none, b, x, xv + b.vb, cls, single, work[NT == 32 ? warp : 0]);
-      }
       if (parts_n == 1) {
-        g.sync();
         for (uint32_t i = g.tid; i < k; i += NT) put_top(p, s, r, i, t.list[i]);
       } else {
         // every block's list is in order: an entry's place in the row's is its own and those in front of it in the others
-        cluster.sync();
         Key* all = t.cand + t.cap;
-        for (uint32_t i = g.tid; i < parts_n * k; i += NT) all[i] = cluster.map_shared_rank(t.list, i / k)[i % k];
+        const uint32_t n = parts_n * k;
+        for (uint32_t i = g.tid; i < n; i += NT) all[i] = cluster.map_shared_rank(t.list, i / k)[i % k];
         __syncthreads();
         if (g.tid < k) {
           const Key key = t.list[g.tid];
           uint32_t at = 0;
-          for (uint32_t q = 0; q < parts_n; ++q) {
-            uint32_t lo = 0, hi = k;
-            while (lo < hi) {
-              const uint32_t mid = (lo + hi) / 2;
-              if (all[q * k + mid] > key) lo = mid + 1;
-              else hi = mid;
+          if (n <= 256) {
+#pragma unroll 8
+            for (uint32_t i = 0; i < n; ++i) at += all[i] > key;
+          } else {
+            for (uint32_t q = 0; q < parts_n; ++q) {
+              uint32_t lo = 0, hi = k;
+              while (lo < hi) {
+                const uint32_t mid = (lo + hi) / 2;
+                if (all[q * k + mid] > key) lo = mid + 1;
+                else hi = mid;
+              }
+              at += lo;
             }
-            at += lo;
           }
           if (key && at < k) put_top(p, s, r, at, key);
         }

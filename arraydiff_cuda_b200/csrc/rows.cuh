@@ -156,6 +156,7 @@ template <> struct Vec<float> {
   __device__ static void unpack(uint4 w, float* f) {
     f[0] = __uint_as_float(w.x); f[1] = __uint_as_float(w.y); f[2] = __uint_as_float(w.z); f[3] = __uint_as_float(w.w);
   }
+  __device__ static float element(uint4 w, uint32_t i) { return __uint_as_float(i & 2 ? (i & 1 ? w.w : w.z) : (i & 1 ? w.y : w.x)); }
   __device__ static uint4 pack(const float* f) {
     return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
   }
@@ -191,6 +192,10 @@ template <> struct Vec<__nv_bfloat16> {
     const uint32_t* p = &w.x;
 #pragma unroll
     for (int i = 0; i < 4; ++i) { f[2 * i] = __uint_as_float(p[i] << 16); f[2 * i + 1] = __uint_as_float(p[i] & 0xffff0000u); }
+  }
+  __device__ static float element(uint4 w, uint32_t i) {
+    const uint32_t q = i & 4 ? (i & 2 ? w.w : w.z) : (i & 2 ? w.y : w.x);
+    return __uint_as_float(i & 1 ? q & 0xffff0000u : q << 16);
   }
   __device__ static uint4 pack(const float* f) {
     uint4 w;
@@ -842,7 +847,7 @@ template <int W> inline bool stream_worth(size_t rows, uint32_t parts) { return 
 // Blocks of a row: few rows share the machine, a part at least 8 KB
 inline uint32_t row_parts(size_t rows, size_t row_bytes) {
   uint32_t n = 1;
-  while (n < 8 && rows * n * 2 <= 4 * kNumSMs && row_bytes / (n * 2) >= 8192) n *= 2;
+  while (n < 8 && rows * n * 2 <= 3 * kNumSMs && row_bytes / (n * 2) >= 8192) n *= 2;
   return n;
 }
 // `units` blocks, or clusters of n blocks; a kernel's blocks go on to further rows where there are more
