@@ -701,7 +701,7 @@ static int launch_distill(const DistillP& p, cudaStream_t s) {
   else if (p.x.step != 1 || (BWD && p.g.step != 1) || mask > kMostMask) {
     rc = AD_OK;
     launch(distill_any<T, BWD>, grid_for(p.x.rows, 8), 256, 0, s, p);
-  } else if (p.x.C * sizeof(T) <= 8192) {
+  } else if (by_warp(p.x.rows, p.x.C * sizeof(T), BWD)) {
     const size_t all = p.rest ? kRowWarps * ((vectors + 15) / 16 * 16) : 0;
     rc = p.rest ? launch_rows<32, T, true, BWD>(p, 1, all, s) : launch_rows<32, T, false, BWD>(p, 1, all, s);
   } else {

@@ -798,7 +798,7 @@ static int launch_logprob(const LogprobP& p, cudaStream_t s) {
   int rc = BWD ? logprob_positions_bwd<T>(p, s) : logprob_positions<T>(p, s);
   if (rc != AD_ERR_UNSUPPORTED) {}
   else if (p.x.step != 1 || (BWD && p.g.step != 1)) rc = launch_any<T, BWD>(p, s);
-  else if (p.x.C * sizeof(T) <= 8192) rc = BWD ? launch_bwd<32, T>(p, s) : launch_fwd<32, T>(p, s);
+  else if (by_warp(p.x.rows, p.x.C * sizeof(T), BWD)) rc = BWD ? launch_bwd<32, T>(p, s) : launch_fwd<32, T>(p, s);
   else rc = BWD ? launch_bwd<256, T>(p, s) : launch_fwd<256, T>(p, s);
   if (rc != AD_OK) return rc;
   count_launch();
