@@ -315,3 +315,53 @@ def test_same_bits_captured_and_on_two_streams(rows, Cc, layout):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(loss, w[0]) and torch.equal(g, w[1])
+
+
+# Forms that only many rows reach, as for the log probabilities, and lists of masks that no shared memory holds
+MANY = [(1200, 4100, "bf16"), (1200, 4099, "f32"), (470, 5003, "f32"), (460, 16391, "bf16"), (450, 33001, "bf16"), (230, 40003, "f32"), (112, 70001, "f32"),
+        (56, 140005, "f32"), (57, 300007, "bf16")]
+
+
+@pytest.mark.parametrize("rest", [0, 1])
+@pytest.mark.parametrize("rows,Cc,dtype", MANY)
+def test_special_rows_among_many(rows, Cc, dtype, rest):
+    x = R.logits(77, rows, Cc, "bf16")
+    at = np.linspace(0, rows - 1, 16).astype(int)
+    x[at] = R.special_rows(Cc, Cc, dtype)
+    some = np.unique(np.concatenate([at, H.rng(3).integers(0, rows, 30)]))
+    old = R.rounded(H.normal(6, x.shape), dtype)
+    dloss = H.uniform(8, (rows,), 0.5, 1.0)
+    for k, kw in ((9, dict()), (128, dict(in_place=True)), (40, dict(accumulate=1, old=old, gpitch=Cc + 7, gshift=1)),
+                  (3, dict(accumulate=1, old=old, pitch=(Cc + 63) // 64 * 64, gpitch=(Cc + 63) // 64 * 64))):
+        g = H.rng(k)
+        cls = (g.integers(0, Cc, (rows, 1)) + np.arange(k) * (Cc // (k + 1))).astype(np.int64) % Cc
+        cls[5::7, 0] = cls[5::7, -1]
+        cls[:, 1] = np.where(g.random(rows) < 0.3, Cc - 1, cls[:, 1])   # among the last elements
+        cls[3::5, 2] = 0
+        cls = cls.astype(np.uint32)
+        cls[2::9, 0] = R.NO_CLASS
+        t = g.normal(size=(rows, k)).astype(np.float32)
+        if rest:
+            t = (t - np.log(np.exp(t.astype(np.float64)).sum(1, keepdims=True)) + np.log(0.7)).astype(np.float32)
+        loss, lmag, grad, gmag = R.distill(x[some], 1.0, cls[some], t[some], 1.0, rest)
+        tol = tolerances(x[some], t[some], 1.0, 1.0, False)
+        check_loss(call(x, dtype, rows, 1, NHWC, cls, t, "fwd", rest=rest)[some], loss, lmag, tol, k)
+        got_loss, got = call(x, dtype, rows, 1, NHWC, cls, t, "bwd", rest=rest, dloss=dloss, **kw)
+        check_loss(got_loss[some], loss, lmag, tol, k)
+        check_grad(got[some], grad, gmag, dloss[some], tol, dtype, old[some] if "old" in kw else None)
+
+
+@pytest.mark.parametrize("rows,Cc,dtype", [(2, 300001, "f32"), (2, 1_000_003, "bf16"), (3, 4_100_003, "f32"), (450, 600_001, "bf16")])
+def test_very_many_classes(rows, Cc, dtype):
+    k = 12
+    x = R.logits(5, rows, Cc, dtype)
+    cls, t = teacher(6, x, k, 1)
+    cls[0, 1] = Cc - 1
+    dloss = H.uniform(8, (rows,), 0.5, 1.0)
+    some = np.arange(min(rows, 4))
+    loss, lmag, grad, gmag = R.distill(x[some], 1.0, cls[some], t[some], 1.0, 1)
+    tol = tolerances(x[some], t[some], 1.0, 1.0, False)
+    check_loss(call(x, dtype, rows, 1, NHWC, cls, t, "fwd", rest=1)[some], loss, lmag, tol, k)
+    got_loss, got = call(x, dtype, rows, 1, NHWC, cls, t, "bwd", rest=1, dloss=dloss)
+    check_loss(got_loss[some], loss, lmag, tol, k)
+    check_grad(got[some], grad, gmag, dloss[some], tol, dtype)

@@ -299,3 +299,118 @@ def test_same_bits_on_streams_and_in_graphs(rows, Cc):
         torch.cuda.synchronize()
         for n in o:
             np.testing.assert_array_equal(o[n].cpu().numpy().view(np.uint32), want[n].view(np.uint32))
+
+
+# Forms that only many rows reach: a warp per row of up to tens of KB, blocks that stay (from 444 rows on) with rows that
+# are kept or copied twice, and clusters that share a row (rows of more than 135, 270 and 540 KB)
+MANY = [(1200, 4100, "bf16"), (1200, 4099, "f32"), (470, 5003, "f32"), (460, 16391, "bf16"), (450, 33001, "bf16"), (230, 40003, "f32"), (112, 70001, "f32"),
+        (56, 140005, "f32"), (57, 300007, "bf16")]
+
+
+def spread(x, rows):
+    """Special rows among ordinary ones, at odd places"""
+    out = R.logits(77, rows, x.shape[1], "bf16")
+    at = np.linspace(0, rows - 1, len(x)).astype(int)
+    out[at] = x
+    return out, at
+
+
+@pytest.mark.parametrize("rows,Cc,dtype", MANY)
+def test_special_rows_among_many(rows, Cc, dtype):
+    x, at = spread(R.special_rows(Cc, Cc, dtype), rows)
+    lab = labels(Cc + 1, x)
+    some = np.unique(np.concatenate([at, H.rng(3).integers(0, rows, 30)]))
+    for k, shift in ((9, 3), (100, 0)):
+        got = fwd(x, lab, dtype, rows, 1, NHWC, k, shift=shift)
+        check_fwd(x[some], lab[some], {n: v[some] for n, v in got.items()}, 1.0, k, False)
+    old = R.rounded(H.normal(6, x.shape), dtype)
+    d3 = factors(9, rows)
+    for kw in (dict(), dict(in_place=True), dict(accumulate=1, old=old, gpitch=Cc + 7, gshift=1), dict(accumulate=1, old=old, pitch=(Cc + 63) // 64 * 64, gpitch=(Cc + 63) // 64 * 64)):
+        for f3 in (d3, (None, None, d3[2])):
+            got, outs = bwd(x, lab, dtype, rows, 1, NHWC, f3, **kw)
+            sub = [None if v is None else v[some] for v in f3]
+            check_bwd(x[some], lab[some], got[some], sub, dtype, 1.0, False, old[some] if "old" in kw else None)
+            check_fwd(x[some], lab[some], {n: v[some] for n, v in outs.items()}, 1.0, 0, False)
+
+
+@pytest.mark.parametrize("rows,Cc,dtype", [(1200, 3500, "f32"), (480, 33000, "bf16"), (480, 9000, "f32"), (444, 140000, "bf16")])
+def test_top_of_many_rows_where_the_large_classes_lie_together(rows, Cc, dtype):
+    """As above, by the blocks that stay: stretches and combs of large and of equal classes, rows of one value"""
+    x = R.logits(3, rows, Cc, dtype, 0.5)
+    steps = (1, 4, 8, 256, 1024, 2048, 8192)
+    for i, step in enumerate(steps):
+        c = np.arange(i, Cc, step)[:300]
+        x[i, c] += 20
+        x[rows - 1 - i, c] = 7.0
+    x[20] = 1.0
+    x[21, : Cc // 2] = -np.inf
+    x[22] = -np.inf
+    x[22, Cc - 3:] = 0.0
+    x = R.rounded(x, dtype)
+    lab = labels(4, x)
+    some = np.concatenate([np.arange(25), np.arange(rows - 8, rows)])
+    for k in (1, 12, 128):
+        got = fwd(x, lab, dtype, rows, 1, NHWC, k, shift=2)
+        check_fwd(x[some], lab[some], {n: v[some] for n, v in got.items()}, 1.0, k, False)
+
+
+def test_masked_rows_keep_their_exact_values():
+    """What is masked by -1e9, by the type's lowest value or by -inf does not touch the rest of a row, and a row of the lowest
+    value alone is uniform"""
+    for dtype in ("f32", "bf16"):
+        for rows, Cc in ((40, 19), (40, 50), (40, 300), (40, 5000), (480, 9000)):
+            x = R.logits(5, rows, Cc, dtype)
+            keep = np.zeros(Cc, bool)
+            keep[H.rng(Cc).permutation(Cc)[:max(2, Cc // 3)]] = True
+            want = R.logprob(np.where(keep, x, -np.inf), 1.0, np.zeros(rows, np.uint32), 0)
+            for mask in (-np.inf, -1e9, -1e30, R.LOWEST[dtype]):
+                y = R.rounded(np.where(keep, x, mask), dtype)
+                got = fwd(y, np.zeros(rows, np.uint32), dtype, rows, 1, NHWC, 0, want=("lse", "entropy"))
+                tol = R.tol_log(x, 1.0, Cc <= 64)
+                R.check_close(got["lse"], want["lse"], tol + 2 * R.EPS * abs(want["lse"]), "lse")
+                R.check_close(got["entropy"], want["entropy"], tol * (2 + abs(want["entropy"])), "entropy")
+            low = np.full((rows, Cc), R.LOWEST[dtype], np.float32)
+            got = fwd(low, np.zeros(rows, np.uint32), dtype, rows, 1, NHWC, 0, want=("entropy", "logp"))
+            np.testing.assert_allclose(got["entropy"], np.log(Cc), rtol=1e-5)
+            np.testing.assert_allclose(got["logp"], -np.log(Cc), rtol=1e-5)
+
+
+def test_gradients_captured_with_clusters_and_on_two_streams():
+    """Rows that clusters share, replayed from a graph and on two streams at once, give the bits of a call by itself"""
+    import torch
+    rows, Cc = 230, 40004
+    xs = [torch.from_numpy(R.logits(s, rows, Cc, "f32")).cuda() for s in (1, 2)]
+    lab = torch.randint(0, Cc, (rows,), device="cuda", dtype=torch.int32)
+    one = torch.randn(rows, device="cuda")
+
+    def make(x):
+        g, lse = torch.empty_like(x), torch.empty(rows, device="cuda")
+        a = abi.LogprobArgs(abi.AD_F32, NHWC, rows, Cc, 1, 1.0, x.data_ptr(), 0, lab.data_ptr(), lse.data_ptr())
+        a.dlogp = a.dentropy = one.data_ptr()
+        a.dlogits = g.data_ptr()
+        return a, g, lse
+
+    want = []
+    for x in xs:
+        a, g, lse = make(x)
+        abi.check(abi.lib().ad_logprob_bwd(C.byref(a), H.stream()))
+        H.sync()
+        want.append((g, lse))
+    jobs, streams = [make(x) for x in xs], [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for s, j in zip(streams, jobs):
+            abi.check(abi.lib().ad_logprob_bwd(C.byref(j[0]), C.c_void_p(s.cuda_stream)))
+    torch.cuda.synchronize()
+    for j, w in zip(jobs, want):
+        assert torch.equal(j[1], w[0]) and torch.equal(j[2], w[1])
+    buf = xs[0].clone()
+    a, g, lse = make(buf)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        abi.check(abi.lib().ad_logprob_bwd(C.byref(a), H.stream()))
+    for x, w in ((xs[1], want[1]), (xs[0], want[0])):
+        buf.copy_(x)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(g, w[0]) and torch.equal(lse, w[1])
