@@ -140,20 +140,20 @@ struct Maxima {
   const uint16_t* m;
   uint32_t shift, slots;
 };
-constexpr uint32_t kMostSlots = 16;
+constexpr uint32_t kMostSlots = 8;
 __device__ __forceinline__ uint32_t half_key(uint32_t h) { return h & 0x8000u ? 0xffffu ^ h : h | 0x8000u; }   // value_key >> 16
 
+constexpr uint32_t kWork = 1024;   // words of 16 bits that a selection works with
 template <int N> struct Loads { static constexpr int value = N; };
 
 // One warp: a strip's list out of its 256 shares, of which lane i has number 32 j + i in kv[j]: the key of its largest value, 0
 // for none.  Share s is the vectors vb + s + 256 n, xv[0] being vector vb.  `single`: a single element of the strip in this
-// lane (class `sc`).  work: 256 words of 16 bits, with maxima 2048.
+// lane (class `sc`).  work: 256 words of 16 bits, with maxima kWork.
 template <typename T>
 __device__ void select_top(const TopMem& t, uint32_t k, const uint32_t (&kv)[8], const Maxima& mx, const Strip<T>& b, const T* x, const uint4* xv, uint32_t sc,
                            float single, uint16_t* work) {
   typedef Vec<T> X;
   constexpr int V = X::V;
-  constexpr uint32_t kWork = 2048;
   Group<32> g(nullptr);
   const uint32_t lane = g.tid;
   const uint32_t tv = kth_share<X::kKeyShift>(kv, k);
@@ -517,39 +517,39 @@ struct LogprobSlot {
   bool strange;
 };
 template <typename T, bool ENT, bool RANK, bool TOP, bool BWD>
-__global__ void __launch_bounds__(Crew<8>::kThreads, Crew<8>::kBlocks) logprob_stream(LogprobP p, RingPlan plan) {
-  constexpr int W = 8;
+__global__ void __launch_bounds__(Crew<8>::kThreads + (TOP ? 32 : 0), Crew<8>::kBlocks) logprob_stream(LogprobP p, RingPlan plan) {
+  constexpr int W = 8, E = TOP ? 2 : 1, N = 2 * E;   // warps beside the streaming ones, rows in hand
   typedef Crew<W> Team;
   typedef Stream<T, W, BWD> Str;
   constexpr int U = Str::U, V = Vec<T>::V;
   constexpr uint32_t NS = Str::NS;
   typedef Scan<(int)NS, T, ENT, RANK, TOP, U> S;
   extern __shared__ __align__(16) uint4 ring[];   // batches of vectors, then what the top classes need
-  __shared__ LogprobSlot<T, W> slot[2];
+  __shared__ LogprobSlot<T, W> slot[N];
   __shared__ Key red[W];
   __shared__ Part whole[2];
-  __shared__ uint16_t work[TOP ? 2048 : 1];
+  __shared__ uint16_t works[E][TOP ? kWork : 1];
   grid_dependency();
   cg::cluster_group cluster = cg::this_cluster();
   const uint32_t parts = BWD ? cluster.num_blocks() : 1, part = BWD ? cluster.block_rank() : 0, row0 = blockIdx.x / parts, stride = gridDim.x / parts;
   const uint32_t rows = (uint32_t)p.x.rows;
   const uint32_t shift = slot_shift<T>(p.x.C), slots = (p.x.C / V + (Str::kBatch << shift) - 1) / (Str::kBatch << shift);
-  uint16_t* maxima = (uint16_t*)((uint8_t*)ring + plan.bytes);   // [2][slots][256]
+  uint16_t* maxima = (uint16_t*)((uint8_t*)ring + plan.bytes);   // [N][slots][256]
   const uint32_t C = p.x.C, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const float nothing = as_nothing(p.cs);
   if (warp < W) {
     Str stream((const T*)p.logits, p.x, ring, plan.slots, plan.twice != 0, row0, stride, part, parts);
     uint32_t i = 0;
     for (uint32_t r = row0; r < rows; r += stride, ++i) {
-      LogprobSlot<T, W>& q = slot[i & 1];
+      LogprobSlot<T, W>& q = slot[i % N];
       const T* x = (const T*)p.logits + p.x.offset(r);
       const Strip<T> b(x, C, part, parts);
-      Team::wait(kBarReady + (i & 1));
+      Team::wait(kBarReady + (i % N));
       const uint32_t lv = q.label.lv;
       const float xl = q.label.xl, thr0 = q.label.thr0;
       S scan;
       scan.clear();
-      uint16_t* mine = maxima + (i & 1) * slots * 256 + tid;
+      uint16_t* mine = maxima + (i % N) * slots * 256 + tid;
       float most = -INFINITY;
       auto sums = [&](uint32_t v0, const uint4 (&w)[U], bool full) {
         const float bm = scan.batch(b.vb + v0, w, full, b, tid, p.cs, nothing, lv, xl, thr0);
@@ -565,7 +565,7 @@ __global__ void __launch_bounds__(Crew<8>::kThreads, Crew<8>::kBlocks) logprob_s
       if (TOP) q.sv[tid] = tid < nv ? value_key(scan.a.m) : 0u;
       scan.a.template join<ENT, 32>(p.cs);
       if (lane == 0) q.parts[warp] = scan.a;
-      Team::arrive(kBarSums + (i & 1));
+      Team::arrive(kBarSums + (i % N));
       if constexpr (BWD) {
         __syncwarp();
         if (parts > 1) cluster.sync();
@@ -610,24 +610,26 @@ __global__ void __launch_bounds__(Crew<8>::kThreads, Crew<8>::kBlocks) logprob_s
     }
   } else {
     TopMem t = {nullptr, nullptr, TopMem::room(p.top)};
-    t.list = (Key*)(maxima + (TOP ? 2 * slots * 256 : 0));
+    const uint32_t who = warp - W;   // rows who, who + E, ...
+    t.list = (Key*)(maxima + (TOP ? N * slots * 256 : 0)) + who * (p.top + t.cap);
     t.cand = t.list + p.top;
     struct Row {   // what this warp keeps of a row between its two turns
       uint32_t cls, own;
       float single, old;
       Factors f;
     };
-    uint32_t coming = p.label && row0 < rows ? p.label[row0] : kNoClass;   // the label of the row to be prepared next
+    const uint32_t first = row0 + who * stride, step = E * stride;
+    uint32_t coming = p.label && first < rows ? p.label[first] : kNoClass;   // the label of the row to be prepared next
     auto prepare = [&](uint32_t r, uint32_t i) {
       Row w = {kNoClass, 0, 0.f, 0.f, {}};
       if (r >= rows) return w;
       if (BWD && i >= 2) Team::wait(kBarFree + (i & 1));
-      LogprobSlot<T, W>& q = slot[i & 1];
+      LogprobSlot<T, W>& q = slot[i % N];
       const T* x = (const T*)p.logits + p.x.offset(r);
       const Strip<T> b(x, C, part, parts);
       Label<T> label;
       label.fetch(p, coming, x, b, 0);
-      coming = p.label && r + stride < rows ? p.label[r + stride] : kNoClass;
+      coming = p.label && r + step < rows ? p.label[r + step] : kNoClass;
       w.cls = lane < 2 * V ? b.single(lane) : kNoClass;
       if (w.cls != kNoClass) {
         w.single = ld_f(x + w.cls);
@@ -637,18 +639,18 @@ __global__ void __launch_bounds__(Crew<8>::kThreads, Crew<8>::kBlocks) logprob_s
       if (BWD) w.f.fetch(p, r, label.l);
       if (lane == 0) q.label = label;
       __syncwarp();
-      Team::arrive(kBarReady + (i & 1));
+      Team::arrive(kBarReady + (i % N));
       return w;
     };
-    uint32_t i = 0;
-    Row now = prepare(row0, 0);
-    for (uint32_t r = row0; r < rows; r += stride, ++i) {
-      const Row next = prepare(r + stride, i + 1);
-      LogprobSlot<T, W>& q = slot[i & 1];
+    uint32_t i = who;
+    Row now = prepare(first, i);
+    for (uint32_t r = first; r < rows; r += step, i += E) {
+      const Row next = prepare(r + step, i + E);
+      LogprobSlot<T, W>& q = slot[i % N];
       const T* x = (const T*)p.logits + p.x.offset(r);
       const Strip<T> b(x, C, part, parts);
       const Label<T> label = q.label;
-      Team::wait(kBarSums + (i & 1));
+      Team::wait(kBarSums + (i % N));
       Part a;
       a.clear();
       if (lane < W) a = q.parts[lane];
@@ -691,8 +693,8 @@ __global__ void __launch_bounds__(Crew<8>::kThreads, Crew<8>::kBlocks) logprob_s
           uint32_t kv[8];
 #pragma unroll
           for (int j = 0; j < 8; ++j) kv[j] = q.sv[j * 32 + lane];
-          const Maxima mx = {maxima + (i & 1) * slots * 256, shift, slots};
-          select_top<T>(t, p.top, kv, mx, b, x, (const uint4*)(x + b.head), now.cls, now.single, work);
+          const Maxima mx = {maxima + (i % N) * slots * 256, shift, slots};
+          select_top<T>(t, p.top, kv, mx, b, x, (const uint4*)(x + b.head), now.cls, now.single, works[who]);
           for (uint32_t j = lane; j < p.top; j += 32) put_top(p, s, r, j, t.list[j]);
           __syncwarp();
         }
@@ -758,11 +760,11 @@ static int launch_rows(const LogprobP& p, cudaStream_t s) {
   if constexpr (NT != 32) {
     constexpr int W = 8;
     const uint32_t shift = slot_shift<T>(p.x.C), slots = (p.x.C / Vec<T>::V + (1024u << shift) - 1) / (1024u << shift);
-    const size_t besides = TOP ? list * sizeof(Key) + 2 * slots * 256 * 2 : 0;
+    const size_t besides = TOP ? 2 * list * sizeof(Key) + 4 * slots * 256 * 2 : 0;
     const RingPlan plan = ring_plan<T, W, BWD>(p.x.C, [&](uint32_t) { return besides; });
     if (stream_worth<W>(p.x.rows, plan.parts)) {
       static StreamLaunch shared;
-      return launch_stream<W>(logprob_stream<T, ENT, RANK, TOP, BWD>, shared, p.x.rows, plan.parts, plan.bytes + besides, s, p, plan);
+      return launch_stream(logprob_stream<T, ENT, RANK, TOP, BWD>, shared, Crew<W>::kThreads + (TOP ? 32 : 0), p.x.rows, plan.parts, plan.bytes + besides, s, p, plan);
     }
   }
   auto kernel = logprob_rows<NT, T, ENT, RANK, TOP, BWD>;

@@ -471,11 +471,11 @@ constexpr size_t kMostFeed = 96 * 1024;
 // of it) that fits into the ring stays there for the second pass, each batch of which makes room for one of the next row;
 // other rows are copied again, out of the L2.  One block of an SM with sixteen warps and 192 KB of ring was slower (4096 rows
 // of 64 KB: 149 us for 122): nothing else fills the SM while a row's sums are joined.
-enum { kBarReady = 1, kBarSums = 3, kBarResult = 5, kBarFree = 7 };   // and the row's parity; 9: Group<W * 32>
+enum { kBarReady = 1, kBarResult = 3, kBarSums = 5, kBarFree = 7 };   // and the row's slot (of four forward, of two backward); 9: Group<W * 32>
 // The sums of the blocks of a cluster: whole[parity] is this block's, the one in the same place the others'.  All threads of
 // all blocks meet in between, and the next row's meeting comes before whole[parity] is written again.
 template <int W> struct Crew {
-  static constexpr uint32_t kStreaming = W * 32, kThreads = W * 32 + 32, kBlocks = 3;   // blocks of an SM
+  static constexpr uint32_t kThreads = W * 32 + 32, kBlocks = 3;   // that meet at a barrier, blocks of an SM
   __device__ static void arrive(uint32_t id) {
     __syncwarp();
     __threadfence_block();
@@ -614,8 +614,8 @@ struct StreamLaunch {
   unsigned long long held[4];   // shared memory << 32 | clusters
 };
 constexpr size_t kMostRing = 218 * 1024;   // dynamic shared memory of the blocks that stay
-template <int W, typename... P, typename... A>
-inline int launch_stream(void (*kernel)(P...), StreamLaunch& l, size_t rows, uint32_t parts, size_t smem, cudaStream_t s, A... args) {
+template <typename... P, typename... A>
+inline int launch_stream(void (*kernel)(P...), StreamLaunch& l, uint32_t threads, size_t rows, uint32_t parts, size_t smem, cudaStream_t s, A... args) {
   int dev = 0;
   cudaGetDevice(&dev);
   if (!(__atomic_load_n(&l.raised, __ATOMIC_RELAXED) & (1u << (dev & 31)))) {
@@ -627,7 +627,7 @@ inline int launch_stream(void (*kernel)(P...), StreamLaunch& l, size_t rows, uin
   }
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute at[2];
-  cfg.blockDim = Crew<W>::kThreads;
+  cfg.blockDim = threads;
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cfg.gridDim = parts;
