@@ -80,13 +80,13 @@ __device__ __forceinline__ Distilled distill_row(const DistillP& p, size_t r, Li
   loss = d.some ? loss + 0.f * d.L : 0.f;   // NaN without any entry, too
   return d;
 }
-// The gradient of entry j's class
-__device__ __forceinline__ float listed_grad(const DistillP& p, const Distilled& d, const List& list, uint32_t j, float f) {
+// The gradient of entry j's class; q: the entries' weights
+__device__ __forceinline__ float listed_grad(const DistillP& p, const Distilled& d, const List& list, const float* q, uint32_t j, float f) {
   const uint32_t c = list.cls[j];
-  float sum = list.a[j];
+  float sum = q[j];
   if (list.twice) {
     sum = 0.f;
-    for (uint32_t i = 0; i < p.top; ++i) sum += list.cls[i] == c ? list.a[i] : 0.f;
+    for (uint32_t i = 0; i < p.top; ++i) sum += list.cls[i] == c ? q[i] : 0.f;
   }
   return d.some ? f * (exp2_fast((list.x[j] - d.mt) * p.cs) * d.rS * d.Q - sum) : 0.f;
 }
@@ -141,7 +141,7 @@ __device__ void plain_row(Group<NT>& g, const DistillP& p, size_t r, List& list,
     for (int i = 0; i < 4; ++i) {
       const uint32_t j = g.tid + i * NT;
       if (j < k && list.cls[j] < C) {
-        const float v = listed_grad(p, d, list, j, f);
+        const float v = listed_grad(p, d, list, list.a, j, f);
         st_f(o + list.cls[j] * p.g.step, p.accumulate ? old[i] + v : v);
       }
     }
@@ -313,7 +313,7 @@ __global__ void __launch_bounds__(256) distill_rows(DistillP p, uint32_t slots) 
 #pragma unroll
       for (int i = 0; i < (NT == 32 ? 4 : 1); ++i) {
         const uint32_t j = g.tid + i * NT;
-        if (j < k && list.cls[j] >= b.begin() && list.cls[j] < b.end()) gl[i] = listed_grad(p, d, list, j, f) + (p.accumulate ? ld_f(o + list.cls[j]) : 0.f);
+        if (j < k && list.cls[j] >= b.begin() && list.cls[j] < b.end()) gl[i] = listed_grad(p, d, list, list.a, j, f) + (p.accumulate ? ld_f(o + list.cls[j]) : 0.f);
       }
       if (p.accumulate) g.sync();
       if (sc != kNoClass) st_f(o + sc, grad(ld_f(x + sc)) + (p.accumulate ? ld_f(o + sc) : 0.f));
@@ -343,7 +343,7 @@ __global__ void __launch_bounds__(256) distill_rows(DistillP p, uint32_t slots) 
 template <int W>
 struct __align__(16) DistillSlot {
   List list;
-  float old[kMostTop], grad[kMostTop];   // what the gradient of an entry's class is added to, and that gradient
+  float q[kMostTop], old[kMostTop], grad[kMostTop];   // an entry's weight, what the gradient of its class is added to, and that gradient
   Part parts[W];
   float mc, coef;
   uint32_t singles;                      // which of the row's single elements are listed
@@ -446,10 +446,11 @@ __global__ void __launch_bounds__(Crew<8>::kThreads, Crew<8>::kBlocks) distill_s
     struct Row {   // what this warp keeps of a row between its two turns
       uint32_t cls;
       float single, old, Q, mk, K, dloss;
-      bool apart;
+      Part sum;   // of the row's single elements that are not listed
     };
     auto prepare = [&](uint32_t r, uint32_t i) {
-      Row w = {kNoClass, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, true};
+      Row w = {kNoClass, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, {}};
+      w.sum.clear();
       if (r >= rows) return w;
       if (BWD && i >= 2) Team::wait(kBarFree + (i & 1));
       DistillSlot<W>& q = slot[i & 1];
@@ -491,7 +492,7 @@ __global__ void __launch_bounds__(Crew<8>::kThreads, Crew<8>::kBlocks) distill_s
         shift = z != 0.f ? am + log2f(z) : 0.f;
       }
       // which classes are listed, and whether one of them stands twice
-      bool twice = false;
+      bool twice = false, apart = true;
       if (REST) {
         for (uint32_t v = lane; v < (b.ve - b.vb + 15) / 16; v += 32) ((uint4*)mask)[v] = make_uint4(0, 0, 0, 0);
         if (lane == 0) q.singles = 0;
@@ -514,7 +515,7 @@ __global__ void __launch_bounds__(Crew<8>::kThreads, Crew<8>::kBlocks) distill_s
         if (parts > 1) twice = true;   // the other parts are not known: looked for below
         twice = __any_sync(0xffffffffu, twice);
         __syncwarp();
-        w.apart = !(q.singles >> lane & 1u);
+        apart = !(q.singles >> lane & 1u);
       }
       if (BWD && !REST) twice = true;   // looked for below
       bool first[4] = {true, true, true, true};
@@ -549,11 +550,16 @@ __global__ void __launch_bounds__(Crew<8>::kThreads, Crew<8>::kBlocks) distill_s
       }
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
+        if (32 * e >= (int)k) break;
         a[e] -= shift;
+        const float weight = exp2f(a[e]);
         q.list.a[lane + 32 * e] = a[e];
-        w.Q += exp2f(a[e]);
+        q.q[lane + 32 * e] = weight;
+        w.Q += weight;
       }
       w.Q = warp_sum(w.Q);
+      if (w.cls != kNoClass && apart) w.sum.add<false>(w.single, p.cs);
+      w.sum.join<false, 32>(p.cs);
       if (lane == 0) q.list.twice = twice;
       Team::arrive(kBarReady + (i & 1));
       return w;
@@ -566,9 +572,9 @@ __global__ void __launch_bounds__(Crew<8>::kThreads, Crew<8>::kBlocks) distill_s
       Team::wait(kBarSums + (i & 1));
       Part a;
       a.clear();
-      if (lane < W) a = q.parts[lane];
-      if (now.cls != kNoClass && now.apart) a.add<false>(now.single, p.cs);
-      a.join<false, 32>(p.cs);
+      if (lane % 16 < W) a = q.parts[lane % 16];
+      else if (lane % 16 == W) a = now.sum;
+      a.join<false, 16>(p.cs);
       if (parts > 1) {
         if (lane == 0) whole[i & 1] = a;
         __syncwarp();
@@ -583,23 +589,11 @@ __global__ void __launch_bounds__(Crew<8>::kThreads, Crew<8>::kBlocks) distill_s
       const Distilled d = row_sums(p, a.m, off, a.S, now.mk, now.K, now.Q, loss);
       const float f = now.dloss * p.scale;
       if (!strange) {
-        float terms = 0.f, w[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint32_t j = lane + 32 * e;
-          const float v = q.list.a[j];
-          w[e] = exp2f(v);
-          terms += d.term(w[e], v, q.list.x[j], p.scale);
-        }
         if (BWD) {
-          __syncwarp();
-#pragma unroll
-          for (int e = 0; e < 4; ++e) q.list.a[lane + 32 * e] = w[e];
-          __syncwarp();
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const uint32_t j = lane + 32 * e;
-            if (j < k) q.grad[j] = listed_grad(p, d, q.list, j, f) + (p.accumulate ? q.old[j] : 0.f);
+            if (j < k) q.grad[j] = listed_grad(p, d, q.list, q.q, j, f) + (p.accumulate ? q.old[j] : 0.f);
           }
           if (lane == 0) {
             q.mc = a.mc;
@@ -609,6 +603,12 @@ __global__ void __launch_bounds__(Crew<8>::kThreads, Crew<8>::kBlocks) distill_s
           // before the list's, which the streaming threads write behind this barrier
           if (now.cls != kNoClass) st_f((T*)p.dlogits + p.g.offset(r) + now.cls, f * d.out * exp2_fast(fmaf(now.single, p.cs, -a.mc)) + now.old);
           Team::arrive(kBarResult + (i & 1));
+        }
+        float terms = 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t j = lane + 32 * e;
+          if (j < k) terms += d.term(q.q[j], q.list.a[j], q.list.x[j], p.scale);
         }
         loss += warp_sum(terms);
         if (lane == 0 && part == 0 && p.loss) p.loss[r] = d.some ? loss + 0.f * d.L : 0.f;

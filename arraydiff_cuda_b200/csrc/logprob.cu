@@ -614,14 +614,16 @@ __global__ void __launch_bounds__(Crew<8>::kThreads + (TOP ? 32 : 0), Crew<8>::k
     t.list = (Key*)(maxima + (TOP ? N * slots * 256 : 0)) + who * (p.top + t.cap);
     t.cand = t.list + p.top;
     struct Row {   // what this warp keeps of a row between its two turns
-      uint32_t cls, own;
+      uint32_t cls;
       float single, old;
       Factors f;
+      Part sum;   // of the row's single elements
     };
     const uint32_t first = row0 + who * stride, step = E * stride;
     uint32_t coming = p.label && first < rows ? p.label[first] : kNoClass;   // the label of the row to be prepared next
     auto prepare = [&](uint32_t r, uint32_t i) {
-      Row w = {kNoClass, 0, 0.f, 0.f, {}};
+      Row w = {kNoClass, 0.f, 0.f, {}, {}};
+      w.sum.clear();
       if (r >= rows) return w;
       if (BWD && i >= 2) Team::wait(kBarFree + (i & 1));
       LogprobSlot<T, W>& q = slot[i % N];
@@ -635,7 +637,9 @@ __global__ void __launch_bounds__(Crew<8>::kThreads + (TOP ? 32 : 0), Crew<8>::k
         w.single = ld_f(x + w.cls);
         if (BWD && p.accumulate) w.old = ld_f((const T*)p.dlogits + p.g.offset(r) + w.cls);
       }
-      if (RANK) w.own = label.own_vector(b, x, C, lane);
+      if (w.cls != kNoClass) w.sum.add<ENT>(w.single, p.cs);
+      if (RANK) w.sum.cnt = label.own_vector(b, x, C, lane) + (w.cls != kNoClass && label.single_counts(w.single, w.cls));
+      w.sum.join<ENT, 32>(p.cs);
       if (BWD) w.f.fetch(p, r, label.l);
       if (lane == 0) q.label = label;
       __syncwarp();
@@ -653,10 +657,9 @@ __global__ void __launch_bounds__(Crew<8>::kThreads + (TOP ? 32 : 0), Crew<8>::k
       Team::wait(kBarSums + (i % N));
       Part a;
       a.clear();
-      if (lane < W) a = q.parts[lane];
-      if (now.cls != kNoClass) a.add<ENT>(now.single, p.cs);
-      if (RANK) a.cnt += now.own + (now.cls != kNoClass && label.single_counts(now.single, now.cls));
-      a.join<ENT, 32>(p.cs);
+      if (lane % 16 < W) a = q.parts[lane % 16];
+      else if (lane % 16 == W) a = now.sum;
+      a.join<ENT, 16>(p.cs);
       if (parts > 1) {
         if (lane == 0) whole[i & 1] = a;
         __syncwarp();
