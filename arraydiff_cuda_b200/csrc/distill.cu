@@ -640,7 +640,7 @@ static int distill_args(const ad_distill_args* a, bool bwd, DistillP& p) {
   if (a->top > kMostTop) return AD_ERR_LIMIT;
   if (a->top == 0 || !a->top_class || !a->top_logit) return AD_ERR_BAD_ARG;
   const size_t elem = (size_t)elem_size(a->dtype);
-  if (!aligned_to(a->logits, elem)) return AD_ERR_ALIGN;
+  if (!aligned_to(a->logits, elem) || !words(a->top_class, a->top_logit, a->top_lse, a->loss)) return AD_ERR_ALIGN;
   p.logits = a->logits;
   p.scale = a->scale;
   p.cs = (float)(a->scale * kLog2e);
@@ -655,7 +655,7 @@ static int distill_args(const ad_distill_args* a, bool bwd, DistillP& p) {
     rc = rows_of(a->dtype, a->layout, a->N, a->C, a->HW, a->dlogits_pitch, p.g);
     if (rc != AD_OK) return rc;
     if (!a->dlogits || !a->dloss) return AD_ERR_BAD_ARG;
-    if (!aligned_to(a->dlogits, elem)) return AD_ERR_ALIGN;
+    if (!aligned_to(a->dlogits, elem) || !words(a->dloss)) return AD_ERR_ALIGN;
     if (!gradient_clear(p.x, a->logits, p.g, a->dlogits, elem, a->accumulate)) return AD_ERR_BAD_ARG;
     p.dlogits = a->dlogits;
     p.dloss = a->dloss;
@@ -697,8 +697,8 @@ static int launch_distill(const DistillP& p, cudaStream_t s) {
   const uint32_t n = row_parts(p.x.rows, (size_t)p.x.C * sizeof(T));
   const size_t mask = p.rest ? (vectors / n + 17) / 16 * 16 : 0;
   int rc = distill_positions<T, BWD>(p, s);
-  if (rc != AD_ERR_UNSUPPORTED) {}
-  else if (p.x.step != 1 || (BWD && p.g.step != 1) || mask > kMostMask) {
+  if (rc != AD_ERR_UNSUPPORTED) {   // a thread per position
+  } else if (p.x.step != 1 || (BWD && p.g.step != 1) || mask > kMostMask) {
     rc = AD_OK;
     launch(distill_any<T, BWD>, grid_for(p.x.rows, 8), 256, 0, s, p);
   } else if (by_warp(p.x.rows, p.x.C * sizeof(T), BWD)) {

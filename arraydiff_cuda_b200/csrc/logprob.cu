@@ -716,7 +716,7 @@ static int logprob_args(const ad_logprob_args* a, bool bwd, LogprobP& p) {
   if (rc != AD_OK || p.x.rows == 0) return rc;
   if (!a->logits || !scale_ok(a->scale)) return AD_ERR_BAD_ARG;
   const size_t elem = (size_t)elem_size(a->dtype);
-  if (!aligned_to(a->logits, elem)) return AD_ERR_ALIGN;
+  if (!aligned_to(a->logits, elem) || !words(a->label, a->lse, a->entropy, a->logp)) return AD_ERR_ALIGN;
   p.logits = a->logits;
   p.scale = a->scale;
   p.cs = (float)(a->scale * kLog2e);
@@ -729,7 +729,7 @@ static int logprob_args(const ad_logprob_args* a, bool bwd, LogprobP& p) {
     rc = rows_of(a->dtype, a->layout, a->N, a->C, a->HW, a->dlogits_pitch, p.g);
     if (rc != AD_OK) return rc;
     if (!a->dlogits || (!a->dlse && !a->dentropy && !a->dlogp) || (a->dlogp && !a->label)) return AD_ERR_BAD_ARG;
-    if (!aligned_to(a->dlogits, elem)) return AD_ERR_ALIGN;
+    if (!aligned_to(a->dlogits, elem) || !words(a->dlse, a->dentropy, a->dlogp)) return AD_ERR_ALIGN;
     if (!gradient_clear(p.x, a->logits, p.g, a->dlogits, elem, a->accumulate)) return AD_ERR_BAD_ARG;
     p.dlogits = a->dlogits;
     p.dlse = a->dlse;
@@ -741,6 +741,7 @@ static int logprob_args(const ad_logprob_args* a, bool bwd, LogprobP& p) {
     if (a->top > kMostTop) return AD_ERR_LIMIT;
     if (a->top && !a->top_class && !a->top_logp) return AD_ERR_BAD_ARG;
     if (!a->lse && !a->entropy && !a->logp && !a->rank && !a->top) return AD_ERR_BAD_ARG;
+    if (!words(a->rank) || (a->top && !words(a->top_class, a->top_logp))) return AD_ERR_ALIGN;
     p.rank = a->rank;
     p.top = a->top;
     p.top_class = a->top_class;
@@ -801,8 +802,8 @@ static int launch_bwd(const LogprobP& p, cudaStream_t s) {
 template <typename T, bool BWD>
 static int launch_logprob(const LogprobP& p, cudaStream_t s) {
   int rc = BWD ? logprob_positions_bwd<T>(p, s) : logprob_positions<T>(p, s);
-  if (rc != AD_ERR_UNSUPPORTED) {}
-  else if (p.x.step != 1 || (BWD && p.g.step != 1)) rc = launch_any<T, BWD>(p, s);
+  if (rc != AD_ERR_UNSUPPORTED) {   // a thread per position
+  } else if (p.x.step != 1 || (BWD && p.g.step != 1)) rc = launch_any<T, BWD>(p, s);
   else if (by_warp(p.x.rows, p.x.C * sizeof(T), BWD)) rc = BWD ? launch_bwd<32, T>(p, s) : launch_fwd<32, T>(p, s);
   else rc = BWD ? launch_bwd<256, T>(p, s) : launch_fwd<256, T>(p, s);
   if (rc != AD_OK) return rc;

@@ -68,6 +68,7 @@ inline bool gradient_clear(const Rows& x, const void* logits, const Rows& g, con
 }
 inline bool scale_ok(float s) { return s >= 1e-30f && s <= 1e30f; }
 inline bool aligned_to(const void* p, size_t a) { return ((uintptr_t)p & (a - 1)) == 0; }
+template <typename... P> inline bool words(P... p) { return ((aligned_to(p, 4)) && ...); }
 
 __device__ __forceinline__ float exp2_fast(float v) {
   float r;

@@ -82,6 +82,21 @@ def test_distill(over, want):
     assert status("ad_distill_bwd", distill(**over)) == want
 
 
+@pytest.mark.parametrize("name", ["label", "lse", "entropy", "logp", "rank", "top_class", "top_logp"])
+def test_logprob_words(name):
+    assert status("ad_logprob_fwd", logprob(**{"top": 2, "top_class": 0x6000, name: 0x7002})) == abi.AD_ERR_ALIGN
+
+
+@pytest.mark.parametrize("name", ["label", "lse", "entropy", "logp", "dlse", "dentropy", "dlogp"])
+def test_logprob_gradient_words(name):
+    assert status("ad_logprob_bwd", logprob(**{name: 0x7001})) == abi.AD_ERR_ALIGN
+
+
+@pytest.mark.parametrize("name", ["top_class", "top_logit", "top_lse", "loss", "dloss"])
+def test_distill_words(name):
+    assert status("ad_distill_bwd", distill(**{name: 0x7003})) == abi.AD_ERR_ALIGN
+
+
 def test_distill_pointers():
     assert status("ad_distill_fwd", distill(loss=None)) == abi.AD_ERR_BAD_ARG
     assert status("ad_distill_bwd", distill(dloss=None)) == abi.AD_ERR_BAD_ARG
