@@ -1,10 +1,14 @@
-// Distillation from a teacher's top classes: the loss and its gradient.
+// Distillation from a teacher's top classes, the loss and its gradient: rows of neighbouring classes.
 //
-// Bytes of the logits, read once (backward: once more out of the L2 or L1, and the gradient written).  The gradient of a
-// class outside of the list is dloss * scale * p_c * (Q - q_r / p_r), which the group writes everywhere; the list's logits
-// are read before, and their gradients written over that.  With rest the pass over the row leaves the list's classes out
-// (a byte of mask per vector in shared memory) and sums the others alone, against their own maximum: p_r is then exact
+// Bytes of the logits, read once (backward: once more out of shared memory or the L2, and the gradient written).  The
+// gradient of a class outside of the list is dloss * scale * p_c * (Q - q_r / p_r), which is written everywhere; the list's
+// logits are read before, and their gradients written over that.  With rest the pass over the row leaves the list's classes
+// out (a byte of mask per vector in shared memory) and sums the others alone, against their own maximum: p_r is then exact
 // however little of the row it is, and the row's sum is theirs and that of the list, each class of it once.
+//
+// 4096 x 65536 bf16 (537 MB, 83 us at the copy rate): loss 86 to 102 us for lists of 1 to 128 classes.  Gradient (166): 221 with
+// one class, 238 with 64 and the rest; 1001 x 50001 fp32 (62): 95; 2048 x 32000 bf16 (41): 63.  Two exponentials per
+// element (119 us of the special units for the first) and the second pass's way through shared memory beside the copies.
 #include <cooperative_groups.h>
 
 #include "distill.cuh"

@@ -1,7 +1,9 @@
 // Distillation with a thread per position: few classes in neighbouring elements, or classes in planes.
 //
 // Up to 32 classes and eight entries: the rows of 128 positions in shared memory, a thread's row and list in registers, the
-// gradient back into the tile, where the entries' classes are written over it, and out by vectors.
+// gradient back into the tile, where the entries' classes are written over it, and out by vectors.  2,097,152 pixels of 19 bf16
+// classes with four entries each (243 MB, 38 us at the copy rate): 96 us, by instructions (1080 per 32 pixels) and 42 % of the warps;
+// with the lists read from memory wherever they are needed it took 142.
 #include "distill.cuh"
 
 namespace adk {
