@@ -172,7 +172,7 @@ __global__ void __launch_bounds__(kPositions) distill_by_position(DistillP p) {
     }
     if (r < p.x.rows) {
       const uint32_t at = threadIdx.x * tile_pitch<T, TM>(C);
-      const Position<T, MODE> x = {MODE ? tile + at : (const T*)p.logits + p.x.offset(r), p.x.step, C};
+      const Position<T, MODE> x = {MODE ? tile + at : (const T*)p.logits + p.x.offset(r), (uint32_t)(p.x.step * sizeof(T)), C};
       const uint32_t* cls = p.top_class + r * k;
       const float* t = p.top_logit + r * k;
       auto listed = [&](uint32_t c) { return bits[(c >> 5) * kPositions] >> (c & 31) & 1u; };
@@ -236,8 +236,8 @@ __global__ void __launch_bounds__(kPositions) distill_by_position(DistillP p) {
         }
       if (p.loss) p.loss[r] = d.some ? loss + 0.f * d.L : 0.f;
       if constexpr (BWD) {
-        const Position<T, MODE> o = {MODE ? tile + at : (T*)p.dlogits + p.g.offset(r), p.g.step, C};
-        const Position<T, MODE> old = {MODE ? olds + at : (T*)p.dlogits + p.g.offset(r), p.g.step, C};
+        const Position<T, MODE> o = {MODE ? tile + at : (T*)p.dlogits + p.g.offset(r), (uint32_t)(p.g.step * sizeof(T)), C};
+        const Position<T, MODE> old = {MODE ? olds + at : (T*)p.dlogits + p.g.offset(r), (uint32_t)(p.g.step * sizeof(T)), C};
         const float f = p.dloss[r] * p.scale, coef = f * d.out;
         // the classes outside of the list; those of the list keep their logits for the loop behind it
         for (uint32_t c = 0; c < C; c += 8) {

@@ -61,11 +61,25 @@ __device__ uint32_t kth_share(const uint32_t (&kv)[8], uint32_t k) {
     return t;
   }
   uint32_t t = 0;
-  for (uint32_t bit = 1u << (31 - SHIFT); bit; bit >>= 1) {
-    uint32_t n = 0;
+  if (k <= 32) {   // of the lanes' two largest, bit by bit
+    uint32_t a = 0, b = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) n += (kv[i] >> SHIFT) >= (t | bit);
-    if (__reduce_add_sync(0xffffffffu, n) >= k) t |= bit;
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t q = kv[i] >> SHIFT;
+      b = max(b, min(a, q));
+      a = max(a, q);
+    }
+    for (uint32_t bit = 1u << (31 - SHIFT); bit; bit >>= 1) {
+      const uint32_t u = t | bit;
+      if (__popc(__ballot_sync(0xffffffffu, a >= u)) + __popc(__ballot_sync(0xffffffffu, b >= u)) >= (int)k) t = u;
+    }
+  } else {
+    for (uint32_t bit = 1u << (31 - SHIFT); bit; bit >>= 1) {
+      uint32_t n = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) n += (kv[i] >> SHIFT) >= (t | bit);
+      if (__reduce_add_sync(0xffffffffu, n) >= k) t |= bit;
+    }
   }
   return t == 0 ? 0u : SHIFT ? t << SHIFT | (t >> (31 - SHIFT) ? 0u : (1u << SHIFT) - 1) : t;   // the bits that a key's sign tells
 }
@@ -778,7 +792,7 @@ static int launch_rows(const LogprobP& p, cudaStream_t s) {
     }
   }
   auto kernel = logprob_rows<NT, T, ENT, RANK, TOP, BWD>;
-  const uint32_t n = NT == 32 ? 1 : row_parts(p.x.rows, bytes), slots = NT == 32 ? 0 : feed_slots(bytes, n, BWD ? kMostFeed : 0);
+  const uint32_t n = NT == 32 ? 1 : row_parts(p.x.rows, bytes), slots = NT == 32 ? 0 : feed_slots(bytes, n, BWD || TOP ? kMostFeed : 0);
   const size_t keys = TOP ? (NT == 32 ? kRowWarps * list : list + (n > 1 ? n * p.top : 0)) : 0;
   const size_t smem = slots * Feed<NT>::kBatch * 16 + keys * sizeof(Key);
   constexpr int most = (int)(NT == 32 ? sizeof(Key) * kRowWarps * (kMostTop + TopMem::room(kMostTop)) : kMostFeed + sizeof(Key) * (9 * kMostTop + TopMem::room(kMostTop)));

@@ -276,17 +276,27 @@ __device__ __forceinline__ void sum_classes(const P& x, Part& a, uint32_t lo, ui
     for (int i = 0; i < 8; ++i) f[i] = next[i];
     if (c + 8 < hi) x.batch(c + 8, hi, next);   // on its way while this one is worked on
     a.reach<ENT>(fmaxf(fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3])), fmaxf(fmaxf(f[4], f[5]), fmaxf(f[6], f[7]))), cs);
-    float S[2] = {0.f, 0.f}, E[2] = {0.f, 0.f};
+    const F2 cs2 = pair(cs, cs), mc2 = pair(-a.mc, -a.mc);
+    F2 S[2] = {0, 0}, E[2] = {0, 0};
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      float u = fmaf(f[i], cs, -a.mc);
-      if (ENT) u = above_nothing(u);
-      const float e = exp2_fast(u);
-      S[i & 1] += e;
-      if (ENT) E[i & 1] = fmaf(e, u, E[i & 1]);
+    for (int i = 0; i < 8; i += 2) {
+      F2 z = fma2(pair(f[i], f[i + 1]), cs2, mc2);
+      float2 q = halves(z);
+      if (ENT) {
+        q.x = above_nothing(q.x);
+        q.y = above_nothing(q.y);
+        z = pair(q.x, q.y);
+      }
+      const F2 e = pair(exp2_fast(q.x), exp2_fast(q.y));
+      S[i / 2 & 1] = add2(S[i / 2 & 1], e);
+      if (ENT) E[i / 2 & 1] = fma2(e, z, E[i / 2 & 1]);
     }
-    a.S += S[0] + S[1];
-    if (ENT) a.E += E[0] + E[1];
+    const float2 s = halves(add2(S[0], S[1]));
+    a.S += s.x + s.y;
+    if (ENT) {
+      const float2 e = halves(add2(E[0], E[1]));
+      a.E += e.x + e.y;
+    }
     also(c, f);
   }
 }
@@ -332,7 +342,7 @@ __global__ void __launch_bounds__(kPositions) logprob_positions_fwd(const __grid
       copy_tile<T>(MODE == 2, (const T*)p.logits, p.x, r0, (uint32_t)(p.x.rows - r0 < N ? p.x.rows - r0 : N), tile);
       __syncthreads();
     }
-    const Position<T, MODE> x = {MODE ? tile + at * tile_pitch<T, MODE ? MODE : 1>(C) : (const T*)p.logits + (mine ? p.x.offset(r) : 0), p.x.step, C};
+    const Position<T, MODE> x = {MODE ? tile + at * tile_pitch<T, MODE ? MODE : 1>(C) : (const T*)p.logits + (mine ? p.x.offset(r) : 0), (uint32_t)(p.x.step * sizeof(T)), C};
     const uint32_t l = p.label && mine ? p.label[r] : kNoClass;
     const float xl = mine && l < C ? x.get(l) : 0.f;
     Part a;
@@ -416,8 +426,8 @@ __global__ void __launch_bounds__(kPositions) logprob_positions_grad(const __gri
     }
     const uint32_t place = at * tile_pitch<T, TM>(C);
     T* out = (T*)p.dlogits + (MODE == 0 && mine ? p.g.offset(r) : 0);
-    const Position<T, MODE> x = {MODE ? tile + place : (const T*)p.logits + (mine ? p.x.offset(r) : 0), p.x.step, C};
-    const Position<T, MODE> o = {MODE ? tile + place : out, p.g.step, C}, old = {MODE ? olds + place : out, p.g.step, C};
+    const Position<T, MODE> x = {MODE ? tile + place : (const T*)p.logits + (mine ? p.x.offset(r) : 0), (uint32_t)(p.x.step * sizeof(T)), C};
+    const Position<T, MODE> o = {MODE ? tile + place : out, (uint32_t)(p.g.step * sizeof(T)), C}, old = {MODE ? olds + place : out, (uint32_t)(p.g.step * sizeof(T)), C};
     const uint32_t l = p.label && mine ? p.label[r] : kNoClass;
     const float xl = mine && l < C ? x.get(l) : 0.f;
     Factors f;
@@ -436,6 +446,8 @@ __global__ void __launch_bounds__(kPositions) logprob_positions_grad(const __gri
         const float H = s.entropy(a.E), mc = s.mc;
         if (part == 0) put_row(p, s, r, H, l, xl);
         f.set<ENT>(p, s, H);
+        float gl = 0.f;
+        if (l >= lo && l < hi) gl = f.grad<ENT>(xl, p.cs, mc) + f.dl + (p.accumulate ? old.get(l) : 0.f);
         float next[8];
         x.batch(lo, hi, next);
         for (uint32_t c = lo; c < hi; c += 8) {
@@ -443,13 +455,30 @@ __global__ void __launch_bounds__(kPositions) logprob_positions_grad(const __gri
 #pragma unroll
           for (int i = 0; i < 8; ++i) h[i] = next[i];
           if (c + 8 < hi) x.batch(c + 8, hi, next);
+          const F2 cs2 = pair(p.cs, p.cs), mc2 = pair(-mc, -mc), c0 = pair(f.c0, f.c0), c1 = pair(f.c1, f.c1);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            h[i] = f.grad<ENT>(h[i], p.cs, mc);
-            if (c + i == l) h[i] += f.dl;
-            if (c + i < hi) o.set(c + i, p.accumulate ? h[i] + old.get(c + i) : h[i]);
+          for (int i = 0; i < 8; i += 2) {
+            F2 z = fma2(pair(h[i], h[i + 1]), cs2, mc2);
+            float2 q = halves(z);
+            if (ENT) {
+              q.x = above_nothing(q.x);
+              q.y = above_nothing(q.y);
+              z = pair(q.x, q.y);
+            }
+            const float2 g = halves(mul2(pair(exp2_fast(q.x), exp2_fast(q.y)), ENT ? fma2(z, c1, c0) : c0));
+            h[i] = g.x;
+            h[i + 1] = g.y;
+          }
+          if (c + 8 <= hi && !p.accumulate) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) o.set(c + i, h[i]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              if (c + i < hi) o.set(c + i, p.accumulate ? h[i] + old.get(c + i) : h[i]);
           }
         }
+        if (l >= lo && l < hi) o.set(l, gl);   // over what the loop wrote
       }
     }
     __syncthreads();

@@ -683,9 +683,10 @@ __device__ void plain_sums(Group<NT>& g, const T* x, int64_t st, uint32_t C, flo
 template <typename T, int MODE>
 struct Position {
   const T* x;
-  int64_t step;   // MODE 0
+  uint32_t step;   // MODE 0: bytes from one class to the next
   uint32_t C;
-  __device__ float get(uint32_t c) const { return ld_f(MODE == 0 ? x + c * step : x + c); }
+  __device__ const T* at(uint32_t c) const { return MODE == 0 ? (const T*)((const char*)x + (uint64_t)c * step) : x + c; }
+  __device__ float get(uint32_t c) const { return ld_f(at(c)); }
   // classes [c, c + 8), -inf from `hi` on (MODE 2: hi is C, a multiple of the vector)
   __device__ void batch(uint32_t c, uint32_t hi, float (&f)[8]) const {
     constexpr uint32_t V = Vec<T>::V;
@@ -700,7 +701,7 @@ struct Position {
       for (uint32_t i = 0; i < 8; ++i) f[i] = c + i < hi ? get(c + i) : -INFINITY;
     }
   }
-  __device__ void set(uint32_t c, float v) const { st_f(const_cast<T*>(MODE == 0 ? x + c * step : x + c), v); }
+  __device__ void set(uint32_t c, float v) const { st_f(const_cast<T*>(at(c)), v); }
 };
 constexpr uint32_t kPositions = 128;         // of a block
 constexpr uint32_t kFewClasses = 64;         // of rows in shared memory
@@ -818,7 +819,7 @@ template <typename T, int MODE> inline size_t tile_bytes(uint32_t C) {
 // The mode that a call's rows are for; -1: none of them
 template <typename T>
 inline int position_mode(const Rows& g, const void* x) {
-  if (g.HW) return g.C <= 0xffffu ? 0 : -1;
+  if (g.HW) return g.C <= 0xffffu && (uint64_t)g.step * sizeof(T) <= 0xffffffffu ? 0 : -1;
   if (g.step != 1 || g.C > kFewClasses) return -1;
   return g.C % Vec<T>::V == 0 && g.pitch % Vec<T>::V == 0 && aligned_to(x, 16) ? 2 : 1;
 }
