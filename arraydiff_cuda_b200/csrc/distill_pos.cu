@@ -8,9 +8,11 @@
 
 namespace adk {
 
-// CM: C rounded up to a multiple of 4.  K: room for the entries.  vec: rows of whole vectors, an odd number of them apart in shared memory.
-template <typename T, int CM, int K, bool BWD>
+// CM: C rounded up to a multiple of 4.  K: room for the entries.  PLANES: the classes come from planes as they lie; else from rows
+// in shared memory, vec: of whole vectors, an odd number of them apart.
+template <typename T, int CM, int K, bool BWD, bool PLANES>
 __global__ void __launch_bounds__(kPositions, 7) distill_few(DistillP p, int vec) {
+  typedef Position<T, PLANES ? 0 : 1> X;
   grid_dependency();
   extern __shared__ __align__(16) uint8_t tiles[];
   __shared__ uint32_t all_cls[kPositions * K];
@@ -27,13 +29,17 @@ __global__ void __launch_bounds__(kPositions, 7) distill_few(DistillP p, int vec
     }
     const float f = BWD && threadIdx.x < n ? p.dloss[r] * p.scale : 0.f;
     float shift = p.rest && p.top_lse && threadIdx.x < n ? (float)(p.top_lse[r] * kLog2e) : 0.f;
-    copy_tile<T>(vec != 0, (const T*)p.logits, p.x, r0, n, tile);
-    if (BWD && p.accumulate) copy_tile<T>(vec != 0, (const T*)p.dlogits, p.g, r0, n, olds);
+    if (!PLANES) {
+      copy_tile<T>(vec != 0, (const T*)p.logits, p.x, r0, n, tile);
+      if (BWD && p.accumulate) copy_tile<T>(vec != 0, (const T*)p.dlogits, p.g, r0, n, olds);
+    }
     __syncthreads();
     if (threadIdx.x < n) {
-      const Position<T, 1> x = {tile + threadIdx.x * tp, 1, C}, old = {olds + threadIdx.x * tp, 1, C};
+      const X x = {PLANES ? (const T*)p.logits + p.x.offset(r) : tile + threadIdx.x * tp, (uint32_t)(p.x.step * sizeof(T)), C};
+      const X o = {PLANES ? (T*)p.dlogits + (BWD ? p.g.offset(r) : 0) : tile + threadIdx.x * tp, (uint32_t)(p.g.step * sizeof(T)), C};
+      const X old = {PLANES ? o.x : olds + threadIdx.x * tp, o.step, C};
       float v[CM];
-      load_few<T, CM>(x.x, C, vec != 0, v);
+      load_few<T, CM>(x, vec != 0, v);
       // the list
       uint32_t cls[K], bits = 0, entries = 0;
       float a[K], xs[K], am = -INFINITY, mk = -INFINITY;
@@ -134,14 +140,14 @@ __global__ void __launch_bounds__(kPositions, 7) distill_few(DistillP p, int vec
           for (uint32_t c = 0; c < CM; ++c)
             if (c + 4 < CM || c < C) v[c] += old.get(c);
         }
-        store_few<T, CM>(const_cast<T*>(x.x), C, vec != 0, v);
+        store_few<T, CM>(o, vec != 0, v);
 #pragma unroll
         for (uint32_t j = 0; j < K; ++j)
-          if (j < k && cls[j] < C) x.set(cls[j], g[j]);
+          if (j < k && cls[j] < C) o.set(cls[j], g[j]);
       }
     }
     __syncthreads();
-    if (BWD) {
+    if (BWD && !PLANES) {
       write_tile<T>(vec != 0, (T*)p.dlogits, p.g, r0, n, tile);
       __syncthreads();
     }
@@ -271,12 +277,14 @@ __global__ void __launch_bounds__(kPositions) distill_by_position(DistillP p) {
   }
 }
 
+// mode: as position_mode() has it
 template <typename T, int CM, int K, bool BWD>
-static int launch_few(const DistillP& p, int vec, cudaStream_t s) {
+static int launch_few(const DistillP& p, int mode, cudaStream_t s) {
   if constexpr (CM <= 32) {
-    if (p.x.C > CM) return launch_few<T, CM + 4, K, BWD>(p, vec, s);
-    const size_t smem = (vec ? tile_bytes<T, 2>(p.x.C) : tile_bytes<T, 1>(p.x.C)) * (BWD && p.accumulate ? 2 : 1);   // 36 KB at most, beside 8 KB of lists
-    launch(distill_few<T, CM, K, BWD>, position_blocks(p.x.rows), kPositions, smem, s, p, vec);
+    if (p.x.C > CM) return launch_few<T, CM + 4, K, BWD>(p, mode, s);
+    const size_t smem = (mode == 0 ? 0 : mode == 2 ? tile_bytes<T, 2>(p.x.C) : tile_bytes<T, 1>(p.x.C)) * (BWD && p.accumulate ? 2 : 1);   // 36 KB at most, beside 8 KB of lists
+    if (mode == 0) launch(distill_few<T, CM, K, BWD, true>, position_blocks(p.x.rows), kPositions, smem, s, p, 0);
+    else launch(distill_few<T, CM, K, BWD, false>, position_blocks(p.x.rows), kPositions, smem, s, p, mode == 2);
     return AD_OK;
   } else return AD_ERR_UNSUPPORTED;
 }
@@ -302,9 +310,9 @@ int distill_positions(const DistillP& p, cudaStream_t s) {
   if (mode > 0 && BWD && p.g.step != 1) mode = -1;
   if (mode == 2 && BWD && position_mode<T>(p.g, p.dlogits) != 2) mode = 1;
   if (mode < 0) return AD_ERR_UNSUPPORTED;
+  if (p.x.C <= 32 && p.top <= 4) return launch_few<T, 4, 4, BWD>(p, mode, s);
+  if (p.x.C <= 32 && p.top <= 8) return launch_few<T, 4, 8, BWD>(p, mode, s);
   if (mode == 0) return launch_positions<T, 0, BWD>(p, s);
-  if (p.x.C <= 32 && p.top <= 4) return launch_few<T, 4, 4, BWD>(p, mode == 2, s);
-  if (p.x.C <= 32 && p.top <= 8) return launch_few<T, 4, 8, BWD>(p, mode == 2, s);
   return mode == 1 ? launch_positions<T, 1, BWD>(p, s) : launch_positions<T, 2, BWD>(p, s);
 }
 template int distill_positions<float, false>(const DistillP&, cudaStream_t);

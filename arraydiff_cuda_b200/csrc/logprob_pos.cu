@@ -131,9 +131,11 @@ __device__ __noinline__ void plain_gradient(const LogprobP& p, P x, P o, P old, 
 }
 
 // ---------------------------------------------------------------- up to 32 classes: a row in registers
-// CM: C rounded up to a multiple of 4.  vec: rows of whole vectors, an odd number of them apart in shared memory.
-template <typename T, int CM, int KT>
+// CM: C rounded up to a multiple of 4.  PLANES: the classes come from planes as they lie; else from rows in shared memory,
+// vec: of whole vectors, an odd number of them apart.
+template <typename T, int CM, int KT, bool PLANES>
 __global__ void __launch_bounds__(kPositions) logprob_few(const __grid_constant__ LogprobP p, int vec) {
+  typedef Position<T, PLANES ? 0 : 1> X;
   grid_dependency();
   extern __shared__ __align__(16) uint8_t tiles[];
   __shared__ uint32_t cls[kPositions * KT];
@@ -146,12 +148,12 @@ __global__ void __launch_bounds__(kPositions) logprob_few(const __grid_constant_
     const size_t r0 = blk * kPositions, r = r0 + threadIdx.x;
     const uint32_t n = (uint32_t)(p.x.rows - r0 < kPositions ? p.x.rows - r0 : kPositions);
     const uint32_t l = p.label && threadIdx.x < n ? p.label[r] : kNoClass;
-    copy_tile<T>(vec != 0, (const T*)p.logits, p.x, r0, n, tile);
+    if (!PLANES) copy_tile<T>(vec != 0, (const T*)p.logits, p.x, r0, n, tile);
     __syncthreads();
     if (threadIdx.x < n) {
-      const Position<T, 1> x = {tile + threadIdx.x * (vec ? tile_pitch<T, 2>(C) : C), 1, C};
+      const X x = {PLANES ? (const T*)p.logits + p.x.offset(r) : tile + threadIdx.x * (vec ? tile_pitch<T, 2>(C) : C), (uint32_t)(p.x.step * sizeof(T)), C};
       float v[CM];
-      load_few<T, CM>(x.x, C, vec != 0, v);
+      load_few<T, CM>(x, vec != 0, v);
       const float xl = l < C ? x.get(l) : 0.f;
       Part a;
       sum_few<true, CM>(a, v, p.cs);
@@ -201,8 +203,9 @@ __global__ void __launch_bounds__(kPositions) logprob_few(const __grid_constant_
   }
 }
 
-template <typename T, int CM, bool ENT>
+template <typename T, int CM, bool ENT, bool PLANES>
 __global__ void __launch_bounds__(kPositions) logprob_few_bwd(const __grid_constant__ LogprobP p, int vec) {
+  typedef Position<T, PLANES ? 0 : 1> X;
   grid_dependency();
   extern __shared__ __align__(16) uint8_t tiles[];
   const uint32_t C = p.x.C, tp = vec ? tile_pitch<T, 2>(C) : C;
@@ -214,18 +217,22 @@ __global__ void __launch_bounds__(kPositions) logprob_few_bwd(const __grid_const
     const uint32_t l = p.label && threadIdx.x < n ? p.label[r] : kNoClass;
     Factors f;
     if (threadIdx.x < n) f.fetch(p, r, l);
-    copy_tile<T>(vec != 0, (const T*)p.logits, p.x, r0, n, tile);
-    if (p.accumulate) copy_tile<T>(vec != 0, (const T*)p.dlogits, p.g, r0, n, olds);
-    __syncthreads();
+    if (!PLANES) {
+      copy_tile<T>(vec != 0, (const T*)p.logits, p.x, r0, n, tile);
+      if (p.accumulate) copy_tile<T>(vec != 0, (const T*)p.dlogits, p.g, r0, n, olds);
+      __syncthreads();
+    }
     if (threadIdx.x < n) {
-      const Position<T, 1> x = {tile + threadIdx.x * tp, 1, C}, old = {olds + threadIdx.x * tp, 1, C};
+      const X x = {PLANES ? (const T*)p.logits + p.x.offset(r) : tile + threadIdx.x * tp, (uint32_t)(p.x.step * sizeof(T)), C};
+      const X o = {PLANES ? (T*)p.dlogits + p.g.offset(r) : tile + threadIdx.x * tp, (uint32_t)(p.g.step * sizeof(T)), C};
+      const X old = {PLANES ? o.x : olds + threadIdx.x * tp, o.step, C};
       float v[CM];
-      load_few<T, CM>(x.x, C, vec != 0, v);
+      load_few<T, CM>(x, vec != 0, v);
       const float xl = l < C ? x.get(l) : 0.f;
       Part a;
       sum_few<ENT, CM>(a, v, p.cs);
       if (a.strange(p.cs)) {
-        plain_gradient<ENT>(p, x, x, old, r, l, xl);
+        plain_gradient<ENT>(p, x, o, old, r, l, xl);
       } else {
         RowSums s;
         s.set(a.m, a.mc, a.S, p.cs);
@@ -253,13 +260,15 @@ __global__ void __launch_bounds__(kPositions) logprob_few_bwd(const __grid_const
           for (uint32_t c = 0; c < CM; ++c)
             if (c + 4 < CM || c < C) v[c] += old.get(c);
         }
-        store_few<T, CM>(const_cast<T*>(x.x), C, vec != 0, v);
-        if (l < C) x.set(l, gl);
+        store_few<T, CM>(o, vec != 0, v);
+        if (l < C) o.set(l, gl);
       }
     }
-    __syncthreads();
-    write_tile<T>(vec != 0, (T*)p.dlogits, p.g, r0, n, tile);
-    __syncthreads();
+    if (!PLANES) {
+      __syncthreads();
+      write_tile<T>(vec != 0, (T*)p.dlogits, p.g, r0, n, tile);
+      __syncthreads();
+    }
   }
 }
 
@@ -322,7 +331,7 @@ __device__ __forceinline__ void join_warps(Part& a, Part (&all)[G][32], float cs
 }
 
 template <typename T, int MODE, int KT, int G>
-__global__ void __launch_bounds__(kPositions) logprob_positions_fwd(const __grid_constant__ LogprobP p) {
+__global__ void __launch_bounds__(kPositions, 8) logprob_positions_fwd(const __grid_constant__ LogprobP p) {
   grid_dependency();
   extern __shared__ __align__(16) uint8_t tiles[];
   __shared__ Part sums[G][32];
@@ -405,7 +414,7 @@ __global__ void __launch_bounds__(kPositions) logprob_positions_fwd(const __grid
 }
 
 template <typename T, int MODE, bool ENT, int G>
-__global__ void __launch_bounds__(kPositions) logprob_positions_grad(const __grid_constant__ LogprobP p) {
+__global__ void __launch_bounds__(kPositions, 10) logprob_positions_grad(const __grid_constant__ LogprobP p) {
   grid_dependency();
   extern __shared__ __align__(16) uint8_t tiles[];
   __shared__ Part sums[G][32];
@@ -500,18 +509,21 @@ static int go(void (*kernel)(K...), const LogprobP& p, uint32_t places, size_t s
   launch(kernel, position_blocks(p.x.rows, places), kPositions, smem, s, p, args...);
   return AD_OK;
 }
+// mode: as position_mode() has it
 template <typename T, int CM, int KT>
-static int go_few(const LogprobP& p, int vec, cudaStream_t s) {
+static int go_few(const LogprobP& p, int mode, cudaStream_t s) {
   if constexpr (CM <= 32) {
-    if (p.x.C > CM) return go_few<T, CM + 4, KT>(p, vec, s);
-    return go(logprob_few<T, CM, KT>, p, kPositions, vec ? tile_bytes<T, 2>(p.x.C) : tile_bytes<T, 1>(p.x.C), s, vec);
+    if (p.x.C > CM) return go_few<T, CM + 4, KT>(p, mode, s);
+    if (mode == 0) return go(logprob_few<T, CM, KT, true>, p, kPositions, 0, s, 0);
+    return go(logprob_few<T, CM, KT, false>, p, kPositions, mode == 2 ? tile_bytes<T, 2>(p.x.C) : tile_bytes<T, 1>(p.x.C), s, mode == 2);
   } else return AD_ERR_UNSUPPORTED;
 }
 template <typename T, int CM, bool ENT>
-static int go_few_bwd(const LogprobP& p, int vec, cudaStream_t s) {
+static int go_few_bwd(const LogprobP& p, int mode, cudaStream_t s) {
   if constexpr (CM <= 32) {
-    if (p.x.C > CM) return go_few_bwd<T, CM + 4, ENT>(p, vec, s);
-    return go(logprob_few_bwd<T, CM, ENT>, p, kPositions, (vec ? tile_bytes<T, 2>(p.x.C) : tile_bytes<T, 1>(p.x.C)) * (p.accumulate ? 2 : 1), s, vec);
+    if (p.x.C > CM) return go_few_bwd<T, CM + 4, ENT>(p, mode, s);
+    if (mode == 0) return go(logprob_few_bwd<T, CM, ENT, true>, p, kPositions, 0, s, 0);
+    return go(logprob_few_bwd<T, CM, ENT, false>, p, kPositions, (mode == 2 ? tile_bytes<T, 2>(p.x.C) : tile_bytes<T, 1>(p.x.C)) * (p.accumulate ? 2 : 1), s, mode == 2);
   } else return AD_ERR_UNSUPPORTED;
 }
 template <typename T, int MODE, int G>
@@ -533,11 +545,11 @@ template <typename T>
 int logprob_positions(const LogprobP& p, cudaStream_t s) {
   const int mode = position_mode<T>(p.x, p.logits);
   if (mode < 0) return AD_ERR_UNSUPPORTED;
-  if (mode == 0) return p.x.C >= kSharedPlanes ? go_fwd<T, 0, 4>(p, s) : go_fwd<T, 0, 1>(p, s);
   if (p.x.C <= 32) {
-    if (p.top <= 1 || p.top > 8) return go_few<T, 4, 1>(p, mode == 2, s);
-    return p.top <= 3 ? go_few<T, 4, 3>(p, mode == 2, s) : go_few<T, 4, 8>(p, mode == 2, s);
+    if (p.top <= 1 || p.top > 8) return go_few<T, 4, 1>(p, mode, s);
+    return p.top <= 3 ? go_few<T, 4, 3>(p, mode, s) : go_few<T, 4, 8>(p, mode, s);
   }
+  if (mode == 0) return go_fwd<T, 0, 4>(p, s);
   return mode == 1 ? go_fwd<T, 1, 1>(p, s) : go_fwd<T, 2, 1>(p, s);
 }
 template <typename T>
@@ -547,8 +559,8 @@ int logprob_positions_bwd(const LogprobP& p, cudaStream_t s) {
   if (mode > 0 && p.g.step != 1) mode = -1;
   if (mode == 2 && position_mode<T>(p.g, p.dlogits) != 2) mode = 1;
   if (mode < 0) return AD_ERR_UNSUPPORTED;
-  if (mode == 0) return p.x.C >= kSharedPlanes ? go_bwd<T, 0, 4>(p, s) : go_bwd<T, 0, 1>(p, s);
-  if (p.x.C <= 32) return p.entropy || p.dentropy ? go_few_bwd<T, 4, true>(p, mode == 2, s) : go_few_bwd<T, 4, false>(p, mode == 2, s);
+  if (p.x.C <= 32) return p.entropy || p.dentropy ? go_few_bwd<T, 4, true>(p, mode, s) : go_few_bwd<T, 4, false>(p, mode, s);
+  if (mode == 0) return go_bwd<T, 0, 4>(p, s);
   return mode == 1 ? go_bwd<T, 1, 1>(p, s) : go_bwd<T, 2, 1>(p, s);
 }
 template int logprob_positions<float>(const LogprobP&, cudaStream_t);

@@ -705,7 +705,6 @@ struct Position {
 };
 constexpr uint32_t kPositions = 128;         // of a block
 constexpr uint32_t kFewClasses = 64;         // of rows in shared memory
-constexpr uint32_t kSharedPlanes = 16;       // classes in planes from which four warps share them
 // MODE 1, 2: elements from one row to the next in shared memory
 template <typename T, int MODE> __host__ __device__ inline uint32_t tile_pitch(uint32_t C) { return MODE == 2 ? (C / Vec<T>::V | 1u) * Vec<T>::V : C; }
 template <typename T>
@@ -747,15 +746,15 @@ __device__ __forceinline__ void write_tile(bool vec, T* to, const Rows& g, size_
   }
 }
 // A row of up to CM classes (C rounded up to a multiple of 4) in registers, -inf behind the last
-template <typename T, int CM>
-__device__ __forceinline__ void load_few(const T* x, uint32_t C, bool vec, float (&v)[CM]) {
+template <typename T, int CM, int MODE>
+__device__ __forceinline__ void load_few(const Position<T, MODE>& x, bool vec, float (&v)[CM]) {
   constexpr int V = Vec<T>::V;
-  if constexpr (CM % V == 0) {
+  if constexpr (CM % V == 0 && MODE != 0) {
     if (vec) {
 #pragma unroll
       for (int c = 0; c < CM; c += V) {
         float f[V];
-        Vec<T>::unpack(*(const uint4*)(x + c), f);
+        Vec<T>::unpack(*(const uint4*)(x.x + c), f);
 #pragma unroll
         for (int i = 0; i < V; ++i) v[c + i] = f[i];
       }
@@ -763,26 +762,26 @@ __device__ __forceinline__ void load_few(const T* x, uint32_t C, bool vec, float
     }
   }
 #pragma unroll
-  for (uint32_t c = 0; c < CM; ++c) v[c] = c + 4 < CM || c < C ? ld_f(x + c) : -INFINITY;
+  for (uint32_t c = 0; c < CM; ++c) v[c] = c + 4 < CM || c < x.C ? x.get(c) : -INFINITY;
 }
-template <typename T, int CM>
-__device__ __forceinline__ void store_few(T* x, uint32_t C, bool vec, const float (&v)[CM]) {
+template <typename T, int CM, int MODE>
+__device__ __forceinline__ void store_few(const Position<T, MODE>& x, bool vec, const float (&v)[CM]) {
   constexpr int V = Vec<T>::V;
-  if constexpr (CM % V == 0) {
+  if constexpr (CM % V == 0 && MODE != 0) {
     if (vec) {
 #pragma unroll
       for (int c = 0; c < CM; c += V) {
         float f[V];
 #pragma unroll
         for (int i = 0; i < V; ++i) f[i] = v[c + i];
-        *(uint4*)(x + c) = Vec<T>::pack(f);
+        *(uint4*)const_cast<T*>(x.x + c) = Vec<T>::pack(f);
       }
       return;
     }
   }
 #pragma unroll
   for (uint32_t c = 0; c < CM; ++c)
-    if (c + 4 < CM || c < C) st_f(x + c, v[c]);
+    if (c + 4 < CM || c < x.C) x.set(c, v[c]);
 }
 template <bool ENT, int CM>
 __device__ __forceinline__ void sum_few(Part& a, const float (&v)[CM], float cs) {
