@@ -306,7 +306,7 @@ static int launch_positions(const DistillP& p, cudaStream_t s) {
 template <typename T, bool BWD>
 int distill_positions(const DistillP& p, cudaStream_t s) {
   int mode = position_mode<T>(p.x, p.logits);
-  if (mode == 0 && (p.x.C > kMostBits || (BWD && p.g.HW == 0))) mode = -1;   // the gradient of an image of one position, packed
+  if (mode == 0 && (p.x.C > kMostBits || (BWD && (p.g.HW == 0 || (uint64_t)p.g.step * sizeof(T) > 0xffffffffu)))) mode = -1;   // the gradient of an image of one position, packed
   if (mode > 0 && BWD && p.g.step != 1) mode = -1;
   if (mode == 2 && BWD && position_mode<T>(p.g, p.dlogits) != 2) mode = 1;
   if (mode < 0) return AD_ERR_UNSUPPORTED;

@@ -555,7 +555,7 @@ int logprob_positions(const LogprobP& p, cudaStream_t s) {
 template <typename T>
 int logprob_positions_bwd(const LogprobP& p, cudaStream_t s) {
   int mode = position_mode<T>(p.x, p.logits);
-  if (mode == 0 && p.g.HW == 0) mode = -1;   // the gradient of an image of one position, packed
+  if (mode == 0 && (p.g.HW == 0 || (uint64_t)p.g.step * sizeof(T) > 0xffffffffu)) mode = -1;   // the gradient of an image of one position, packed
   if (mode > 0 && p.g.step != 1) mode = -1;
   if (mode == 2 && position_mode<T>(p.g, p.dlogits) != 2) mode = 1;
   if (mode < 0) return AD_ERR_UNSUPPORTED;
