@@ -680,7 +680,8 @@ static int launch_rows(const DistillP& p, uint32_t n, size_t mask, cudaStream_t 
     const size_t one = bytes(plan.parts);
     if (one <= kMostMask / 2 && stream_worth<W>(p.x.rows, plan.parts)) {
       static StreamLaunch shared;
-      return launch_stream(distill_stream<T, REST, BWD>, shared, Crew<W>::kThreads, p.x.rows, plan.parts, plan.bytes + 2 * one, s, p, plan, (uint32_t)one);
+      const int rc = launch_stream(distill_stream<T, REST, BWD>, shared, Crew<W>::kThreads, p.x.rows, plan.parts, plan.bytes + 2 * one, s, p, plan, (uint32_t)one);
+      if (rc != AD_ERR_UNSUPPORTED) return rc;
     }
   }
   auto kernel = distill_rows<NT, T, REST, BWD>;

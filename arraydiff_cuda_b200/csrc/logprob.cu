@@ -107,6 +107,16 @@ __device__ __forceinline__ void sort_candidates(const TopMem& t, uint32_t n, uin
       if (key[q] >= least && key[q] && at[q] < k) t.list[at[q]] = key[q];
   }
 }
+// One warp: the k-th of n candidates, bit by bit; 0: fewer
+__device__ __forceinline__ Key kth_candidate(const TopMem& t, uint32_t n, uint32_t k) {
+  Key least = 0;
+  for (Key bit = 1ull << 63; bit; bit >>= 1) {
+    uint32_t m = 0;
+    for (uint32_t i = threadIdx.x & 31; i < n; i += 32) m += t.cand[i] >= (least | bit);
+    if (__reduce_add_sync(0xffffffffu, m) >= k) least |= bit;
+  }
+  return least;
+}
 __device__ void sort_candidates(const TopMem& t, uint32_t n, uint32_t k) {
   const uint32_t lane = threadIdx.x & 31;
   __syncwarp();
@@ -114,12 +124,8 @@ __device__ void sort_candidates(const TopMem& t, uint32_t n, uint32_t k) {
   if (n <= 32) {
     sort_candidates<1>(t, n, k, 0);
   } else {
-    if (n > 64 + 2 * k) {   // many equal or clustered ones: the k-th first, bit by bit, and only those up to it
-      for (Key bit = 1ull << 63; bit; bit >>= 1) {
-        uint32_t m = 0;
-        for (uint32_t i = lane; i < n; i += 32) m += t.cand[i] >= (least | bit);
-        if (__reduce_add_sync(0xffffffffu, m) >= k) least |= bit;
-      }
+    if (n > 64 + 2 * k) {   // many equal or clustered ones: the k-th first, and only those up to it
+      least = kth_candidate(t, n, k);
       uint32_t kept = 0;
       for (uint32_t i0 = 0; i0 < n; i0 += 32) {
         const Key key = i0 + lane < n ? t.cand[i0 + lane] : 0;
@@ -163,7 +169,7 @@ struct Maxima {
 constexpr uint32_t kMostSlots = 8;
 __device__ __forceinline__ uint32_t half_key(uint32_t h) { return h & 0x8000u ? 0xffffu ^ h : h | 0x8000u; }   // value_key >> 16
 
-constexpr uint32_t kWork = 1024;   // words of 16 bits that a selection works with
+constexpr uint32_t kWork = 512;   // words of 16 bits that a selection works with: shares, and slots of 32 of them
 template <int N> struct Loads { static constexpr int value = N; };
 
 // One warp: a strip's list out of its 256 shares, of which lane i has number 32 j + i in kv[j]: the key of its largest value, 0
@@ -176,11 +182,13 @@ __device__ void select_top(const TopMem& t, uint32_t k, const uint32_t (&kv)[8],
   constexpr int V = X::V;
   Group<32> g(nullptr);
   const uint32_t lane = g.tid;
-  const uint32_t tv = kth_share<X::kKeyShift>(kv, k);
-  const float bound = tv ? key_value(tv) : -INFINITY;
+  uint32_t tv = kth_share<X::kKeyShift>(kv, k);
   const uint32_t nv = b.ve - b.vb, per = mx.m ? mx.slots : (nv + 255) / 256;
-  // all elements of the shares that reach the bound; where that is too many, those above it, and of the equal ones the first
-  for (int strict = 0; strict < 2; ++strict) {
+  // All elements of the shares that reach the bound.  Where there is no room for them the bound rises to the k-th of those
+  // found so far; where it cannot, because so many equal it, only those above it are taken, and of the equal ones the first.
+  bool strict = false;
+  for (int tries = 0; tries < 64; ++tries) {
+    const float bound = tv ? key_value(tv) : -INFINITY;
     auto reaches = [&](float v) { return strict ? v > bound : v >= bound; };
     uint32_t ns = 0, n = 0, mine = 0;
 #pragma unroll
@@ -188,38 +196,23 @@ __device__ void select_top(const TopMem& t, uint32_t k, const uint32_t (&kv)[8],
     each_bit(mine, ns, [&](uint32_t i, uint32_t at) { work[at] = (uint16_t)(i * 32 + lane); });
     __syncwarp();
     const uint32_t wide = per <= 1 ? 0 : 32 - __clz(per - 1);   // a share's vectors as a power of two
-    uint32_t vectors = ns << wide;   // of the shares, or (maxima) of their slots that reach it
     uint16_t* list = work + 256;
-    if (mx.m) {
-      uint32_t found = 0;
-      for (uint32_t i0 = 0; i0 < ns; i0 += 32) {
-        uint32_t slots = 0;
-        const uint32_t share = i0 + lane < ns ? work[i0 + lane] : 0;
-        if (i0 + lane < ns)
-          for (uint32_t q = 0; q < per; ++q) slots |= half_key(mx.m[q * 256 + share]) >= tv >> 16 ? 1u << q : 0u;
-        each_bit(slots, found, [&](uint32_t q, uint32_t at) {
-          if (at < kWork - 256) list[at] = (uint16_t)(q * 256 + share);
-        });
-      }
-      if (found > kWork - 256) continue;
-      vectors = found * (4u << mx.shift);
-      __syncwarp();
-    }
-    auto vector_of = [&](uint32_t i) -> uint32_t {
-      if (i >= vectors) return nv;
-      if (mx.m) {
-        const uint32_t e = list[i >> (2 + mx.shift)], sub = i & ((4u << mx.shift) - 1);
-        return (((e >> 8) << (2 + mx.shift)) + sub) * 256 + (e & 255);
-      }
-      return (i & ((1u << wide) - 1)) * 256 + work[i >> wide];
-    };
-    auto look = [&](auto loads, uint32_t i0) {   // so many loads at a time
+    auto look = [&](auto loads, uint32_t i0, uint32_t vectors) {   // so many loads at a time
       constexpr int Q = decltype(loads)::value;
       uint4 w[Q];
       uint32_t at[Q];
 #pragma unroll
       for (int q = 0; q < Q; ++q) {
-        at[q] = vector_of(i0 + q * 32 + lane);
+        const uint32_t i = i0 + q * 32 + lane;
+        at[q] = nv;
+        if (i < vectors) {
+          if (mx.m) {
+            const uint32_t e = list[i >> (2 + mx.shift)], sub = i & ((4u << mx.shift) - 1);
+            at[q] = (((e >> 8) << (2 + mx.shift)) + sub) * 256 + (e & 255);
+          } else {
+            at[q] = (i & ((1u << wide) - 1)) * 256 + work[i >> wide];
+          }
+        }
         w[q] = at[q] < nv ? xv[at[q]] : X::none();
       }
 #pragma unroll
@@ -237,23 +230,43 @@ __device__ void select_top(const TopMem& t, uint32_t k, const uint32_t (&kv)[8],
         });
       }
     };
-    for (uint32_t i0 = 0; i0 < vectors && n <= t.cap;) {
-      if (vectors - i0 <= 32) {
-        look(Loads<1>(), i0);
-        i0 += 32;
-      } else {
-        look(Loads<4>(), i0);
-        i0 += 128;
+    auto look_at = [&](uint32_t vectors) {
+      for (uint32_t i0 = 0; i0 < vectors && n <= t.cap;) {
+        if (vectors - i0 <= 32) {
+          look(Loads<1>(), i0, vectors);
+          i0 += 32;
+        } else {
+          look(Loads<4>(), i0, vectors);
+          i0 += 128;
+        }
       }
+    };
+    if (mx.m) {   // the slots that reach it, of 32 shares at a time
+      for (uint32_t i0 = 0; i0 < ns && n <= t.cap; i0 += 32) {
+        uint32_t slots = 0, found = 0;
+        const uint32_t share = i0 + lane < ns ? work[i0 + lane] : 0;
+        if (i0 + lane < ns)
+          for (uint32_t q = 0; q < per; ++q) slots |= half_key(mx.m[q * 256 + share]) >= tv >> 16 ? 1u << q : 0u;
+        __syncwarp();
+        each_bit(slots, found, [&](uint32_t q, uint32_t at) { list[at] = (uint16_t)(q * 256 + share); });
+        __syncwarp();
+        look_at(found * (4u << mx.shift));
+      }
+    } else {
+      look_at(ns << wide);
     }
     each_bit(sc != kNoClass && reaches(single) ? 1u : 0u, n, [&](uint32_t, uint32_t to) {
       if (to < t.cap) t.cand[to] = key_of(single, sc);
     });
+    __syncwarp();
     if (n <= t.cap) {
       if (strict && n < k) add_equal<T>(t, b, x, bound, k - n, n);
       sort_candidates(t, n, k);
       return;
     }
+    const uint32_t higher = (uint32_t)(kth_candidate(t, t.cap, k) >> 32);
+    strict = !strict && higher == tv;
+    tv = higher;
     __syncwarp();
   }
   rounds<32, T>(g, t, x, 1, b.begin(), b.end(), k);
@@ -788,7 +801,8 @@ static int launch_rows(const LogprobP& p, cudaStream_t s) {
     const RingPlan plan = ring_plan<T, W, BWD>(p.x.C, [&](uint32_t) { return besides; });
     if (stream_worth<W>(p.x.rows, plan.parts)) {
       static StreamLaunch shared;
-      return launch_stream(logprob_stream<T, ENT, RANK, TOP, BWD>, shared, Crew<W>::kThreads + (TOP ? 32 : 0), p.x.rows, plan.parts, plan.bytes + besides, s, p, plan);
+      const int rc = launch_stream(logprob_stream<T, ENT, RANK, TOP, BWD>, shared, Crew<W>::kThreads + (TOP ? 32 : 0), p.x.rows, plan.parts, plan.bytes + besides, s, p, plan);
+      if (rc != AD_ERR_UNSUPPORTED) return rc;
     }
   }
   auto kernel = logprob_rows<NT, T, ENT, RANK, TOP, BWD>;

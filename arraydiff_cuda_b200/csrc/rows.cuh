@@ -642,9 +642,9 @@ inline int launch_stream(void (*kernel)(P...), StreamLaunch& l, uint32_t threads
   unsigned long long held = __atomic_load_n(&l.held[i], __ATOMIC_RELAXED);
   if (held >> 32 != smem) {
     int n = 0;
-    if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n < 1) {
+    if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n < 1) {   // part of a GPU: the other kernels serve it
       cudaGetLastError();
-      return AD_ERR_CUDA;
+      return AD_ERR_UNSUPPORTED;
     }
     held = (unsigned long long)smem << 32 | (unsigned)n;
     __atomic_store_n(&l.held[i], held, __ATOMIC_RELAXED);

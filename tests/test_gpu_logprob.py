@@ -414,3 +414,20 @@ def test_gradients_captured_with_clusters_and_on_two_streams():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(g, w[0]) and torch.equal(lse, w[1])
+
+
+@pytest.mark.parametrize("rows,Cc,dtype,V", [(448, 140000, "bf16", 8), (446, 140000, "f32", 4), (3, 140000, "bf16", 8), (1200, 16000, "bf16", 8)])
+def test_top_of_rows_whose_large_classes_share_a_thread(rows, Cc, dtype, V):
+    """Hundreds of large classes, different and equal, in the vectors that one thread or lane takes"""
+    x = R.logits(3, rows, Cc, dtype, 0.5)
+    mine = (np.arange(Cc) // V) % 256
+    g = H.rng(9)
+    for i in range(min(rows, 3)):
+        at = np.flatnonzero((mine == 5) | (mine == 77 + i))
+        x[i, at] = 30 + g.normal(size=len(at)) * (3.0 if i < 2 else 0.0)   # the third: all alike
+    x = R.rounded(x, dtype)
+    lab = labels(4, x)
+    some = np.arange(min(rows, 6))
+    for k in (1, 5, 12, 33):
+        got = fwd(x, lab, dtype, rows, 1, NHWC, k)
+        check_fwd(x[some], lab[some], {n: v[some] for n, v in got.items()}, 1.0, k, False)
