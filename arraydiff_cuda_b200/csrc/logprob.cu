@@ -108,11 +108,11 @@ __device__ __forceinline__ void sort_candidates(const TopMem& t, uint32_t n, uin
   }
 }
 // One warp: the k-th of n candidates, bit by bit; 0: fewer
-__device__ __forceinline__ Key kth_candidate(const TopMem& t, uint32_t n, uint32_t k) {
+__device__ __noinline__ Key kth_candidate(const Key* cand, uint32_t n, uint32_t k) {
   Key least = 0;
   for (Key bit = 1ull << 63; bit; bit >>= 1) {
     uint32_t m = 0;
-    for (uint32_t i = threadIdx.x & 31; i < n; i += 32) m += t.cand[i] >= (least | bit);
+    for (uint32_t i = threadIdx.x & 31; i < n; i += 32) m += cand[i] >= (least | bit);
     if (__reduce_add_sync(0xffffffffu, m) >= k) least |= bit;
   }
   return least;
@@ -125,7 +125,7 @@ __device__ void sort_candidates(const TopMem& t, uint32_t n, uint32_t k) {
     sort_candidates<1>(t, n, k, 0);
   } else {
     if (n > 64 + 2 * k) {   // many equal or clustered ones: the k-th first, and only those up to it
-      least = kth_candidate(t, n, k);
+      least = kth_candidate(t.cand, n, k);
       uint32_t kept = 0;
       for (uint32_t i0 = 0; i0 < n; i0 += 32) {
         const Key key = i0 + lane < n ? t.cand[i0 + lane] : 0;
@@ -182,17 +182,17 @@ __device__ void select_top(const TopMem& t, uint32_t k, const uint32_t (&kv)[8],
   constexpr int V = X::V;
   Group<32> g(nullptr);
   const uint32_t lane = g.tid;
-  uint32_t tv = kth_share<X::kKeyShift>(kv, k);
+  uint32_t lo = kth_share<X::kKeyShift>(kv, k);
   const uint32_t nv = b.ve - b.vb, per = mx.m ? mx.slots : (nv + 255) / 256;
   // All elements of the shares that reach the bound.  Where there is no room for them the bound rises to the k-th of those
-  // found so far; where it cannot, because so many equal it, only those above it are taken, and of the equal ones the first.
+  // found so far; where it is that one already, because so many equal it, only those above are taken, and of the equal ones the first.
   bool strict = false;
   for (int tries = 0; tries < 64; ++tries) {
-    const float bound = tv ? key_value(tv) : -INFINITY;
-    auto reaches = [&](float v) { return strict ? v > bound : v >= bound; };
+    const float bound = lo ? key_value(lo) : -INFINITY;
+    auto reaches = [&](float v) { return v >= bound; };
     uint32_t ns = 0, n = 0, mine = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) mine |= kv[i] && (strict ? kv[i] > tv : kv[i] >= tv) ? 1u << i : 0u;
+    for (int i = 0; i < 8; ++i) mine |= kv[i] && kv[i] >= lo ? 1u << i : 0u;
     each_bit(mine, ns, [&](uint32_t i, uint32_t at) { work[at] = (uint16_t)(i * 32 + lane); });
     __syncwarp();
     const uint32_t wide = per <= 1 ? 0 : 32 - __clz(per - 1);   // a share's vectors as a power of two
@@ -230,43 +230,40 @@ __device__ void select_top(const TopMem& t, uint32_t k, const uint32_t (&kv)[8],
         });
       }
     };
-    auto look_at = [&](uint32_t vectors) {
-      for (uint32_t i0 = 0; i0 < vectors && n <= t.cap;) {
-        if (vectors - i0 <= 32) {
-          look(Loads<1>(), i0, vectors);
-          i0 += 32;
-        } else {
-          look(Loads<4>(), i0, vectors);
-          i0 += 128;
-        }
-      }
-    };
-    if (mx.m) {   // the slots that reach it, of 32 shares at a time
-      for (uint32_t i0 = 0; i0 < ns && n <= t.cap; i0 += 32) {
+    for (uint32_t i0 = 0; i0 < ns && n <= t.cap; i0 += mx.m ? 32 : 256) {
+      uint32_t vectors = ns << wide;
+      if (mx.m) {   // the slots that reach it, of 32 shares at a time
         uint32_t slots = 0, found = 0;
         const uint32_t share = i0 + lane < ns ? work[i0 + lane] : 0;
         if (i0 + lane < ns)
-          for (uint32_t q = 0; q < per; ++q) slots |= half_key(mx.m[q * 256 + share]) >= tv >> 16 ? 1u << q : 0u;
-        __syncwarp();
+          for (uint32_t q = 0; q < per; ++q) slots |= half_key(mx.m[q * 256 + share]) >= lo >> 16 ? 1u << q : 0u;
+        if (i0) __syncwarp();
         each_bit(slots, found, [&](uint32_t q, uint32_t at) { list[at] = (uint16_t)(q * 256 + share); });
         __syncwarp();
-        look_at(found * (4u << mx.shift));
+        vectors = found * (4u << mx.shift);
       }
-    } else {
-      look_at(ns << wide);
+      for (uint32_t j0 = 0; j0 < vectors && n <= t.cap;) {
+        if (vectors - j0 <= 32) {
+          look(Loads<1>(), j0, vectors);
+          j0 += 32;
+        } else {
+          look(Loads<4>(), j0, vectors);
+          j0 += 128;
+        }
+      }
     }
     each_bit(sc != kNoClass && reaches(single) ? 1u : 0u, n, [&](uint32_t, uint32_t to) {
       if (to < t.cap) t.cand[to] = key_of(single, sc);
     });
     __syncwarp();
     if (n <= t.cap) {
-      if (strict && n < k) add_equal<T>(t, b, x, bound, k - n, n);
+      if (strict && n < k) add_equal<T>(t, b, x, key_value(lo - 1), k - n, n);
       sort_candidates(t, n, k);
       return;
     }
-    const uint32_t higher = (uint32_t)(kth_candidate(t, t.cap, k) >> 32);
-    strict = !strict && higher == tv;
-    tv = higher;
+    const uint32_t higher = (uint32_t)(kth_candidate(t.cand, t.cap, k) >> 32);
+    strict = higher == lo;
+    lo = higher + strict;
     __syncwarp();
   }
   rounds<32, T>(g, t, x, 1, b.begin(), b.end(), k);
