@@ -670,7 +670,6 @@ static int distill_args(const ad_distill_args* a, bool bwd, DistillP& p) {
   return AD_OK;
 }
 
-
 template <int NT, typename T, bool REST, bool BWD>
 static int launch_rows(const DistillP& p, uint32_t n, size_t mask, cudaStream_t s) {
   if constexpr (NT != 32) {

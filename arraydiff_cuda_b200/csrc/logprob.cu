@@ -3,13 +3,13 @@
 // Forward: bytes of the logits, read once.  The top classes come out of the same pass: the row is dealt out in 256 shares
 // (a block's threads, or eight per lane of a warp), each share keeps its largest value, and the k-th of these 256 bounds
 // the row's k-th class from below.  Only the shares that reach it, or the batches of theirs that do, are looked at again.
-// Equal values go by class: where more reach the bound than there is room for, those above it and the first equal ones.
+// Where more reach the bound than there is room for it rises; equal values go by class: those above it and the first equal ones.
 // Backward: the sums as in the forward pass, then the row once more (out of shared memory or the L2) for the gradient.
 //
 // 4001 x 50001 bf16 (400 MB, 62 us at the copy rate): log-sum-exp 71 us, with the entropy 75, the rank 77, 8 alternatives
-// 78; all of them 100, bound by instructions (70 M, 69 % of the issue slots).  2000 x 100000 fp32 (124): 126.  Gradient of 4096 x
+// 78; all of them 96, bound by instructions (70 M, 69 % of the issue slots).  2000 x 100000 fp32 (124): 126.  Gradient of 4096 x
 // 32000 bf16 (81): 109, with the entropy's 114: two exponentials per element (57 us of the special units) and a meeting of the
-// block's warps between the passes.  64 x 131072 with 20 alternatives: 18, one row of 32768 with 5: 8, both by the
+// block's warps between the passes.  64 x 131072 with 20 alternatives: 16, one row of 32768 with 5: 8, both by the
 // latency of label, loads, sums, selection and a cluster's meeting, one behind the other.
 #include <cooperative_groups.h>
 
@@ -779,7 +779,6 @@ static int logprob_args(const ad_logprob_args* a, bool bwd, LogprobP& p) {
   }
   return AD_OK;
 }
-
 
 template <typename T, bool BWD>
 static int launch_any(const LogprobP& p, cudaStream_t s) {

@@ -659,7 +659,7 @@ inline int launch_stream(void (*kernel)(P...), StreamLaunch& l, uint32_t threads
 // Plain loops over a row in any layout: what the fast pass does not serve
 template <int NT, typename T, bool ENT>
 __device__ void plain_sums(Group<NT>& g, const T* x, int64_t st, uint32_t C, float cs, RowSums& s, float& E) {
-    float m = -INFINITY, S = 0.f;
+  float m = -INFINITY, S = 0.f;
   for (uint32_t c = g.tid; c < C; c += NT) m = fmaxf(m, ld_f(x + c * st));
   m = g.max(m);
   if (m == -INFINITY) m = 0.f;
