@@ -365,3 +365,20 @@ def test_very_many_classes(rows, Cc, dtype):
     got_loss, got = call(x, dtype, rows, 1, NHWC, cls, t, "bwd", rest=1, dloss=dloss)
     check_loss(got_loss[some], loss, lmag, tol, k)
     check_grad(got[some], grad, gmag, dloss[some], tol, dtype)
+
+
+@pytest.mark.parametrize("Cc,pitch,gpitch", [(3, 2 ** 30 - 1, 0), (2, 2 ** 30 + 3, 0), (2, 0, 2 ** 30 + 3)])
+def test_planes_four_gigabytes_apart(Cc, pitch, gpitch):
+    """Class strides in bytes on either side of 2^32, of the logits and of the gradient"""
+    import torch
+    x = R.logits(61, 5, Cc, "f32")
+    cls, t = teacher(62, x, 2, 0, odd=False)
+    loss, lmag, grad, gmag = R.distill(x, 0.8, cls, t, 1.0, 0)
+    tol = tolerances(x, t, 0.8, 1.0, True)
+    dloss = np.linspace(0.5, 2, 5).astype(np.float32)
+    try:
+        got_loss, got = call(x, "f32", 1, 5, NCHW, cls, t, "bwd", scale=0.8, pitch=pitch, gpitch=gpitch, dloss=dloss)
+        check_loss(got_loss, loss, lmag, tol, 2)
+        check_grad(got, grad, gmag, dloss, tol, "f32")
+    finally:
+        torch.cuda.empty_cache()

@@ -431,3 +431,20 @@ def test_top_of_rows_whose_large_classes_share_a_thread(rows, Cc, dtype, V):
     for k in (1, 5, 12, 33):
         got = fwd(x, lab, dtype, rows, 1, NHWC, k)
         check_fwd(x[some], lab[some], {n: v[some] for n, v in got.items()}, 1.0, k, False)
+
+
+@pytest.mark.parametrize("Cc,pitch,gpitch", [(3, 2 ** 30 - 1, 0), (2, 2 ** 30 + 3, 0), (2, 0, 2 ** 30 + 3)])
+def test_planes_four_gigabytes_apart(Cc, pitch, gpitch):
+    """Class strides in bytes on either side of 2^32, of the logits and of the gradient"""
+    import torch
+    x = R.logits(51, 5, Cc, "f32")
+    lab = np.array([0, 1, Cc - 1, R.NO_CLASS, 1], np.uint32)
+    d3 = factors(52, 5)
+    try:
+        if pitch:
+            check_fwd(x, lab, fwd(x, lab, "f32", 1, 5, NCHW, 2, 0.9, pitch), 0.9, 2, True)
+            torch.cuda.empty_cache()
+        got, _ = bwd(x, lab, "f32", 1, 5, NCHW, d3, 0.9, pitch, gpitch)
+        check_bwd(x, lab, got, d3, "f32", 0.9, True)
+    finally:
+        torch.cuda.empty_cache()
