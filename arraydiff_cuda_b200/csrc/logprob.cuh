@@ -71,7 +71,8 @@ struct Factors {
   template <bool ENT> __device__ float grad(float x, float cs, float mc) const {
     float u = fmaf(x, cs, -mc);
     if (ENT) u = above_nothing(u);
-    return exp2_fast(u) * (ENT ? fmaf(c1, u, c0) : c0);
+    const float e = exp2_fast(u);
+    return ENT ? entropy_grad(e, u, c0, c1) : e * c0;
   }
 };
 

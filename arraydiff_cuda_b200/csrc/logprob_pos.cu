@@ -125,7 +125,8 @@ __device__ __noinline__ void plain_gradient(const LogprobP& p, P x, P o, P old, 
   for (uint32_t c = 0; c < x.C; ++c) {
     float u = (x.get(c) - s.m) * p.cs;
     if (ENT) u = above_nothing(u);
-    float g = exp2_fast(u) * (ENT ? fmaf(f.c1, u, f.c0) : f.c0);
+    const float e = exp2_fast(u);
+    float g = ENT ? entropy_grad(e, u, f.c0, f.c1) : e * f.c0;
     if (c == l) g += f.dl;
     o.set(c, p.accumulate ? g + old.get(c) : g);
   }
@@ -251,7 +252,8 @@ __global__ void __launch_bounds__(kPositions) logprob_few_bwd(const __grid_const
             q.y = above_nothing(q.y);
             z = pair(q.x, q.y);
           }
-          const float2 g = halves(mul2(pair(exp2_fast(q.x), exp2_fast(q.y)), ENT ? fma2(z, c1, c0) : c0));
+          const F2 e = pair(exp2_fast(q.x), exp2_fast(q.y));
+          const float2 g = halves(ENT ? entropy_grad(e, z, c0, c1) : mul2(e, c0));
           v[c] = g.x;
           v[c + 1] = g.y;
         }
@@ -475,7 +477,8 @@ __global__ void __launch_bounds__(kPositions, 10) logprob_positions_grad(const _
               q.y = above_nothing(q.y);
               z = pair(q.x, q.y);
             }
-            const float2 g = halves(mul2(pair(exp2_fast(q.x), exp2_fast(q.y)), ENT ? fma2(z, c1, c0) : c0));
+            const F2 e = pair(exp2_fast(q.x), exp2_fast(q.y));
+            const float2 g = halves(ENT ? entropy_grad(e, z, c0, c1) : mul2(e, c0));
             h[i] = g.x;
             h[i + 1] = g.y;
           }

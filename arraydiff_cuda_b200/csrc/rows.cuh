@@ -335,7 +335,11 @@ __device__ __forceinline__ void add_vectors(Part& a, const uint4 (&w)[U], int n,
     a.E += e.x + e.y;
   }
 }
-// The gradient of a vector's elements.  e (c0 + c1 u) with e = 2^u; without ENT c0 e.
+// The gradient of an element, e (c0 + c1 u) with e = 2^u: u meets the exponential first, which is 0 where u stands for something
+// masked.  c1, the size of the caller's factors, would make it infinite, and 0 times that NaN.
+__device__ __forceinline__ float entropy_grad(float e, float u, float c0, float c1) { return fmaf(__fmul_rn(e, u), c1, __fmul_rn(e, c0)); }
+__device__ __forceinline__ F2 entropy_grad(F2 e, F2 u, F2 c0, F2 c1) { return fma2(mul2(e, u), c1, mul2(e, c0)); }
+// ... of a vector's elements; without ENT c0 e
 template <bool ENT, typename T>
 __device__ __forceinline__ void grad_vector(uint4 w, float (&h)[Vec<T>::V], float cs, float mc, float c0, float c1, float nothing) {
   float f[Vec<T>::V];
@@ -345,7 +349,7 @@ __device__ __forceinline__ void grad_vector(uint4 w, float (&h)[Vec<T>::V], floa
     const F2 z = fma2(pair(f[i], f[i + 1]), pair(cs, cs), pair(-mc, -mc));
     const float2 q = halves(z);
     const F2 e = pair(exp2_fast(q.x), exp2_fast(q.y));
-    const float2 g = halves(mul2(e, ENT ? fma2(z, pair(c1, c1), pair(c0, c0)) : pair(c0, c0)));
+    const float2 g = halves(ENT ? entropy_grad(e, z, pair(c0, c0), pair(c1, c1)) : mul2(e, pair(c0, c0)));
     h[i] = g.x;
     h[i + 1] = g.y;
   }
