@@ -11,6 +11,7 @@
 // A row of -inf has S = 0, which is how it is recognised.
 #pragma once
 
+#include "cluster_counts.h"
 #include "common.cuh"
 
 namespace adk {
@@ -612,11 +613,11 @@ inline RingPlan ring_plan(uint32_t C, F&& besides) {
   p.bytes = (size_t)p.slots * Str::kBytes;
   return p;
 }
-// What the launches of one kernel share: on which devices (a bit each) its limit is raised, and how many clusters of a size
-// (1, 2, 4, 8 blocks) and of blocks of so much shared memory (KB) the machine holds at a time, as last asked
+// What the launches of one kernel share: on which devices (a bit each) its limit is raised, and how many clusters of each shape
+// a device holds at a time
 struct StreamLaunch {
   unsigned raised;
-  unsigned long long held[4];   // shared memory << 32 | clusters
+  ClusterCounts held;
 };
 constexpr size_t kMostRing = 218 * 1024;   // dynamic shared memory of the blocks that stay
 template <typename... P, typename... A>
@@ -642,18 +643,17 @@ inline int launch_stream(void (*kernel)(P...), StreamLaunch& l, uint32_t threads
   cfg.attrs = at;
   cfg.numAttrs = 1;
   // as many clusters as are resident together, which is less than three blocks per SM: a cluster stays within one group of SMs
-  const int i = parts == 1 ? 0 : parts == 2 ? 1 : parts == 4 ? 2 : 3;
-  unsigned long long held = __atomic_load_n(&l.held[i], __ATOMIC_RELAXED);
-  if (held >> 32 != smem) {
-    int n = 0;
-    if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n < 1) {   // part of a GPU: the other kernels serve it
+  const uint32_t shape = ClusterCounts::key(dev, parts, smem);
+  size_t n = l.held.find(shape);
+  if (n == 0) {
+    int most = 0;
+    if (cudaOccupancyMaxActiveClusters(&most, kernel, &cfg) != cudaSuccess || most < 1) {   // part of a GPU: the other kernels serve it
       cudaGetLastError();
       return AD_ERR_UNSUPPORTED;
     }
-    held = (unsigned long long)smem << 32 | (unsigned)n;
-    __atomic_store_n(&l.held[i], held, __ATOMIC_RELAXED);
+    n = (uint32_t)most;
+    l.held.keep(shape, (uint32_t)most);
   }
-  const size_t n = (uint32_t)held;
   cfg.gridDim = (unsigned)((rows < n ? rows : n) * parts);
   launch_attr(cfg, at);
   cudaLaunchKernelEx(&cfg, kernel, P(args)...);   // an error is what launch_status() returns
