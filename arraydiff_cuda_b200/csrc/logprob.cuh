@@ -49,7 +49,7 @@ __device__ __forceinline__ void put_top(const LogprobP& p, const RowSums& s, siz
 }
 __device__ __forceinline__ void put_row(const LogprobP& p, const RowSums& s, size_t r, float H, uint32_t l, float xl) {
   if (p.lse) p.lse[r] = s.lse(p.scale);
-  if (p.entropy) p.entropy[r] = H;
+  if (p.entropy) p.entropy[r] = H < 0.f ? 0.f : H;   // by the rounding of log S and of E / S, where a row is nearly certain
   if (p.logp) p.logp[r] = l < p.x.C ? s.log_p(xl, p.scale) : 0.f;
 }
 

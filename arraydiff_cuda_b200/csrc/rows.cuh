@@ -99,6 +99,13 @@ __device__ __forceinline__ float above_nothing(float v) {
   return r;
 }
 
+// v, not above w, and NaN where v is
+__device__ __forceinline__ float not_above(float v, float w) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(v), "f"(w));
+  return r;
+}
+
 // In front of: the larger value, then the lower class
 __device__ __forceinline__ bool in_front(float v, uint32_t c, float w, uint32_t d) { return v > w || (v == w && c < d); }
 // The same order as whole numbers.  -0 and 0 are one value.
@@ -382,7 +389,10 @@ struct RowSums {
     L = some ? log2f(S) : 0.f;
     low = some ? L + fmaf(-m, cs, mc) : 0.f;
   }
-  __device__ float log_p(float x, float scale) const { return some ? fmaf(-kLn2, low, __fmul_rn(x - m, scale)) : -INFINITY; }
+  // The sum of a nearly certain row may be rounded to less than its largest term: no log probability is above 0 all the same
+  __device__ float log_p(float x, float scale) const {
+    return not_above(some ? fmaf(-kLn2, low, __fmul_rn(x - m, scale)) : -INFINITY, 0.f);
+  }
   __device__ float entropy(float E) const { return some ? __fmul_rn(kLn2, L - __fdiv_rn(E, S)) : 0.f; }
   __device__ float lse(float scale) const { return some ? fmaf(kLn2, low, __fmul_rn(m, scale)) : -INFINITY; }
 };

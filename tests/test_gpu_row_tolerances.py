@@ -186,3 +186,20 @@ def test_entropy_of_nearly_certain_rows(rows, Cc, layout):
     _, _, p, _ = R.softmax_rows(x)
     got, _ = bwd(x, lab, "f32", N, HW, layout, d3)
     R.check_close(got, dwant, gradient_bound(dwant, mag, p, bounds(x, np.ones(x.shape, bool), 1.0, n), n, 1.0, d3, want["entropy"], "f32"), "dlogits")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,Cc,layout", FORMS + [(300, 31, NHWC), (300, 32, NCHW), (1200, 5000, NHWC)])
+def test_signs_of_nearly_certain_rows(rows, Cc, layout, dtype):
+    """An entropy is not below 0 and a log probability not above it, whatever the rounding of the sums that they come from"""
+    x = H.normal(7, (rows, Cc), 1.0)
+    at = H.rng(Cc).integers(0, Cc, rows)
+    x[np.arange(rows), at] = (x.max(1) + np.linspace(13, 40, rows)).astype(np.float32)
+    one = np.arange(rows) % 4 == 3
+    x[one] = np.where(np.arange(Cc) == at[one, None], x[one], -np.inf)
+    N, HW = (1, rows) if layout == NCHW else (rows, 1)
+    for scale in (1.0, 0.83):
+        got = fwd(R.rounded(x, dtype), at.astype(np.uint32), dtype, N, HW, layout, 2, scale)
+        assert (got["entropy"] >= 0).all() and (got["logp"] <= 0).all() and (got["top_logp"] <= 0).all()
+        _, outs = bwd(R.rounded(x, dtype), at.astype(np.uint32), dtype, N, HW, layout, (np.ones(rows), None, None), scale)
+        assert (outs["entropy"] >= 0).all() and (outs["logp"] <= 0).all()
