@@ -698,8 +698,11 @@ static int launch_rows(const DistillP& p, uint32_t n, size_t mask, cudaStream_t 
 template <typename T, bool BWD>
 static int launch_distill(const DistillP& p, cudaStream_t s) {
   const size_t vectors = p.x.C / Vec<T>::V;
-  const uint32_t n = row_parts(p.x.rows, (size_t)p.x.C * sizeof(T));
-  const size_t mask = p.rest ? (vectors / n + 17) / 16 * 16 : 0;
+  uint32_t n = row_parts(p.x.rows, (size_t)p.x.C * sizeof(T));
+  auto mask_of = [&](uint32_t parts) { return p.rest ? (vectors / parts + 17) / 16 * 16 : (size_t)0; };
+  // blocks enough to hold the row's mask: element by element 450 x 600001 fp32 took 23 ms and its gradient 32
+  while (n < 8 && mask_of(n) > kMostMask) n *= 2;
+  const size_t mask = mask_of(n);
   int rc = distill_positions<T, BWD>(p, s);
   if (rc != AD_ERR_UNSUPPORTED) {   // a thread per position
   } else if (p.x.step != 1 || (BWD && p.g.step != 1) || mask > kMostMask) {
