@@ -454,7 +454,8 @@ __global__ void __launch_bounds__(256, NT == 32 ? (TOP ? 2 : 4) : 3) logprob_row
     } else if (TOP) {
       g.sync();
     }
-    if (a.strange(p.cs)) {
+    const bool far = !BWD && a.far(p.cs);
+    if (a.strange(p.cs) && !far) {
       if (parts_n > 1) cluster.sync();   // the others' sums have been read
       if (part == 0) plain_row<NT, T, BWD>(g, p, r, t);
       if (parts_n > 1) cluster.sync();
@@ -462,7 +463,8 @@ __global__ void __launch_bounds__(256, NT == 32 ? (TOP ? 2 : 4) : 3) logprob_row
       continue;
     }
     RowSums s;
-    s.set(a.m, a.mc, a.S, p.cs);
+    if (far) plain_sums<NT, T, ENT>(g, x, 1, C, p.cs, s, a.E);   // list and rank stand; each block of a cluster for itself
+    else s.set(a.m, a.mc, a.S, p.cs);
     const float H = s.entropy(a.E);
     if (g.tid == 0 && part == 0) {
       put_row(p, s, r, H, label.l, label.xl);
@@ -698,9 +700,14 @@ __global__ void __launch_bounds__(Crew<8>::kThreads + (TOP ? 32 : 0), Crew<8>::k
         if (lane % 8 < parts) a = *cluster.map_shared_rank(&whole[i & 1], lane % 8);
         a.join<ENT, 8>(p.cs);
       }
-      const bool strange = a.strange(p.cs);
+      const bool far = !BWD && a.far(p.cs), strange = !far && a.strange(p.cs);
       RowSums s;
-      s.set(a.m, a.mc, a.S, p.cs);
+      if (far) {   // list and rank stand
+        Group<32> g(nullptr);
+        plain_sums<32, T, ENT>(g, x, 1, p.x.C, p.cs, s, a.E);
+      } else {
+        s.set(a.m, a.mc, a.S, p.cs);
+      }
       const float H = s.entropy(a.E);
       if constexpr (BWD) {
         Factors f = now.f;

@@ -310,7 +310,9 @@ struct Part {
     }
   }
   // not for the fast pass: beyond the range of its products, or not a number
-  __device__ bool strange(float cs) const { return S != S || (fabsf(m * cs) > kFar && m != -INFINITY); }
+  __device__ bool strange(float cs) const { return S != S || far(cs); }
+  // beyond the range, and no NaN or +inf among the elements (their S is NaN): only the sums are to be done again
+  __device__ bool far(float cs) const { return S == S && fabsf(m * cs) > kFar && m != -INFINITY; }
 };
 
 // The vectors w[0..U) of a thread, of which bm is the largest element, into its share.  ENT: `nothing`, a number whose product

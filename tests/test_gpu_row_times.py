@@ -50,3 +50,30 @@ def test_distillation_whose_mask_no_block_holds():
         torch.cuda.empty_cache()
     for few, many in zip(*times.values()):
         assert many < 6 * few, times
+
+
+@pytest.mark.parametrize("rows", [8, 2001])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_a_padded_row_among_others(rows, dtype):
+    """One row of the type's lowest value, of a batch with long lists: its sums are done again, its list and its rank are not"""
+    import torch
+    Cc, k, at = 50_001, 128, rows // 2
+    T = torch.bfloat16 if dtype == "bf16" else torch.float32
+    x = torch.randn((rows, Cc), device="cuda").mul_(2.5).to(T)
+    lab = torch.full((rows,), 77, dtype=torch.int32, device="cuda")
+    lse, ent, logp = (torch.empty(rows, device="cuda") for _ in range(3))
+    rank, cls = torch.empty(rows, dtype=torch.int32, device="cuda"), torch.empty((rows, k), dtype=torch.int32, device="cuda")
+    top = torch.empty((rows, k), device="cuda")
+    a = abi.LogprobArgs(R.dtype_of(dtype), abi.AD_NHWC, rows, Cc, 1, 1.0, x.data_ptr(), 0, lab.data_ptr(), lse.data_ptr(), ent.data_ptr(), logp.data_ptr(), rank.data_ptr(), k)
+    a.top_class, a.top_logp = cls.data_ptr(), top.data_ptr()
+    call = lambda: abi.check(abi.lib().ad_logprob_fwd(C.byref(a), H.stream()))
+    ordinary = least(call)
+    x[at] = torch.finfo(T).min
+    padded = least(call)
+    assert rank[at].item() == 77 and (cls[at] == torch.arange(k, device="cuda")).all()
+    np.testing.assert_allclose([ent[at].item(), -logp[at].item()] + (-top[at]).tolist(), np.log(Cc), rtol=1e-6)
+    x[at, 40_000], x[at, 77] = -1e9, -1e30               # some above the others
+    call()
+    H.sync()
+    assert rank[at].item() == 1 and cls[at, :3].tolist() == [40_000, 77, 0] and ent[at].item() == 0 and top[at, 0].item() == 0
+    assert padded < 6 * ordinary, (ordinary, padded)
