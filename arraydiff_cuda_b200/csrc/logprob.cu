@@ -454,7 +454,7 @@ __global__ void __launch_bounds__(256, NT == 32 ? (TOP ? 2 : 4) : 3) logprob_row
     } else if (TOP) {
       g.sync();
     }
-    const bool far = !BWD && a.far(p.cs);
+    const bool far = TOP && a.far(p.cs);   // without a list plain_row() costs one pass more, and its place here registers
     if (a.strange(p.cs) && !far) {
       if (parts_n > 1) cluster.sync();   // the others' sums have been read
       if (part == 0) plain_row<NT, T, BWD>(g, p, r, t);
@@ -700,7 +700,7 @@ __global__ void __launch_bounds__(Crew<8>::kThreads + (TOP ? 32 : 0), Crew<8>::k
         if (lane % 8 < parts) a = *cluster.map_shared_rank(&whole[i & 1], lane % 8);
         a.join<ENT, 8>(p.cs);
       }
-      const bool far = !BWD && a.far(p.cs), strange = !far && a.strange(p.cs);
+      const bool far = TOP && a.far(p.cs), strange = !far && a.strange(p.cs);
       RowSums s;
       if (far) {   // list and rank stand
         Group<32> g(nullptr);
