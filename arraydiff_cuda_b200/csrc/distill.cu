@@ -6,9 +6,10 @@
 // out (a byte of mask per vector in shared memory) and sums the others alone, against their own maximum: p_r is then exact
 // however little of the row it is, and the row's sum is theirs and that of the list, each class of it once.
 //
-// 4096 x 65536 bf16 (537 MB, 83 us at the copy rate): loss 86 to 102 us for lists of 1 to 128 classes.  Gradient (166): 221 with
-// one class, 238 with 64 and the rest; 1001 x 50001 fp32 (62): 95; 2048 x 32000 bf16 (41): 63.  Two exponentials per
-// element (119 us of the special units for the first) and the second pass's way through shared memory beside the copies.
+// 4096 x 65536 bf16 (537 MB, 83 us at the copy rate): loss with the rest 89 to 109 us for lists of 1 to 128 classes.  Gradient (166):
+// 221 with one class, 235 to 240 with 64 and the rest; 1001 x 50001 fp32 (62): 96; 2048 x 32000 bf16 (41) with 16 classes: 64, with
+// the rest 72.  Two exponentials per element (119 us of the special units for the first) and the second pass's way through
+// shared memory beside the copies.
 #include <cooperative_groups.h>
 
 #include "distill.cuh"

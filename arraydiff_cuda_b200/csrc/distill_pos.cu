@@ -3,8 +3,9 @@
 // Up to 32 classes and eight entries: the rows of 128 positions in shared memory, a thread's row and list in registers, the
 // gradient back into the tile, where the entries' classes are written over it, and out by vectors; planes as they lie (1,048,576
 // positions of 19 fp32 classes: 55 us, from memory class by class 97).  2,097,152 pixels of 19 bf16
-// classes with four entries each (243 MB, 38 us at the copy rate): 96 us, by instructions (1080 per 32 pixels) and 42 % of the warps;
-// with the lists read from memory wherever they are needed it took 142.
+// classes with four entries each (243 MB, 38 us at the copy rate): 96 us, 61 of it instructions (1080 per 32 pixels), the rest latency
+// at 42 % of the warps; with the lists read from memory wherever they are needed it took 142.  72 registers hold 20 classes and four
+// entries; more spill (32 classes and eight entries 316 to 372 bytes: 1,048,576 positions in 104 us, with four entries in 60).
 #include "distill.cuh"
 
 namespace adk {

@@ -6,11 +6,12 @@
 // Where more reach the bound than there is room for it rises; equal values go by class: those above it and the first equal ones.
 // Backward: the sums as in the forward pass, then the row once more (out of shared memory or the L2) for the gradient.
 //
-// 4001 x 50001 bf16 (400 MB, 62 us at the copy rate): log-sum-exp 71 us, with the entropy 75, the rank 77, 8 alternatives
-// 78; all of them 96, bound by instructions (70 M, 69 % of the issue slots).  2000 x 100000 fp32 (124): 126.  Gradient of 4096 x
-// 32000 bf16 (81): 109, with the entropy's 114: two exponentials per element (57 us of the special units) and a meeting of the
-// block's warps between the passes.  64 x 131072 with 20 alternatives: 16, one row of 32768 with 5: 8, both by the
-// latency of label, loads, sums, selection and a cluster's meeting, one behind the other.
+// 4001 x 50001 bf16 (400 MB, 62 us at the copy rate): log-sum-exp 70 us, with the entropy 74, the rank 81 (labels
+// at random), 8 alternatives 78; all of them 96 where labels are likely, 102 where not, bound by instructions (70 M, 69 % of the issue
+// slots).  2000 x 100000 fp32 (124): 123.  Gradient of 4096 x 32000 bf16 (81): 109, with the entropy's 116: two exponentials per
+// element (57 us of the special units) and a meeting of the block's warps between the passes.  One row of 32768 with 5
+// alternatives: 8, by the latency of label, loads, sums, selection and a cluster's meeting, one behind the other; 64 x 131072 with
+// 20: 16, by that and by four blocks a row, 256 of the 444 that the machine holds.
 #include <cooperative_groups.h>
 
 #include "logprob.cuh"

@@ -4,7 +4,7 @@
 // thread takes its own row into registers; gradients go back into the tile and out by vectors.  Planes are read as they lie,
 // neighbouring threads at neighbouring positions: up to 32 classes into registers, too (1,048,576 positions of 19 fp32 classes, 80
 // MB: log-sum-exp 18 us, by four warps as below 66; gradient 32, 100), of more each of four warps takes a quarter.
-// 4,194,304 pixels of 19 bf16 classes with three alternatives (344 MB, 53 us at the copy rate): 115 us, by instructions (865
+// 4,194,304 pixels of 19 bf16 classes with three alternatives (344 MB, 53 us at the copy rate): 118 us, by instructions (865
 // per 32 pixels: about 20 per class, and as many again for labels, logarithms, lists and stores).  Gradient of 2 x 150 x 256 x 255
 // fp32 planes (157 MB, 24): 41, by the latency of eight loads in flight per thread, ten blocks of an SM.
 #include "logprob.cuh"

@@ -6,7 +6,7 @@
 // where mc - m * cs, the rounding of mc, is what an FMA gives.  One pass over the row: a thread keeps its own maximum,
 // and S and E against it, and rescales them when the maximum of a batch of loads is larger.
 // mc is off by up to 2^-24 of itself, and the terms by 2 to that: a row whose maximum is beyond +-kFar in units of log 2, or
-// that holds +inf or NaN, is done again by plain loops over x_c - m.  A share's reference is at least kFloor, so that
+// that holds +inf or NaN, is done again by plain loops over x_c - m; a list of the former, and its rank, stand.  A share's reference is at least kFloor, so that
 // what is masked (-inf, the type's lowest value, -1e9) adds 2^-4e6 = 0 to the row and never inf or inf - inf.
 // A row of -inf has S = 0, which is how it is recognised.
 #pragma once
@@ -608,7 +608,7 @@ struct RingPlan {
 // besides(parts): bytes of shared memory that a block needs for other things.  Backward: the rows that are in hand together
 // have to stay in the L2 for the second pass, or in the ring where they fit.  444 rows of 200 KB did not (1001 of them read 1.7
 // times, 107 us), 222 rows shared by two blocks each do (95); of 400 KB four blocks each (2000 rows: 401 -> 352 us).  Sharing costs
-// a meeting per row: 444 rows of 131 KB take 223 us unshared (4096 of them) and 232 by twos.
+// a meeting per row: the log probabilities' gradient of 4096 rows of 131 KB takes 221 us unshared and took 232 by twos.
 constexpr size_t kRowsInL2 = 60 << 20;
 template <typename T, int W, bool BWD, typename F>
 inline RingPlan ring_plan(uint32_t C, F&& besides) {
