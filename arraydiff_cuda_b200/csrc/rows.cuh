@@ -6,8 +6,9 @@
 // where mc - m * cs, the rounding of mc, is what an FMA gives.  One pass over the row: a thread keeps its own maximum,
 // and S and E against it, and rescales them when the maximum of a batch of loads is larger.
 // mc is off by up to 2^-24 of itself, and the terms by 2 to that: a row whose maximum is beyond +-kFar in units of log 2, or
-// that holds +inf or NaN, is done again by plain loops over x_c - m; a list of the former, and its rank, stand.  A share's reference is at least kFloor, so that
-// what is masked (-inf, the type's lowest value, -1e9) adds 2^-4e6 = 0 to the row and never inf or inf - inf.
+// that holds +inf or NaN, is done again by plain loops over x_c - m; a list of the former, and its rank, stand.  A share's
+// reference is at least kFloor, so that what is masked (-inf, the type's lowest value, -1e9) adds 2^-4e6 = 0 to the row and never
+// inf or inf - inf.
 // A row of -inf has S = 0, which is how it is recognised.
 #pragma once
 
